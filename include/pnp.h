@@ -510,6 +510,154 @@ int32_t pnp_env_evaluate_f64(pnp_model* model, const pnp_state_f64* state, const
                              const pnp_env_state* env, const double* ag, const double* dg, const pnp_env_out* out,
                              int32_t B, void* stream);
 
+/* ------------------------------------------------------------------ sequence operators
+ * The operators of a policy with memory (pnp_amd/seqops.py, pnp_amd/history.py): the residual's
+ * addition with the RMS norm, the product in 8-bit integers, the short causal convolution and the
+ * selective state space scan, each with its gradient where it trains and its single-token form
+ * where it serves.  Additions to ABI 14: no earlier struct or entry point changes.
+ *
+ * `type` of a tensor: PNP_F32, PNP_BF16 or PNP_F16.  Tensors are device memory of the current
+ * device, the last dimension contiguous; `*_stride` fields are in elements, outputs without one
+ * are contiguous.  Weights, biases, states, statistics and sums are fp32 whatever `type` is.  An
+ * empty batch is PNP_OK and launches nothing.  Workspaces belong to the caller: one call's
+ * workspace is free again when the call's work on its stream is done.  No atomics: the same call
+ * gives the same bits. */
+#define PNP_F32 0
+#define PNP_BF16 1
+#define PNP_F16 2
+
+/* s = x + residual (x alone where residual is NULL), held in res_type; rho = 1 / sqrt(mean(s^2) + eps);
+ * y = s * rho * weight.  rows x dim.  Forward writes s (may be NULL without a residual), rstd = rho
+ * [rows] (may be NULL) and y (type `type`), or, where q is given instead of y, q = rint(y / scale) in
+ * 8 bits with scale = max|y| / 127 per row (0 for a row of zeros; NaN, with q = 0, for a row that holds
+ * NaN or infinity).  weight NULL: ones. */
+typedef struct pnp_norm_desc {
+  int64_t rows;
+  int32_t dim, type, res_type;
+  float eps;
+  const void *x, *residual;
+  int64_t x_stride, r_stride;
+  const float* weight;
+  void *y, *s;
+  float* rstd;
+  int8_t* q;
+  int64_t q_stride;
+  float* scale;
+} pnp_norm_desc;
+int32_t pnp_rms_norm(const pnp_norm_desc* d, void* stream);
+
+/* The gradient: dy (type), ds (res_type, may be NULL: nothing comes back through s), s as the forward
+ * stored it, rstd; dx (type) and, where dres is given, the same values in res_type; dweight [dim] (may
+ * be NULL) from per-workgroup sums in `workspace` (pnp_rms_norm_bwd_workspace floats). */
+typedef struct pnp_norm_bwd_desc {
+  int64_t rows;
+  int32_t dim, type, res_type;
+  const void *dy, *ds, *s;
+  int64_t dy_stride, ds_stride, s_stride;
+  const float *weight, *rstd;
+  void *dx, *dres;
+  float* dweight;
+  float* workspace;
+  int64_t workspace_floats;
+} pnp_norm_bwd_desc;
+int64_t pnp_rms_norm_bwd_workspace(const pnp_norm_bwd_desc* d);
+int32_t pnp_rms_norm_bwd(const pnp_norm_bwd_desc* d, void* stream);
+
+/* Rows of x in 8 bits: scale = max|x| / 127, q = rint(x / scale), as the norm's 8-bit output. */
+int32_t pnp_quantize_rows(const void* x, int64_t x_stride, int32_t type, int64_t rows, int32_t dim, int8_t* q,
+                          int64_t q_stride, float* scale, void* stream);
+
+/* out[m][n] = (sum_k q[m][k] * wq[n][k]) * scale[m] * wscale[n] + bias[n] (bias may be NULL), the sum
+ * in 32-bit integers: exact for K <= 131071. */
+typedef struct pnp_i8_desc {
+  int64_t M;
+  int32_t N, K, out_type, pad;
+  const int8_t *q, *wq;
+  int64_t q_stride, wq_stride;
+  const float *scale, *wscale, *bias;
+  void* out;
+} pnp_i8_desc;
+int32_t pnp_matmul_i8(const pnp_i8_desc* d, void* stream);
+
+/* pre[b][t][d] = bias[d] + sum_{j < W} weight[d][j] * x[b][t - W + 1 + j][d], y = pre (or pre *
+ * sigmoid(pre) where silu).  Tokens before t = 0 come from state [B][W - 1][dim] (type `type`, zeros
+ * where NULL).  starts [B][L] (bytes, may be NULL): a token with a nonzero start begins a sequence, it
+ * and what follows see nothing from before it.  last_state [B][W - 1][dim] (may be NULL): the last
+ * W - 1 tokens of the sequence that goes on, zeros before its start.  W 2, 3 or 4. */
+typedef struct pnp_conv_desc {
+  int64_t B, L;
+  int32_t dim, width, type, silu;
+  const void* x;
+  int64_t x_bstride, x_tstride;
+  const float *weight, *bias;
+  const uint8_t* starts;
+  const void* state;
+  void *y, *last_state;
+} pnp_conv_desc;
+int32_t pnp_causal_conv(const pnp_conv_desc* d, void* stream);
+
+/* The gradient of y and last_state (dlast, may be NULL): dx [B][L][dim], dstate (may be NULL),
+ * dweight [dim][W] and dbias [dim] (either may be NULL). */
+typedef struct pnp_conv_bwd_desc {
+  pnp_conv_desc f;
+  const void *dy, *dlast;
+  int64_t dy_bstride, dy_tstride;
+  void *dx, *dstate;
+  float *dweight, *dbias;
+  float* workspace;
+  int64_t workspace_floats;
+} pnp_conv_bwd_desc;
+int64_t pnp_causal_conv_bwd_workspace(const pnp_conv_bwd_desc* d);
+int32_t pnp_causal_conv_bwd(const pnp_conv_bwd_desc* d, void* stream);
+
+/* One token of each of B sequences: as pnp_causal_conv with L = 1, state advanced in place; reset [B]
+ * (bytes, may be NULL) nonzero: the sequence starts at this token. */
+int32_t pnp_causal_conv_step(const void* x, int64_t x_stride, void* state, const float* weight, const float* bias,
+                             const uint8_t* reset, int64_t B, int32_t dim, int32_t width, int32_t type, int32_t silu,
+                             void* y, void* stream);
+
+/* dt = softplus(delta + delta_bias[d]); a = exp(dt * A[d][n]), 0 where starts[b][t] is nonzero;
+ * h[t] = a * h[t - 1] + dt * u * Bm[b][t][g][n]; y = sum_n Cm[b][t][g][n] * h + D[d] * u;
+ * out = y * z * sigmoid(z) (y where z is NULL).  Channel d belongs to group g = d / (dim / groups).
+ * h before t = 0: state [B][dim][N] (zeros where NULL); last_state the h after the last token.
+ * N 1 .. 64.  ckpt (may be NULL; pnp_scan_ckpt_floats): the states the gradient starts its pieces
+ * from.  workspace (pnp_scan_workspace floats) serves the split over the length. */
+typedef struct pnp_scan_desc {
+  int64_t B, L;
+  int32_t dim, N, groups, type;
+  const void *u, *delta, *z, *Bm, *Cm;
+  int64_t u_bstride, u_tstride, delta_bstride, delta_tstride, z_bstride, z_tstride;
+  int64_t B_bstride, B_tstride, C_bstride, C_tstride;
+  const float *A, *D, *delta_bias, *state;
+  const uint8_t* starts;
+  void* out;
+  float *last_state, *ckpt, *workspace;
+  int64_t ckpt_floats, workspace_floats;
+} pnp_scan_desc;
+int64_t pnp_scan_ckpt_floats(const pnp_scan_desc* d);
+int64_t pnp_scan_workspace(const pnp_scan_desc* d);
+int32_t pnp_selective_scan(const pnp_scan_desc* d, void* stream);
+
+/* The gradient of out and last_state (dlast, may be NULL).  du, ddelta, dz (NULL without z) [B][L][dim],
+ * dB, dC [B][L][groups][N] (type `type`); dA [dim][N], dD, ddelta_bias [dim] (may be NULL), dstate
+ * [B][dim][N] (may be NULL) fp32.  f.ckpt as the forward wrote it. */
+typedef struct pnp_scan_bwd_desc {
+  pnp_scan_desc f;
+  const void* dout;
+  int64_t dout_bstride, dout_tstride;
+  const float* dlast;
+  void *du, *ddelta, *dz, *dB, *dC;
+  float *dA, *dD, *ddelta_bias, *dstate;
+  float* workspace;
+  int64_t workspace_floats;
+} pnp_scan_bwd_desc;
+int64_t pnp_scan_bwd_workspace(const pnp_scan_bwd_desc* d);
+int32_t pnp_selective_scan_bwd(const pnp_scan_bwd_desc* d, void* stream);
+
+/* One token of each of f.B sequences (f.L = 1, the token strides unread): state [B][dim][N] (f.state and
+ * f.last_state: the same memory, or not) advanced; f.starts is reset [B]. */
+int32_t pnp_selective_scan_step(const pnp_scan_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,104 @@
+// seq_dev.h — what the sequence operators' kernels share (seq_norm.hip, seq_i8.hip, seq_conv.hip,
+// seq_scan.hip): element types, vector loads, cross-lane sums, the host-side checks.
+//
+// Every kernel computes in fp32 whatever the tensors' type is and rounds a result once, where it is
+// stored (nearest even).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/pnp.h"
+
+void pnp_set_error(const char* fmt, ...);
+int32_t pnp_check_launch(const char* what);
+
+namespace seq {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+template <typename T> __device__ __forceinline__ float to_f(T v) { return (float)v; }
+template <typename T> __device__ __forceinline__ T from_f(float v) { return (T)v; }
+
+// V elements of T moved by one load or store (V * sizeof(T) <= 16, aligned to it)
+template <typename T, int V> struct alignas(V * sizeof(T)) Pack { T v[V]; };
+
+template <int V, typename T> __device__ __forceinline__ void load_f(const T* p, float (&o)[V]) {
+  const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+  for (int i = 0; i < V; i++) o[i] = to_f(k.v[i]);
+}
+template <int V, typename T> __device__ __forceinline__ void store_f(T* p, const float (&o)[V]) {
+  Pack<T, V> k;
+#pragma unroll
+  for (int i = 0; i < V; i++) k.v[i] = from_f<T>(o[i]);
+  *reinterpret_cast<Pack<T, V>*>(p) = k;
+}
+
+// sigmoid by the hardware's exp2 and reciprocal: 1 / (1 + 2^(-x log2 e)), relative error a few 2^-24;
+// x -> -inf gives 1 / inf = 0, x -> inf 1
+__device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
+#define SEQ_LOG2E 1.44269504088896340736f
+__device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.f + exp2_f(-SEQ_LOG2E * x)); }
+
+// softplus(x) = max(x, 0) + log1p(exp(-|x|)), with e = exp(-|x|) in (0, 1]: no overflow, and log1p
+// keeps the relative accuracy of small results (log(1 + e) would lose it: at x = -10 to 1e-3)
+__device__ __forceinline__ float softplus_f(float x) {
+  const float e = exp2_f(-SEQ_LOG2E * fabsf(x));
+  return fmaxf(x, 0.f) + log1pf(e);   // (NaN: through e)
+}
+
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+#define SEQ_DPP_XOR1 0xB1         // quad_perm [1, 0, 3, 2]
+#define SEQ_DPP_XOR2 0x4E         // quad_perm [2, 3, 0, 1]
+#define SEQ_DPP_HALF_MIRROR 0x141 // lane i of 8 -> 7 - i
+#define SEQ_DPP_MIRROR 0x140      // lane i of 16 -> 15 - i
+#define SEQ_DPP_ROR8 0x128        // lane i of 16 -> i + 8 mod 16 (the same as xor 8)
+
+// the sum over groups of S neighbouring lanes, in every lane of the group (S 1 .. 64, a power of two);
+// every lane of the wave takes part.  Mirrors serve as xor 4 / xor 8 once the lanes they pair hold equal
+// sums of their quads / halves.
+template <int S> __device__ __forceinline__ float group_sum(float v) {
+  if (S >= 2) v += dpp<SEQ_DPP_XOR1>(v);
+  if (S >= 4) v += dpp<SEQ_DPP_XOR2>(v);
+  if (S >= 8) v += dpp<SEQ_DPP_HALF_MIRROR>(v);
+  if (S >= 16) v += dpp<SEQ_DPP_MIRROR>(v);
+  if (S >= 32) v += __shfl_xor(v, 16, 64);
+  if (S >= 64) v += __shfl_xor(v, 32, 64);
+  return v;
+}
+// max that keeps NaN (fmaxf drops it)
+__device__ __forceinline__ float max_nan(float a, float b) { return (a > b || a != a) ? a : b; }
+__device__ __forceinline__ float wave_max_nan(float v) {
+  v = max_nan(v, dpp<SEQ_DPP_XOR1>(v));
+  v = max_nan(v, dpp<SEQ_DPP_XOR2>(v));
+  v = max_nan(v, dpp<SEQ_DPP_HALF_MIRROR>(v));
+  v = max_nan(v, dpp<SEQ_DPP_MIRROR>(v));
+  v = max_nan(v, __shfl_xor(v, 16, 64));
+  v = max_nan(v, __shfl_xor(v, 32, 64));
+  return v;
+}
+
+// ---- host
+inline int type_bytes(int t) { return t == PNP_F32 ? 4 : t == PNP_BF16 || t == PNP_F16 ? 2 : 0; }
+inline bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p % n) == 0; }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// f(T{}) for the type code, PNP_ERR_ARG for any other
+#define SEQ_BY_TYPE(type, T, ...)                                       \
+  [&]() -> int32_t {                                                    \
+    switch (type) {                                                     \
+      case PNP_F32: { typedef float T; __VA_ARGS__; }                   \
+      case PNP_BF16: { typedef seq::bf16 T; __VA_ARGS__; }              \
+      case PNP_F16: { typedef seq::f16 T; __VA_ARGS__; }                \
+    }                                                                   \
+    return PNP_ERR_ARG;                                                 \
+  }()
+
+// out[c] = sum over r < n of part[r * stride + c], c < cols, rows in a fixed order (seq_norm.hip)
+int32_t column_sums(const float* part, int64_t n, int64_t stride, int64_t cols, float* out, hipStream_t st);
+
+}  // namespace seq

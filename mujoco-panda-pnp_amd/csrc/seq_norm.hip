@@ -1,0 +1,586 @@
+// seq_norm.hip — the residual's addition with the root-mean-square norm, its 8-bit output, its
+// gradient, and rows quantised to 8 bits (include/pnp.h pnp_rms_norm, pnp_rms_norm_bwd,
+// pnp_quantize_rows).
+//
+//   s = x + r (rounded to the stream's type: what later layers read is what is normalised),
+//   rho = 1 / sqrt(mean(s^2) + eps), n = s rho, y = n w
+//   dx = ds + rho (w dy - n mean(w dy n)),  dw = sum over rows of dy n
+//
+// Bound by HBM: a row is read once, kept in registers between its sums and its outputs, and written
+// once.  One wave holds a row of up to 4 packs a lane, a workgroup of 256 threads a wider one (up to
+// 8 packs a thread); rows past that are read twice (the second time from cache).
+#include <type_traits>
+
+#include "seq_dev.h"
+
+namespace seq {
+namespace {
+
+constexpr int NT = 256;
+
+struct NormArgs {
+  int64_t rows, xs, rs, qs;
+  int dim;
+  float eps;
+  const void *x, *r;
+  const float* w;
+  void *y, *s;
+  float* rstd;
+  int8_t* q;
+  float* scale;
+};
+
+// sum over the TPR threads of a row, in each of them; red: NT / 64 floats of LDS, a use apart each call
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red) {
+  v = group_sum<64>(v);
+  if (TPR == 64) return v;
+  const int w = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) red[w] = v;
+  __syncthreads();
+  return red[0] + red[1] + red[2] + red[3];
+}
+template <int TPR> __device__ __forceinline__ float row_max(float v, float* red) {
+  v = wave_max_nan(v);
+  if (TPR == 64) return v;
+  const int w = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) red[w] = v;
+  __syncthreads();
+  return max_nan(max_nan(red[0], red[1]), max_nan(red[2], red[3]));
+}
+
+// scale and 1 / scale of a row whose largest magnitude is m: 0 / 0 where the scale would be below the
+// least normal number, NaN / 0 where m is not finite
+__device__ __forceinline__ void q8_scale(float m, float& scale, float& inv) {
+  scale = m / 127.f;
+  inv = 1.f / scale;
+  if (!(m < __builtin_inff())) { scale = __builtin_nanf(""); inv = 0.f; }
+  else if (scale < 1.17549435e-38f) { scale = 0.f; inv = 0.f; }
+}
+__device__ __forceinline__ int8_t q8(float y, float inv) {
+  // inv = 0 gives q = 0 for the finite values of a row; NaN and infinity in it are cut here
+  const float v = rintf(y * inv);
+  return (int8_t)(int)(v == v ? fminf(fmaxf(v, -127.f), 127.f) : 0.f);
+}
+
+// T: x and y; R: the residual stream; V elements a load; TPR threads a row; NV packs a thread (0: rows
+// of any length, read twice); Q8: 8-bit output
+template <typename T, typename R, int V, int TPR, int NV, bool Q8>
+__device__ __forceinline__ void norm_fwd_row(const NormArgs& a, int64_t row, float (&red)[2][NT / 64]) {
+  const int lane = threadIdx.x % TPR;
+  const T* x = (const T*)a.x + row * a.xs;
+  const R* r = a.r ? (const R*)a.r + row * a.rs : nullptr;
+  R* so = a.s ? (R*)a.s + row * a.dim : nullptr;
+  auto read = [&](int i, float (&v)[V]) {
+    load_f<V>(x + i, v);
+    if (r) {
+      float b[V];
+      load_f<V>(r + i, b);
+#pragma unroll
+      for (int k = 0; k < V; k++) v[k] = to_f(from_f<R>(v[k] + b[k]));
+    }
+  };
+  auto scaled = [&](int i, float rho, float (&v)[V]) {
+    float w[V];
+    if (a.w) load_f<V>(a.w + i, w);
+#pragma unroll
+    for (int k = 0; k < V; k++) v[k] = a.w ? v[k] * rho * w[k] : v[k] * rho;
+  };
+  float sum = 0.f, m = 0.f;
+  if constexpr (NV > 0) {
+    float v[NV][V];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const int i = (j * TPR + lane) * V;
+      if (i < a.dim) read(i, v[j]);
+      else
+#pragma unroll
+        for (int k = 0; k < V; k++) v[j][k] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const int i = (j * TPR + lane) * V;
+      if (so && i < a.dim) store_f<V>(so + i, v[j]);
+#pragma unroll
+      for (int k = 0; k < V; k++) sum += v[j][k] * v[j][k];
+    }
+    const float rho = 1.f / sqrtf(row_sum<TPR>(sum, red[0]) / (float)a.dim + a.eps);
+    if (a.rstd && lane == 0) a.rstd[row] = rho;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const int i = (j * TPR + lane) * V;
+      if (i >= a.dim) continue;
+      scaled(i, rho, v[j]);
+      if constexpr (Q8) {
+#pragma unroll
+        for (int k = 0; k < V; k++) m = max_nan(m, fabsf(v[j][k]));
+      } else {
+        store_f<V>((T*)a.y + row * a.dim + i, v[j]);
+      }
+    }
+    if constexpr (Q8) {
+      float scale, inv;
+      q8_scale(row_max<TPR>(m, red[1]), scale, inv);
+      if (lane == 0) a.scale[row] = scale;
+#pragma unroll
+      for (int j = 0; j < NV; j++) {
+        const int i = (j * TPR + lane) * V;
+        if (i >= a.dim) continue;
+        Pack<int8_t, V> o;
+#pragma unroll
+        for (int k = 0; k < V; k++) o.v[k] = q8(v[j][k], inv);
+        *reinterpret_cast<Pack<int8_t, V>*>(a.q + row * a.qs + i) = o;
+      }
+    }
+  } else {
+    for (int i = lane * V; i < a.dim; i += TPR * V) {
+      float v[V];
+      read(i, v);
+      if (so) store_f<V>(so + i, v);
+#pragma unroll
+      for (int k = 0; k < V; k++) sum += v[k] * v[k];
+    }
+    const float rho = 1.f / sqrtf(row_sum<TPR>(sum, red[0]) / (float)a.dim + a.eps);
+    if (a.rstd && lane == 0) a.rstd[row] = rho;
+    for (int i = lane * V; i < a.dim; i += TPR * V) {
+      float v[V];
+      read(i, v);
+      scaled(i, rho, v);
+      if constexpr (Q8) {
+#pragma unroll
+        for (int k = 0; k < V; k++) m = max_nan(m, fabsf(v[k]));
+      } else {
+        store_f<V>((T*)a.y + row * a.dim + i, v);
+      }
+    }
+    if constexpr (Q8) {
+      float scale, inv;
+      q8_scale(row_max<TPR>(m, red[1]), scale, inv);
+      if (lane == 0) a.scale[row] = scale;
+      for (int i = lane * V; i < a.dim; i += TPR * V) {
+        float v[V];
+        read(i, v);
+        scaled(i, rho, v);
+        Pack<int8_t, V> o;
+#pragma unroll
+        for (int k = 0; k < V; k++) o.v[k] = q8(v[k], inv);
+        *reinterpret_cast<Pack<int8_t, V>*>(a.q + row * a.qs + i) = o;
+      }
+    }
+  }
+}
+
+// rows dealt to the grid; whole waves (TPR 64) or the whole workgroup work on one
+#define SEQ_ROWS(BODY)                                                                                      \
+  for (int64_t row = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR; row < a.rows;                    \
+       row += (int64_t)gridDim.x * (NT / TPR)) {                                                            \
+    BODY;                                                                                                   \
+    if (TPR > 64) __syncthreads(); /* the next row's sums go where this row's were read */                  \
+  }
+
+template <typename T, typename R, int V, int TPR, int NV, bool Q8>
+__global__ __launch_bounds__(NT) void norm_fwd_kernel(NormArgs a) {
+  __shared__ float red[2][NT / 64];
+  SEQ_ROWS((norm_fwd_row<T, R, V, TPR, NV, Q8>(a, row, red)))
+}
+
+// rows in 8 bits: the norm's kernel without the norm
+template <typename T, int V, int TPR, int NV>
+__device__ __forceinline__ void quantize_row(const NormArgs& a, int64_t row, float (&red)[NT / 64]) {
+  const int lane = threadIdx.x % TPR;
+  const T* x = (const T*)a.x + row * a.xs;
+  int8_t* q = a.q + row * a.qs;
+  float m = 0.f, scale, inv;
+  if constexpr (NV > 0) {
+    float v[NV][V];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const int i = (j * TPR + lane) * V;
+#pragma unroll
+      for (int k = 0; k < V; k++) v[j][k] = 0.f;
+      if (i < a.dim) load_f<V>(x + i, v[j]);
+#pragma unroll
+      for (int k = 0; k < V; k++) m = max_nan(m, fabsf(v[j][k]));
+    }
+    q8_scale(row_max<TPR>(m, red), scale, inv);
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const int i = (j * TPR + lane) * V;
+      if (i >= a.dim) continue;
+      Pack<int8_t, V> o;
+#pragma unroll
+      for (int k = 0; k < V; k++) o.v[k] = q8(v[j][k], inv);
+      *reinterpret_cast<Pack<int8_t, V>*>(q + i) = o;
+    }
+  } else {
+    for (int i = lane * V; i < a.dim; i += TPR * V) {
+      float v[V];
+      load_f<V>(x + i, v);
+#pragma unroll
+      for (int k = 0; k < V; k++) m = max_nan(m, fabsf(v[k]));
+    }
+    q8_scale(row_max<TPR>(m, red), scale, inv);
+    for (int i = lane * V; i < a.dim; i += TPR * V) {
+      float v[V];
+      load_f<V>(x + i, v);
+      Pack<int8_t, V> o;
+#pragma unroll
+      for (int k = 0; k < V; k++) o.v[k] = q8(v[k], inv);
+      *reinterpret_cast<Pack<int8_t, V>*>(q + i) = o;
+    }
+  }
+  if (lane == 0) a.scale[row] = scale;
+}
+
+template <typename T, int V, int TPR, int NV> __global__ __launch_bounds__(NT) void quantize_kernel(NormArgs a) {
+  __shared__ float red[NT / 64];
+  SEQ_ROWS((quantize_row<T, V, TPR, NV>(a, row, red)))
+}
+
+struct NormBwdArgs {
+  int64_t rows, dys, dss, ss;
+  int dim;
+  const void *dy, *ds, *s;
+  const float *w, *rstd;
+  void *dx, *dres;
+  float* part;   // [gridDim.x][dim] sums of dy n, or null
+};
+
+// A workgroup takes rows blockIdx, blockIdx + gridDim, ...: the weight's gradient stays in registers
+// over all of them (a thread keeps its columns) and leaves as one row of `part`.
+template <typename T, typename R, int V, int TPR, int NV>
+__global__ __launch_bounds__(NT) void norm_bwd_kernel(NormBwdArgs a) {
+  constexpr int RPB = NT / TPR;
+  __shared__ float red[2][NT / 64];
+  const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  float acc[NV > 0 ? NV : 1][V] = {};
+  int flip = 0;
+  const float rdim = 1.f / (float)a.dim;
+  for (int64_t row = (int64_t)blockIdx.x * RPB + sub; row < a.rows; row += (int64_t)gridDim.x * RPB) {
+    const T* dy = (const T*)a.dy + row * a.dys;
+    const R* s = (const R*)a.s + row * a.ss;
+    const R* ds = a.ds ? (const R*)a.ds + row * a.dss : nullptr;
+    T* dx = (T*)a.dx + row * a.dim;
+    R* dr = a.dres ? (R*)a.dres + row * a.dim : nullptr;
+    const float rho = a.rstd[row];
+    float dot = 0.f;
+    auto pair = [&](int i, float (&g)[V], float (&n)[V]) {
+      load_f<V>(dy + i, g);
+      load_f<V>(s + i, n);
+#pragma unroll
+      for (int k = 0; k < V; k++) n[k] *= rho;
+    };
+    auto weigh = [&](int i, float (&g)[V]) {
+      float w[V];
+      if (!a.w) return;
+      load_f<V>(a.w + i, w);
+#pragma unroll
+      for (int k = 0; k < V; k++) g[k] *= w[k];
+    };
+    auto put = [&](int i, float mean, const float (&g)[V], const float (&n)[V]) {
+      float d[V], b[V];
+      if (ds) load_f<V>(ds + i, b);
+#pragma unroll
+      for (int k = 0; k < V; k++) {
+        d[k] = rho * (g[k] - n[k] * mean);
+        if (ds) d[k] += b[k];
+      }
+      store_f<V>(dx + i, d);
+      if (dr) store_f<V>(dr + i, d);
+    };
+    if constexpr (NV > 0) {
+      float g[NV][V], n[NV][V];
+#pragma unroll
+      for (int j = 0; j < NV; j++) {
+        const int i = (j * TPR + lane) * V;
+        if (i < a.dim) pair(i, g[j], n[j]);
+        else
+#pragma unroll
+          for (int k = 0; k < V; k++) g[j][k] = n[j][k] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < NV; j++) {
+        const int i = (j * TPR + lane) * V;
+        if (i >= a.dim) continue;
+#pragma unroll
+        for (int k = 0; k < V; k++) acc[j][k] += g[j][k] * n[j][k];
+        weigh(i, g[j]);
+#pragma unroll
+        for (int k = 0; k < V; k++) dot += g[j][k] * n[j][k];
+      }
+      const float mean = row_sum<TPR>(dot, red[flip]) * rdim;
+      flip ^= 1;   // (the next row's sums may be written while a slow wave still reads this row's)
+#pragma unroll
+      for (int j = 0; j < NV; j++) {
+        const int i = (j * TPR + lane) * V;
+        if (i < a.dim) put(i, mean, g[j], n[j]);
+      }
+    } else {
+      for (int i = lane * V; i < a.dim; i += TPR * V) {
+        float g[V], n[V];
+        pair(i, g, n);
+        weigh(i, g);
+#pragma unroll
+        for (int k = 0; k < V; k++) dot += g[k] * n[k];
+      }
+      const float mean = row_sum<TPR>(dot, red[flip]) * rdim;
+      flip ^= 1;
+      for (int i = lane * V; i < a.dim; i += TPR * V) {
+        float g[V], n[V];
+        pair(i, g, n);
+        weigh(i, g);
+        put(i, mean, g, n);
+      }
+    }
+  }
+  if constexpr (NV > 0) {
+    if (!a.part) return;
+    if constexpr (RPB > 1) {   // the waves' sums of the same columns, in wave order
+      __shared__ float sh[RPB - 1][64 * V];
+#pragma unroll
+      for (int j = 0; j < NV; j++) {
+        if (sub)
+#pragma unroll
+          for (int k = 0; k < V; k++) sh[sub - 1][lane * V + k] = acc[j][k];
+        __syncthreads();
+        const int i = (j * TPR + lane) * V;
+        if (!sub && i < a.dim) {
+#pragma unroll
+          for (int u = 0; u < RPB - 1; u++)
+#pragma unroll
+            for (int k = 0; k < V; k++) acc[j][k] += sh[u][lane * V + k];
+          store_f<V>(a.part + (int64_t)blockIdx.x * a.dim + i, acc[j]);
+        }
+        __syncthreads();
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; j++) {
+        const int i = (j * TPR + lane) * V;
+        if (i < a.dim) store_f<V>(a.part + (int64_t)blockIdx.x * a.dim + i, acc[j]);
+      }
+    }
+  }
+}
+
+// sums of dy n over a strip of rows, a thread a column: for rows too wide for registers
+template <typename T, typename R> __global__ __launch_bounds__(NT) void norm_dw_kernel(NormBwdArgs a) {
+  const int c = blockIdx.x * NT + threadIdx.x;
+  if (c >= a.dim) return;
+  float acc = 0.f;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y)
+    acc += to_f(((const T*)a.dy)[row * a.dys + c]) * (to_f(((const R*)a.s)[row * a.ss + c]) * a.rstd[row]);
+  a.part[(int64_t)blockIdx.y * a.dim + c] = acc;
+}
+
+// 64 columns a workgroup, the rows dealt to 16 waves, their sums joined in wave order
+__global__ __launch_bounds__(1024) void column_sums_kernel(const float* part, int64_t n, int64_t stride, int64_t cols, float* out) {
+  __shared__ float sh[16][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+  if (c < cols) {
+    int64_t r = w;
+    for (; r + 48 < n; r += 64) {
+      const float* p = part + r * stride + c;
+      s0 += p[0];
+      s1 += p[16 * stride];
+      s2 += p[32 * stride];
+      s3 += p[48 * stride];
+    }
+    for (; r < n; r += 16) s0 += part[r * stride + c];
+  }
+  sh[w][lane] = (s0 + s1) + (s2 + s3);
+  __syncthreads();
+  if (w == 0 && c < cols) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) s += sh[i][lane];
+    out[c] = s;
+  }
+}
+
+// ---- host: the variant by the row's length.  A wave for rows of up to 4 packs a lane, else a workgroup.
+struct RowPlan { int tpr, nv; };
+// workgroups of a launch: a launch holds fewer than 2^32 threads
+unsigned row_blocks(int64_t rows, int tpr) {
+  const int64_t n = ceil_div(rows, NT / tpr);
+  return (unsigned)(n < (1 << 22) ? n : (1 << 22));
+}
+RowPlan plan_rows(int dim, int V) {
+  for (int nv = 1; nv <= 4; nv *= 2)
+    if (dim <= 64 * V * nv) return {64, nv};
+  for (int nv = 2; nv <= 8; nv *= 2)
+    if (dim <= NT * V * nv) return {NT, nv};
+  return {NT, 0};
+}
+
+template <typename F> int32_t by_plan(RowPlan p, F f) {
+  if (p.tpr == 64) {
+    if (p.nv == 1) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+    if (p.nv == 2) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+    return f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+  }
+  if (p.nv == 2) return f(std::integral_constant<int, NT>(), std::integral_constant<int, 2>());
+  if (p.nv == 4) return f(std::integral_constant<int, NT>(), std::integral_constant<int, 4>());
+  if (p.nv == 8) return f(std::integral_constant<int, NT>(), std::integral_constant<int, 8>());
+  return f(std::integral_constant<int, NT>(), std::integral_constant<int, 0>());
+}
+
+// rows start on a pack's boundary
+bool packs(const void* p, int64_t stride, int bytes, int V) {
+  return !p || (aligned_to(p, (size_t)bytes * V) && stride % V == 0);
+}
+
+template <typename T, typename R, int V> int32_t launch_fwd(const NormArgs& a, hipStream_t st) {
+  const RowPlan p = plan_rows(a.dim, V);
+  const unsigned grid = row_blocks(a.rows, p.tpr);
+  return by_plan(p, [&](auto tpr, auto nv) -> int32_t {
+    if (a.q) hipLaunchKernelGGL((norm_fwd_kernel<T, R, V, tpr, nv, true>), dim3(grid), dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((norm_fwd_kernel<T, R, V, tpr, nv, false>), dim3((unsigned)grid), dim3(NT), 0, st, a);
+    return pnp_check_launch("norm_fwd_kernel");
+  });
+}
+
+template <typename T, typename R> int32_t run_fwd(const NormArgs& a, hipStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool wide = a.dim % V == 0 && packs(a.x, a.xs, sizeof(T), V) && packs(a.r, a.rs, sizeof(R), V) &&
+                    packs(a.w, 0, 4, V) && packs(a.y, a.dim, sizeof(T), V) && packs(a.s, a.dim, sizeof(R), V) &&
+                    packs(a.q, a.qs, 1, V);
+  return wide ? launch_fwd<T, R, V>(a, st) : launch_fwd<T, R, 1>(a, st);
+}
+
+// workgroups of the gradient: enough for the chip, few enough that their rows of `part` stay small
+// next to what they read (each takes 8 rows or more where there are that many)
+int64_t bwd_blocks(int64_t rows, int tpr) {
+  const int64_t per = NT / tpr;
+  const int64_t want = ceil_div(rows, per * 8);
+  return want < 1 ? 1 : want > 1024 ? 1024 : want;
+}
+constexpr int64_t DW_STRIPS = 64;   // row strips of norm_dw_kernel
+int64_t bwd_parts(int64_t rows, int dim, int V) {
+  const RowPlan p = plan_rows(dim, V);
+  return p.nv ? bwd_blocks(rows, p.tpr) : DW_STRIPS;
+}
+
+template <typename T, typename R, int V> int32_t launch_bwd(NormBwdArgs a, float* dw, hipStream_t st) {
+  const RowPlan p = plan_rows(a.dim, V);
+  const int64_t grid = bwd_blocks(a.rows, p.tpr);
+  int32_t rc = by_plan(p, [&](auto tpr, auto nv) -> int32_t {
+    hipLaunchKernelGGL((norm_bwd_kernel<T, R, V, tpr, nv>), dim3((unsigned)grid), dim3(NT), 0, st, a);
+    return pnp_check_launch("norm_bwd_kernel");
+  });
+  if (rc || !dw) return rc;
+  if (!p.nv) {
+    hipLaunchKernelGGL((norm_dw_kernel<T, R>), dim3((unsigned)ceil_div(a.dim, NT), DW_STRIPS), dim3(NT), 0, st, a);
+    if ((rc = pnp_check_launch("norm_dw_kernel"))) return rc;
+  }
+  return column_sums(a.part, p.nv ? grid : DW_STRIPS, a.dim, a.dim, dw, st);
+}
+
+template <typename T, typename R> int32_t run_bwd(const NormBwdArgs& a, float* dw, hipStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool wide = a.dim % V == 0 && packs(a.dy, a.dys, sizeof(T), V) && packs(a.s, a.ss, sizeof(R), V) &&
+                    packs(a.ds, a.dss, sizeof(R), V) && packs(a.w, 0, 4, V) && packs(a.dx, a.dim, sizeof(T), V) &&
+                    packs(a.dres, a.dim, sizeof(R), V) && packs(a.part, a.dim, 4, V);
+  return wide ? launch_bwd<T, R, V>(a, dw, st) : launch_bwd<T, R, 1>(a, dw, st);
+}
+
+template <typename T> int32_t run_quantize(const NormArgs& a, hipStream_t st) {
+  constexpr int W = 16 / sizeof(T);
+  auto go = [&](auto v) -> int32_t {
+    constexpr int V = decltype(v)::value;
+    const RowPlan p = plan_rows(a.dim, V);
+    const unsigned grid = row_blocks(a.rows, p.tpr);
+    return by_plan(p, [&](auto tpr, auto nv) -> int32_t {
+      hipLaunchKernelGGL((quantize_kernel<T, V, tpr, nv>), dim3((unsigned)grid), dim3(NT), 0, st, a);
+      return pnp_check_launch("quantize_kernel");
+    });
+  };
+  const bool wide = a.dim % W == 0 && packs(a.x, a.xs, sizeof(T), W) && packs(a.q, a.qs, 1, W);
+  return wide ? go(std::integral_constant<int, W>()) : go(std::integral_constant<int, 1>());
+}
+
+bool rows_ok(int64_t rows, int dim) { return rows >= 0 && rows <= ((int64_t)1 << 40) && dim > 0 && dim <= (1 << 24); }
+
+}  // namespace
+
+int32_t column_sums(const float* part, int64_t n, int64_t stride, int64_t cols, float* out, hipStream_t st) {
+  hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)ceil_div(cols, 64)), dim3(1024), 0, st, part, n, stride, cols, out);
+  return pnp_check_launch("column_sums_kernel");
+}
+
+}  // namespace seq
+
+using namespace seq;
+
+extern "C" int32_t pnp_rms_norm(const pnp_norm_desc* d, void* stream) {
+  const char* fn = "pnp_rms_norm";
+  if (!d || !rows_ok(d->rows, d->dim) || !type_bytes(d->type) || (d->res_type != d->type && d->res_type != PNP_F32)) {
+    pnp_set_error("%s: bad shape or type", fn);
+    return PNP_ERR_ARG;
+  }
+  if (!d->rows) return PNP_OK;
+  if (!d->x || (!d->y) == (!d->q) || (d->q && (!d->scale || d->q_stride < d->dim)) || (d->residual && !d->s)) {
+    pnp_set_error("%s: null buffer, or not one of y and q", fn);
+    return PNP_ERR_ARG;
+  }
+  if (!d->residual && d->s && d->res_type != d->type) {
+    pnp_set_error("%s: the stream alone is in its own type", fn);
+    return PNP_ERR_ARG;
+  }
+  NormArgs a{d->rows, d->x_stride, d->r_stride, d->q_stride, d->dim, d->eps, d->x, d->residual, d->weight, d->y, d->s,
+             d->rstd, d->q, d->scale};
+  const hipStream_t st = (hipStream_t)stream;
+  if (d->res_type == d->type) return SEQ_BY_TYPE(d->type, T, return (run_fwd<T, T>(a, st)));
+  return SEQ_BY_TYPE(d->type, T, return (run_fwd<T, float>(a, st)));
+}
+
+extern "C" int64_t pnp_rms_norm_bwd_workspace(const pnp_norm_bwd_desc* d) {
+  if (!d || !rows_ok(d->rows, d->dim) || !type_bytes(d->type)) {
+    pnp_set_error("pnp_rms_norm_bwd_workspace: bad shape or type");
+    return PNP_ERR_ARG;
+  }
+  if (!d->rows) return 0;
+  // whichever of the two loads the tensors' alignment leads to
+  const int64_t wide = bwd_parts(d->rows, d->dim, 16 / type_bytes(d->type)), one = bwd_parts(d->rows, d->dim, 1);
+  return (wide > one ? wide : one) * d->dim;
+}
+
+extern "C" int32_t pnp_rms_norm_bwd(const pnp_norm_bwd_desc* d, void* stream) {
+  const char* fn = "pnp_rms_norm_bwd";
+  if (!d || !rows_ok(d->rows, d->dim) || !type_bytes(d->type) || (d->res_type != d->type && d->res_type != PNP_F32)) {
+    pnp_set_error("%s: bad shape or type", fn);
+    return PNP_ERR_ARG;
+  }
+  const hipStream_t st = (hipStream_t)stream;
+  if (!d->rows) return d->dweight ? column_sums(nullptr, 0, 0, d->dim, d->dweight, st) : PNP_OK;
+  if (!d->dy || !d->s || !d->rstd || !d->dx) {
+    pnp_set_error("%s: null buffer", fn);
+    return PNP_ERR_ARG;
+  }
+  if (d->dweight && (!d->workspace || d->workspace_floats < pnp_rms_norm_bwd_workspace(d))) {
+    pnp_set_error("%s: workspace too small", fn);
+    return PNP_ERR_ARG;
+  }
+  NormBwdArgs a{d->rows, d->dy_stride, d->ds_stride, d->s_stride, d->dim, d->dy, d->ds, d->s, d->weight, d->rstd,
+                d->dx, d->dres, d->dweight ? d->workspace : nullptr};
+  if (d->res_type == d->type) return SEQ_BY_TYPE(d->type, T, return (run_bwd<T, T>(a, d->dweight, st)));
+  return SEQ_BY_TYPE(d->type, T, return (run_bwd<T, float>(a, d->dweight, st)));
+}
+
+extern "C" int32_t pnp_quantize_rows(const void* x, int64_t x_stride, int32_t type, int64_t rows, int32_t dim, int8_t* q,
+                                     int64_t q_stride, float* scale, void* stream) {
+  if (!rows_ok(rows, dim) || !type_bytes(type) || q_stride < dim) {
+    pnp_set_error("pnp_quantize_rows: bad shape or type");
+    return PNP_ERR_ARG;
+  }
+  if (!rows) return PNP_OK;
+  if (!x || !q || !scale) {
+    pnp_set_error("pnp_quantize_rows: null buffer");
+    return PNP_ERR_ARG;
+  }
+  NormArgs a{};
+  a.rows = rows; a.xs = x_stride; a.qs = q_stride; a.dim = dim; a.x = x; a.q = q; a.scale = scale;
+  const hipStream_t st = (hipStream_t)stream;
+  return SEQ_BY_TYPE(type, T, return run_quantize<T>(a, st));
+}

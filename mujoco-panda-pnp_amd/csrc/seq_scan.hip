@@ -1,0 +1,870 @@
+// seq_scan.hip — the selective state space scan: forward, gradient, and the single-token form
+// (include/pnp.h pnp_selective_scan and its kin).
+//
+//   dt = softplus(delta + bias), a = exp(dt A), h[t] = a h[t-1] + dt u B, y = sum_n C h + D u,
+//   out = y z sigmoid(z); a = 0 at a token that starts a sequence.
+// With dy = dout z sigmoid(z) and g[t] = C dy + a[t+1] g[t+1]:
+//   dC = sum_d dy h, dB = sum_d g dt u, du = D dy + dt sum_n g B,
+//   ddt = sum_n g (a h[t-1]) A + u sum_n g B, ddelta = ddt sigmoid(delta + bias),
+//   dA = sum_{b,t} g dt (a h[t-1]), dD = sum dy u, dz = dout y sigmoid(z) (1 + z (1 - sigmoid(z)))
+//
+// Layout: a lane holds 4 states of one channel, S = ceil(N / 4) lanes (a power of two) a channel, so a
+// wave has 64 / S channels and a workgroup of 4 waves CW = 256 / S.  The workgroup walks its channels
+// along the length in tiles: it loads a tile of u, delta, z whole lines at a time, turns them into
+// dt and dt u once (a lane's S - 1 neighbours would repeat the softplus), and leaves them in LDS with
+// the tile's B and C, which all its channels share.  The next tile's loads are in flight meanwhile.
+//
+// Per state and token the recurrence costs one exp2 (a quarter-rate instruction: 4) and 4 more
+// instructions; with N = 16 that, not HBM, bounds it.
+//
+// Few sequences of great length do not fill the chip: the length is cut in chunks, a first pass gets
+// each chunk's state from a zero start and its decay (exp(A sum dt): one number a channel), a small
+// kernel chains them, and the main pass starts every chunk from its true state.  The gradient does the
+// same from the other end.
+#include "seq_dev.h"
+
+namespace seq {
+namespace {
+
+constexpr int NT = 256;
+
+// tile of the forward, and tile of the gradient (its states stay in registers: 4 * 2 a token)
+constexpr int tile_f(int S) { return S == 1 ? 8 : S == 2 ? 16 : 32; }
+constexpr int tile_b(int S) { return S == 1 ? 8 : 16; }
+
+struct ScanArgs {
+  int64_t B, L;
+  int dim, N, groups, per;       // per: channels of a group
+  int tiles;                     // workgroups across a group's channels
+  int nch;                       // chunks of the length
+  int64_t chunk;                 // tokens of a chunk, a multiple of the tile
+  int64_t nck;                   // states kept a sequence: one each tile_b tokens
+  const void *u, *delta, *z, *Bm, *Cm;
+  int64_t ub, ut, db, dt, zb, zt, Bb, Bt, Cb, Ct;
+  const float *A, *D, *bias, *state;
+  const uint8_t* starts;
+  void* out;
+  float *last, *ckpt;
+  float *hin;                    // [B][nch][dim][4 S] states at the chunks' starts (nch > 1)
+  float *dsum;                   // [B][nch][dim] sums of dt; NaN where the chunk holds a start
+  int wide;                      // packs of channels are aligned
+  int wide_bc;                   // packs of 4 states of B and C are aligned
+};
+
+struct Where { int64_t b, row; int chunk, g, c0, ch; };   // c0: first channel within the group; row: b * nch + chunk
+template <int S> __device__ __forceinline__ Where where(const ScanArgs& a) {
+  const int per_row = a.groups * a.tiles;
+  const int64_t row = blockIdx.x / per_row;
+  const int r = (int)(blockIdx.x - row * per_row);
+  Where w;
+  w.row = row;
+  w.b = row / a.nch;
+  w.chunk = (int)(row - w.b * a.nch);
+  w.g = r / a.tiles;
+  w.c0 = (r - w.g * a.tiles) * (NT / S);
+  w.ch = w.g * a.per + w.c0;
+  return w;
+}
+
+// E neighbouring channels of one token, as fp32; channels past the group's and tokens past the end as 0
+template <int E, typename T>
+__device__ __forceinline__ void load_channels(const T* p, int left, bool wide, float (&v)[E]) {
+  constexpr int V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
+  if (wide && left >= E) {
+#pragma unroll
+    for (int i = 0; i < E; i += V) {
+      float w[V];
+      load_f<V>(p + i, w);
+#pragma unroll
+      for (int k = 0; k < V; k++) v[i + k] = w[k];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; i++) v[i] = i < left ? to_f(p[i]) : 0.f;
+  }
+}
+template <int E, typename T> __device__ __forceinline__ void store_channels(T* p, int left, bool wide, const float (&v)[E]) {
+  constexpr int V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
+  if (wide && left >= E) {
+#pragma unroll
+    for (int i = 0; i < E; i += V) {
+      float w[V];
+#pragma unroll
+      for (int k = 0; k < V; k++) w[k] = v[i + k];
+      store_f<V>(p + i, w);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; i++)
+      if (i < left) p[i] = from_f<T>(v[i]);
+  }
+}
+
+// 4 states of B or C of one token, zeros past N
+template <typename T> __device__ __forceinline__ float4 load_states(const T* p, int n, int N, bool wide) {
+  if (wide) {   // N is a multiple of 4: a pack is whole or not there
+    if (n >= N) return float4{0.f, 0.f, 0.f, 0.f};
+    float v[4];
+    load_f<4>(p + n, v);
+    return float4{v[0], v[1], v[2], v[3]};
+  }
+  float4 r;
+  r.x = n < N ? to_f(p[n]) : 0.f;
+  r.y = n + 1 < N ? to_f(p[n + 1]) : 0.f;
+  r.z = n + 2 < N ? to_f(p[n + 2]) : 0.f;
+  r.w = n + 3 < N ? to_f(p[n + 3]) : 0.f;
+  return r;
+}
+__device__ __forceinline__ void load_state4(const float* p, int n, int N, float (&h)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) h[i] = n + i < N ? p[n + i] : 0.f;
+}
+
+// the tile's tokens that start a sequence, a bit each (TT <= 32), the same in every wave
+template <int TT> __device__ __forceinline__ uint32_t start_bits(const ScanArgs& a, int64_t b, int64_t t0, int64_t t1) {
+  if (!a.starts) return 0;
+  const int l = threadIdx.x & 63;
+  const bool s = l < TT && t0 + l < t1 && a.starts[b * a.L + t0 + l] != 0;
+  return (uint32_t)__builtin_amdgcn_ballot_w64(s);
+}
+
+// STATE: the chunk's state from a zero start and its decay alone
+template <typename T, int S, bool STATE> __global__ __launch_bounds__(NT) void scan_fwd_kernel(ScanArgs a) {
+  constexpr int TT = tile_f(S), TB = tile_b(S), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S;
+  __shared__ float2 dd[TT][CW];
+  __shared__ float4 sB[TT][S], sC[STATE ? 1 : TT][S];
+  const Where w = where<S>(a);
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int cl = wave * (64 / S) + lane / S, ng = lane % S;         // the lane's channel and states
+  const int lt = tid / RT, lc = (tid % RT) * E;                     // the thread's part of a tile
+  const int left = a.per - w.c0 - lc;                               // channels from there to the group's end
+  const bool on = w.c0 + cl < a.per;
+  const int64_t t0 = (int64_t)w.chunk * a.chunk, t1 = t0 + a.chunk < a.L ? t0 + a.chunk : a.L;
+  const T* u = (const T*)a.u + w.b * a.ub + w.ch + lc;
+  const T* dl = (const T*)a.delta + w.b * a.db + w.ch + lc;
+  const T* z = !STATE && a.z ? (const T*)a.z + w.b * a.zb + w.ch + lc : nullptr;
+  const T* Bm = (const T*)a.Bm + w.b * a.Bb + (int64_t)w.g * a.N;
+  const T* Cm = (const T*)a.Cm + w.b * a.Cb + (int64_t)w.g * a.N;
+
+  float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f}, dsum = 0.f;
+  const int64_t ch = w.ch + (on ? cl : 0);
+  load_state4(a.A + ch * a.N, 4 * ng, a.N, A2);
+#pragma unroll
+  for (int i = 0; i < 4; i++) A2[i] *= SEQ_LOG2E;
+  if (!STATE) {
+    if (a.nch > 1) load_state4(a.hin + (w.row * a.dim + ch) * NP, 4 * ng, NP, h);
+    else if (a.state) load_state4(a.state + (w.b * a.dim + ch) * a.N, 4 * ng, a.N, h);
+  }
+  float Dv[E], bias[E];
+#pragma unroll
+  for (int i = 0; i < E; i++) {
+    Dv[i] = !STATE && a.D && i < left ? a.D[w.ch + lc + i] : 0.f;
+    bias[i] = a.bias && i < left ? a.bias[w.ch + lc + i] : 0.f;
+  }
+  float nu[E], nd[E], nz[E], cu[E], cz[E];
+  constexpr int NBC = STATE ? TT * S : 2 * TT * S;                  // packs of 4 states a tile
+  constexpr int PER = (NBC + NT - 1) / NT;
+  float4 nbc[PER];
+  auto fetch = [&](int64_t t) {
+    const int64_t tt = t + lt;
+    const int l = tt < t1 ? left : 0;
+    load_channels<E>(u + tt * a.ut, l, a.wide, nu);
+    load_channels<E>(dl + tt * a.dt, l, a.wide, nd);
+    if (z) load_channels<E>(z + tt * a.zt, l, a.wide, nz);
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const int i = k * NT + tid;
+      const bool isC = i >= TT * S;
+      const int r = isC ? i - TT * S : i;
+      const int64_t bt = t + r / S;
+      nbc[k] = float4{0.f, 0.f, 0.f, 0.f};
+      if (i < NBC && bt < t1)
+        nbc[k] = isC ? load_states(Cm + bt * a.Ct, 4 * (r % S), a.N, a.wide_bc) : load_states(Bm + bt * a.Bt, 4 * (r % S), a.N, a.wide_bc);
+    }
+  };
+  if (t0 < t1) fetch(t0);
+  for (int64_t t = t0; t < t1; t += TT) {
+    const bool mine = t + lt < t1;
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+      const float d = mine && i < left ? softplus_f(nd[i] + bias[i]) : 0.f;
+      dd[lt][lc + i] = float2{d, d * nu[i]};
+      cu[i] = nu[i];
+      cz[i] = nz[i];
+    }
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const int i = k * NT + tid;
+      if (i < TT * S) (&sB[0][0])[i] = nbc[k];
+      else if (!STATE && i < 2 * TT * S) (&sC[0][0])[i - TT * S] = nbc[k];
+    }
+    const uint32_t bits = start_bits<TT>(a, w.b, t, t1);
+    __syncthreads();
+    if (t + TT < t1) fetch(t + TT);
+#pragma unroll
+    for (int p = 0; p < TT; p += TB) {
+      if (!STATE && a.ckpt && on && t + p < t1)
+        *reinterpret_cast<float4*>(a.ckpt + ((w.b * a.nck + (t + p) / TB) * a.dim + ch) * NP + 4 * ng) = float4{h[0], h[1], h[2], h[3]};
+#pragma unroll 4
+      for (int k = p; k < p + TB; k++) {
+        const float2 d = dd[k][cl];
+        const float4 b = sB[k][ng];
+        if (bits >> k & 1) {
+          h[0] = h[1] = h[2] = h[3] = 0.f;
+          if (STATE) dsum = __builtin_nanf("");
+        }
+        h[0] = exp2_f(d.x * A2[0]) * h[0] + d.y * b.x;
+        h[1] = exp2_f(d.x * A2[1]) * h[1] + d.y * b.y;
+        h[2] = exp2_f(d.x * A2[2]) * h[2] + d.y * b.z;
+        h[3] = exp2_f(d.x * A2[3]) * h[3] + d.y * b.w;
+        if (STATE) {
+          dsum += d.x;
+        } else {
+          const float4 c = sC[k][ng];
+          const float y = group_sum<S>(c.x * h[0] + c.y * h[1] + c.z * h[2] + c.w * h[3]);
+          if (ng == 0) dd[k][cl].x = y;   // (its dt has been read by every lane of the channel)
+        }
+      }
+    }
+    __syncthreads();
+    if (!STATE && mine) {
+      float o[E];
+#pragma unroll
+      for (int i = 0; i < E; i++) {
+        o[i] = dd[lt][lc + i].x + Dv[i] * cu[i];
+        if (z) o[i] *= cz[i] * sigmoid_f(cz[i]);
+      }
+      store_channels<E>((T*)a.out + (w.b * a.L + t + lt) * a.dim + w.ch + lc, left, a.wide, o);
+    }
+  }
+  if (!on) return;
+  if (STATE) {
+    *reinterpret_cast<float4*>(a.hin + (w.row * a.dim + ch) * NP + 4 * ng) = float4{h[0], h[1], h[2], h[3]};
+    if (ng == 0) a.dsum[w.row * a.dim + ch] = dsum;
+  } else if (a.last && w.chunk == a.nch - 1) {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (4 * ng + i < a.N) a.last[(w.b * a.dim + ch) * a.N + 4 * ng + i] = h[i];
+  }
+}
+
+// the chunks chained: what a chunk starts from takes the place of its own state.  back: from the other
+// end, the gradient's way.
+__global__ __launch_bounds__(NT) void scan_chain_kernel(ScanArgs a, const float* first, int NP, int back) {
+  const int64_t id = (int64_t)blockIdx.x * NT + threadIdx.x;
+  if (id >= a.B * a.dim * NP) return;
+  const int n = (int)(id % NP);
+  const int64_t bd = id / NP, b = bd / a.dim;
+  const int d = (int)(bd - b * a.dim);
+  const float A2 = n < a.N ? a.A[(int64_t)d * a.N + n] * SEQ_LOG2E : 0.f;
+  float h = first && n < a.N ? first[bd * a.N + n] : 0.f;
+  for (int i = 0; i < a.nch; i++) {
+    const int64_t row = b * a.nch + (back ? a.nch - 1 - i : i);
+    float* p = a.hin + (row * a.dim + d) * NP + n;
+    const float own = *p, s = a.dsum[row * a.dim + d];
+    *p = h;
+    // a start in the chunk lets nothing through
+    h = s == s ? own + exp2_f(A2 * s) * h : own;
+  }
+}
+
+struct ScanBwdArgs {
+  ScanArgs f;
+  const void* dout;
+  int64_t ob, ot;
+  const float* dlast;
+  void *du, *ddelta, *dz, *dB, *dC;
+  float *dA, *dD, *dbias, *dstate;
+  float* part;    // [B * nch][dim * N + 2 dim]: dA, dD, ddelta_bias of a chunk
+  float* bc;      // [tiles][B * L][groups][2][4 S]: dB, dC of a workgroup's channels
+};
+
+// sums of v[8] over the lanes of a wave that differ in the channel (lane / S): lane l is left with
+// v[4 b5 + 2 b4 + b3] of all of them (b5, b4, b3: bits of l), for S = 16 with that and the next in v[0], v[1].
+// Halving: of two values a lane keeps one and gives the other away, so 8 sums over 16 lanes take 16
+// instructions, not 64.
+__device__ __forceinline__ float swap_add32(float x, float y) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float swap_add16(float x, float y) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <int S> __device__ __forceinline__ void channel_sums(float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = swap_add32(v[i], v[i + 4]);
+#pragma unroll
+  for (int i = 0; i < 2; i++) v[i] = swap_add16(v[i], v[i + 2]);
+  if (S < 16) {
+    const bool up = threadIdx.x & 8;
+    const float give = up ? v[0] : v[1], keep = up ? v[1] : v[0];
+    v[0] = keep + dpp<SEQ_DPP_ROR8>(give);
+  }
+  if (S < 8) v[0] += dpp<0x1B>(dpp<SEQ_DPP_HALF_MIRROR>(v[0]));   // xor 7, then quad_perm [3, 2, 1, 0]: xor 4
+  if (S < 4) v[0] += dpp<SEQ_DPP_XOR2>(v[0]);
+  if (S < 2) v[0] += dpp<SEQ_DPP_XOR1>(v[0]);
+}
+
+// STATE: the chunk's adjoint from a zero end and its decay alone
+template <typename T, int S, bool STATE> __global__ __launch_bounds__(NT, 2) void scan_bwd_kernel(ScanBwdArgs a) {
+  constexpr int TT = tile_b(S), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S;
+  const ScanArgs& f = a.f;
+  __shared__ float4 dd[TT][CW];                        // dt, u, dy, dt u; then sum g B, sum g (a h') A
+  __shared__ float yb[STATE ? 1 : TT][CW];             // sum C h
+  __shared__ float4 sB[TT][S], sC[TT][S];
+  __shared__ float bc[STATE ? 1 : 4][STATE ? 1 : TT][2 * NP];
+  const Where w = where<S>(f);
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int cl = wave * (64 / S) + lane / S, ng = lane % S;
+  const int lt = tid / RT, lc = (tid % RT) * E;
+  const int left = f.per - w.c0 - lc;
+  const bool on = w.c0 + cl < f.per;
+  const int64_t t0 = (int64_t)w.chunk * f.chunk, t1 = t0 + f.chunk < f.L ? t0 + f.chunk : f.L;
+  const T* u = (const T*)f.u + w.b * f.ub + w.ch + lc;
+  const T* dl = (const T*)f.delta + w.b * f.db + w.ch + lc;
+  const T* z = f.z ? (const T*)f.z + w.b * f.zb + w.ch + lc : nullptr;
+  const T* dout = (const T*)a.dout + w.b * a.ob + w.ch + lc;
+  const T* Bm = (const T*)f.Bm + w.b * f.Bb + (int64_t)w.g * f.N;
+  const T* Cm = (const T*)f.Cm + w.b * f.Cb + (int64_t)w.g * f.N;
+
+  float A[4], A2[4], dA[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {0.f, 0.f, 0.f, 0.f}, dsum = 0.f;
+  const int64_t ch = w.ch + (on ? cl : 0);
+  load_state4(f.A + ch * f.N, 4 * ng, f.N, A);
+#pragma unroll
+  for (int i = 0; i < 4; i++) A2[i] = A[i] * SEQ_LOG2E;
+  if (!STATE) {
+    if (f.nch > 1) load_state4(f.hin + (w.row * f.dim + ch) * NP, 4 * ng, NP, g);
+    else if (a.dlast) load_state4(a.dlast + (w.b * f.dim + ch) * f.N, 4 * ng, f.N, g);
+  }
+  float Dv[E], bias[E], dD[E] = {}, dbias[E] = {};
+#pragma unroll
+  for (int i = 0; i < E; i++) {
+    Dv[i] = f.D && i < left ? f.D[w.ch + lc + i] : 0.f;
+    bias[i] = f.bias && i < left ? f.bias[w.ch + lc + i] : 0.f;
+  }
+  constexpr int NBC = 2 * TT * S, PER = (NBC + NT - 1) / NT;
+  float nu[E], nd[E], nz[E], no[E], cu[E], cd[E], cz[E], co[E];
+  float4 nbc[PER], nh = {0.f, 0.f, 0.f, 0.f};
+  auto fetch = [&](int64_t t) {
+    const int64_t tt = t + lt;
+    const int l = tt < t1 ? left : 0;
+    load_channels<E>(u + tt * f.ut, l, f.wide, nu);
+    load_channels<E>(dl + tt * f.dt, l, f.wide, nd);
+    if (z) load_channels<E>(z + tt * f.zt, l, f.wide, nz);
+    load_channels<E>(dout + tt * a.ot, l, f.wide, no);
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const int i = k * NT + tid;
+      const bool isC = i >= TT * S;
+      const int r = isC ? i - TT * S : i;
+      const int64_t bt = t + r / S;
+      nbc[k] = float4{0.f, 0.f, 0.f, 0.f};
+      if (i < NBC && bt < t1)
+        nbc[k] = isC ? load_states(Cm + bt * f.Ct, 4 * (r % S), f.N, f.wide_bc) : load_states(Bm + bt * f.Bt, 4 * (r % S), f.N, f.wide_bc);
+    }
+    if (!STATE) nh = *reinterpret_cast<const float4*>(f.ckpt + ((w.b * f.nck + t / TT) * f.dim + ch) * NP + 4 * ng);
+  };
+  const int64_t tiles = (t1 - t0 + TT - 1) / TT;
+  if (tiles > 0) fetch(t0 + (tiles - 1) * TT);
+  for (int64_t t = t0 + (tiles - 1) * TT; t >= t0; t -= TT) {
+    const bool mine = t + lt < t1;
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+      const bool in = mine && i < left;
+      const float d = in ? softplus_f(nd[i] + bias[i]) : 0.f;
+      cu[i] = nu[i];
+      cd[i] = nd[i] + bias[i];
+      cz[i] = nz[i];
+      co[i] = no[i];
+      const float dy = !in ? 0.f : z ? no[i] * nz[i] * sigmoid_f(nz[i]) : no[i];
+      dd[lt][lc + i] = float4{d, nu[i], dy, d * nu[i]};
+    }
+    const float4 h0 = nh;
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const int i = k * NT + tid;
+      if (i < TT * S) (&sB[0][0])[i] = nbc[k];
+      else if (i < 2 * TT * S) (&sC[0][0])[i - TT * S] = nbc[k];
+    }
+    const uint32_t bits = start_bits<TT>(f, w.b, t, t1);
+    __syncthreads();
+    if (t > t0) fetch(t - TT);
+    if constexpr (STATE) {
+#pragma unroll 4
+      for (int k = TT - 1; k >= 0; k--) {
+        const float4 d = dd[k][cl];
+        const float4 c = sC[k][ng];
+        g[0] = exp2_f(d.x * A2[0]) * (g[0] + c.x * d.z);
+        g[1] = exp2_f(d.x * A2[1]) * (g[1] + c.y * d.z);
+        g[2] = exp2_f(d.x * A2[2]) * (g[2] + c.z * d.z);
+        g[3] = exp2_f(d.x * A2[3]) * (g[3] + c.w * d.z);
+        dsum += d.x;
+        if (bits >> k & 1) {
+          g[0] = g[1] = g[2] = g[3] = 0.f;
+          dsum = __builtin_nanf("");
+        }
+      }
+      __syncthreads();
+    } else {
+      float e[TT][4], h[TT + 1][4];
+      h[0][0] = h0.x; h[0][1] = h0.y; h[0][2] = h0.z; h[0][3] = h0.w;
+#pragma unroll
+      for (int k = 0; k < TT; k++) {
+        const float4 d = dd[k][cl];
+        const float4 b = sB[k][ng];
+        const float bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) e[k][i] = exp2_f(d.x * A2[i]);
+        float ah[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) ah[i] = e[k][i] * h[k][i];
+        if (bits >> k & 1) ah[0] = ah[1] = ah[2] = ah[3] = 0.f;   // (whatever the state: 0 times infinity is NaN)
+#pragma unroll
+        for (int i = 0; i < 4; i++) h[k + 1][i] = ah[i] + d.w * bv[i];
+        if (z) {
+          const float4 c = sC[k][ng];
+          const float y = group_sum<S>(c.x * h[k + 1][0] + c.y * h[k + 1][1] + c.z * h[k + 1][2] + c.w * h[k + 1][3]);
+          if (ng == 0) yb[k][cl] = y;
+        }
+      }
+#pragma unroll
+      for (int k = TT - 1; k >= 0; k--) {
+        const float4 d = dd[k][cl];
+        const float4 b = sB[k][ng], c = sC[k][ng];
+        const float bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
+        float s1 = 0.f, s2 = 0.f, v[8], ah[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) ah[i] = e[k][i] * h[k][i];
+        if (bits >> k & 1) ah[0] = ah[1] = ah[2] = ah[3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          g[i] += cv[i] * d.z;
+          v[4 + i] = h[k + 1][i] * d.z;
+          v[i] = g[i] * d.w;
+          s1 += g[i] * bv[i];
+          const float gah = g[i] * ah[i];
+          s2 += gah * A[i];
+          dA[i] += gah * d.x;
+          g[i] *= e[k][i];
+        }
+        if (bits >> k & 1) g[0] = g[1] = g[2] = g[3] = 0.f;
+        s1 = group_sum<S>(s1);
+        s2 = group_sum<S>(s2);
+        if (ng == 0) *reinterpret_cast<float2*>(&dd[k][cl]) = float2{s1, s2};
+        channel_sums<S>(v);
+        if (S >= 8 || (lane & 7) < S) {
+          const int at = (lane >> 5) * NP + 4 * ng + 2 * (lane >> 4 & 1);
+          if (S < 16) bc[wave][k][at + (lane >> 3 & 1)] = v[0];
+          else {
+            bc[wave][k][at] = v[0];
+            bc[wave][k][at + 1] = v[1];
+          }
+        }
+      }
+      __syncthreads();
+      if (mine) {
+        float du[E], dr[E], dz[E];
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+          const float4 s = dd[lt][lc + i];
+          const float dy = s.z, dtv = softplus_f(cd[i]);
+          du[i] = Dv[i] * dy + dtv * s.x;
+          dr[i] = i < left ? (s.y + cu[i] * s.x) * sigmoid_f(cd[i]) : 0.f;
+          dD[i] += dy * cu[i];
+          dbias[i] += dr[i];
+          if (z) {
+            const float sg = sigmoid_f(cz[i]);
+            dz[i] = co[i] * (yb[lt][lc + i] + Dv[i] * cu[i]) * (sg * (1.f + cz[i] * (1.f - sg)));
+          }
+        }
+        const int64_t at = (w.b * f.L + t + lt) * f.dim + w.ch + lc;
+        store_channels<E>((T*)a.du + at, left, f.wide, du);
+        store_channels<E>((T*)a.ddelta + at, left, f.wide, dr);
+        if (z) store_channels<E>((T*)a.dz + at, left, f.wide, dz);
+      }
+      // this workgroup's share of dB and dC
+      const int64_t tile = w.c0 / CW;
+      for (int i = tid; i < TT * 2 * NP; i += NT) {
+        const int k = i / (2 * NP), j = i - k * 2 * NP;
+        if (t + k < t1)
+          a.bc[(((tile * f.B + w.b) * f.L + t + k) * f.groups + w.g) * (2 * NP) + j] = bc[0][k][j] + bc[1][k][j] + bc[2][k][j] + bc[3][k][j];
+      }
+    }
+  }
+  if (STATE) {
+    if (!on) return;
+    *reinterpret_cast<float4*>(f.hin + (w.row * f.dim + ch) * NP + 4 * ng) = float4{g[0], g[1], g[2], g[3]};
+    if (ng == 0) f.dsum[w.row * f.dim + ch] = dsum;
+    return;
+  }
+  float* part = a.part + w.row * ((int64_t)f.dim * (f.N + 2));
+  if (on) {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (4 * ng + i < f.N) {
+        part[ch * f.N + 4 * ng + i] = dA[i];
+        if (a.dstate && w.chunk == 0) a.dstate[(w.b * f.dim + ch) * f.N + 4 * ng + i] = g[i];
+      }
+  }
+  // dD and ddelta_bias: the sums of the TT threads that share channels
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < E; i++) *reinterpret_cast<float2*>(&dd[lt][lc + i]) = float2{dD[i], dbias[i]};
+  __syncthreads();
+  if (tid < CW && w.c0 + tid < f.per) {
+    float2 s = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < TT; k++) {
+      const float2 v = *reinterpret_cast<const float2*>(&dd[k][tid]);
+      s.x += v.x;
+      s.y += v.y;
+    }
+    part[(int64_t)f.dim * f.N + w.ch + tid] = s.x;
+    part[(int64_t)f.dim * (f.N + 1) + w.ch + tid] = s.y;
+  }
+}
+
+// dB, dC [B][L][groups][N] from the workgroups' shares
+template <typename T> __global__ __launch_bounds__(NT) void scan_bc_kernel(const float* bc, int64_t rows, int N, int NP, int tiles, T* dB, T* dC) {
+  for (int64_t id = (int64_t)blockIdx.x * NT + threadIdx.x; id < rows * 2 * NP; id += (int64_t)gridDim.x * NT) {
+    const int64_t r = id / (2 * NP);
+    const int j = (int)(id - r * 2 * NP), n = j % NP;
+    if (n >= N) continue;
+    float s = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < tiles; i++) s += bc[i * rows * 2 * NP + id];
+    (j < NP ? dB : dC)[r * N + n] = from_f<T>(s);
+  }
+}
+
+// dA, dD, ddelta_bias from the chunks' rows
+__global__ __launch_bounds__(1024) void scan_sums_kernel(const float* part, int64_t rows, int dim, int N, float* dA, float* dD, float* dbias) {
+  __shared__ float sh[16][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t cols = (int64_t)dim * (N + 2), c = (int64_t)blockIdx.x * 64 + lane;
+  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+  if (c < cols) {
+    int64_t r = w;
+    for (; r + 48 < rows; r += 64) {
+      const float* p = part + r * cols + c;
+      s0 += p[0];
+      s1 += p[16 * cols];
+      s2 += p[32 * cols];
+      s3 += p[48 * cols];
+    }
+    for (; r < rows; r += 16) s0 += part[r * cols + c];
+  }
+  sh[w][lane] = (s0 + s1) + (s2 + s3);
+  __syncthreads();
+  if (w || c >= cols) return;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; i++) s += sh[i][lane];
+  const int64_t na = (int64_t)dim * N;
+  if (c < na) dA[c] = s;
+  else if (c < na + dim) { if (dD) dD[c - na] = s; }
+  else if (dbias) dbias[c - na - dim] = s;
+}
+
+// one token: a lane holds 4 states of a channel
+template <typename T, int S, bool W4> __global__ __launch_bounds__(NT) void scan_step_kernel(ScanArgs a) {
+  const int64_t n = a.B * a.dim * S;
+  for (int64_t base = (int64_t)blockIdx.x * NT; base < n; base += (int64_t)gridDim.x * NT) {
+    const int64_t id = base + threadIdx.x, bd = id < n ? id / S : 0;
+    const int ng = threadIdx.x % S;
+    const int64_t b = bd / a.dim;
+    const int d = (int)(bd - b * a.dim);
+    const bool on = id < n;
+    float h[4] = {0.f, 0.f, 0.f, 0.f}, A2[4];
+    const float* hp = a.state ? a.state + bd * a.N + 4 * ng : nullptr;
+    if (W4) {
+      if (hp) load_f<4>(hp, h);
+      load_f<4>(a.A + (int64_t)d * a.N + 4 * ng, A2);
+    } else {
+      if (hp) load_state4(hp - 4 * ng, 4 * ng, a.N, h);
+      load_state4(a.A + (int64_t)d * a.N, 4 * ng, a.N, A2);
+    }
+    const float uv = to_f(((const T*)a.u)[b * a.ub + d]);
+    const float raw = to_f(((const T*)a.delta)[b * a.db + d]) + (a.bias ? a.bias[d] : 0.f);
+    const float zv = a.z ? to_f(((const T*)a.z)[b * a.zb + d]) : 0.f;
+    const int g = d / a.per;
+    const float4 bm = load_states((const T*)a.Bm + b * a.Bb + (int64_t)g * a.N, 4 * ng, a.N, a.wide_bc);
+    const float4 cm = load_states((const T*)a.Cm + b * a.Cb + (int64_t)g * a.N, 4 * ng, a.N, a.wide_bc);
+    const float dt = softplus_f(raw), dtu = dt * uv;
+    if (a.starts && a.starts[b]) h[0] = h[1] = h[2] = h[3] = 0.f;
+    const float bv[4] = {bm.x, bm.y, bm.z, bm.w}, cv[4] = {cm.x, cm.y, cm.z, cm.w};
+    float y = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      h[i] = exp2_f(dt * (A2[i] * SEQ_LOG2E)) * h[i] + dtu * bv[i];
+      y += cv[i] * h[i];
+    }
+    y = group_sum<S>(y);
+    if (!on) continue;
+    if (W4) store_f<4>(a.last + bd * a.N + 4 * ng, h);
+    else
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (4 * ng + i < a.N) a.last[bd * a.N + 4 * ng + i] = h[i];
+    if (ng == 0) {
+      if (a.D) y += a.D[d] * uv;
+      if (a.z) y *= zv * sigmoid_f(zv);
+      ((T*)a.out)[bd] = from_f<T>(y);
+    }
+  }
+}
+
+// ---- host
+int lanes_of(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+int host_tile_f(int S) { return tile_f(S); }
+int host_tile_b(int S) { return tile_b(S); }
+
+bool scan_ok(const pnp_scan_desc* d) {
+  return d && d->B >= 0 && d->L >= 0 && d->dim > 0 && d->dim <= (1 << 24) && d->N >= 1 && d->N <= 64 && d->groups >= 1 &&
+         d->dim % d->groups == 0 && type_bytes(d->type) && d->B <= ((int64_t)1 << 31) && d->L <= ((int64_t)1 << 31);
+}
+
+// how a call is cut: chunks of the length where sequences and channels alone leave the chip idle
+struct Plan { int S, tiles, nch; int64_t chunk, nck, blocks; };
+Plan plan(const pnp_scan_desc* d) {
+  Plan p;
+  p.S = lanes_of(d->N);
+  const int per = d->dim / d->groups, tt = host_tile_f(p.S);
+  p.tiles = (int)ceil_div(per, NT / p.S);
+  const int64_t base = d->B * d->groups * p.tiles;
+  int64_t nch = 1;
+  if (base < 512) {
+    nch = ceil_div(1024, base ? base : 1);
+    const int64_t most = d->L / (4 * tt);   // a chunk of 4 tiles at least
+    if (nch > most) nch = most;
+    if (nch < 1) nch = 1;
+  }
+  p.chunk = ceil_div(ceil_div(d->L ? d->L : 1, nch), tt) * tt;
+  p.nch = (int)(d->L ? ceil_div(d->L, p.chunk) : 1);
+  p.nck = ceil_div(d->L, host_tile_b(p.S));
+  p.blocks = base * p.nch;
+  return p;
+}
+int64_t split_floats(const pnp_scan_desc* d, const Plan& p) {
+  return p.nch > 1 ? d->B * p.nch * d->dim * (int64_t)(4 * p.S + 1) : 0;
+}
+
+ScanArgs scan_args(const pnp_scan_desc* d, const Plan& p, float* workspace) {
+  ScanArgs a{};
+  a.B = d->B; a.L = d->L; a.dim = d->dim; a.N = d->N; a.groups = d->groups; a.per = d->dim / d->groups;
+  a.tiles = p.tiles; a.nch = p.nch; a.chunk = p.chunk; a.nck = p.nck;
+  a.u = d->u; a.delta = d->delta; a.z = d->z; a.Bm = d->Bm; a.Cm = d->Cm;
+  a.ub = d->u_bstride; a.ut = d->u_tstride; a.db = d->delta_bstride; a.dt = d->delta_tstride; a.zb = d->z_bstride; a.zt = d->z_tstride;
+  a.Bb = d->B_bstride; a.Bt = d->B_tstride; a.Cb = d->C_bstride; a.Ct = d->C_tstride;
+  a.A = d->A; a.D = d->D; a.bias = d->delta_bias; a.state = d->state; a.starts = d->starts;
+  a.out = d->out; a.last = d->last_state; a.ckpt = d->ckpt;
+  if (p.nch > 1) {
+    a.hin = workspace;
+    a.dsum = workspace + d->B * p.nch * d->dim * (int64_t)(4 * p.S);
+  }
+  return a;
+}
+
+// E channels of a thread start on a 16-byte boundary (or on the whole E, where that is less) in every tensor
+bool even(const void* p, int64_t s1, int64_t s2, int V, int bytes) {
+  return !p || (aligned_to(p, (size_t)V * bytes) && s1 % V == 0 && s2 % V == 0);
+}
+bool bc_even(const ScanArgs& a, int bytes) {
+  return a.N % 4 == 0 && even(a.Bm, a.Bb, a.Bt, 4, bytes) && even(a.Cm, a.Cb, a.Ct, 4, bytes);
+}
+
+#define BY_LANES(S_, S, ...)                                  \
+  [&]() -> int32_t {                                          \
+    switch (S_) {                                             \
+      case 1: { constexpr int S = 1; __VA_ARGS__; }           \
+      case 2: { constexpr int S = 2; __VA_ARGS__; }           \
+      case 4: { constexpr int S = 4; __VA_ARGS__; }           \
+      case 8: { constexpr int S = 8; __VA_ARGS__; }           \
+    }                                                         \
+    constexpr int S = 16;                                     \
+    __VA_ARGS__;                                              \
+  }()
+
+int32_t chain(const ScanArgs& a, const float* first, int S, int back, hipStream_t st) {
+  const int64_t n = a.B * a.dim * 4 * S;
+  hipLaunchKernelGGL(scan_chain_kernel, dim3((unsigned)ceil_div(n, NT)), dim3(NT), 0, st, a, first, 4 * S, back);
+  return pnp_check_launch("scan_chain_kernel");
+}
+
+template <typename T, int S> int32_t run_scan(ScanArgs a, int64_t blocks, hipStream_t st) {
+  constexpr int E = tile_f(S) / S, V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
+  a.wide = a.per % V == 0 && a.dim % V == 0 && even(a.u, a.ub, a.ut, V, sizeof(T)) && even(a.delta, a.db, a.dt, V, sizeof(T)) &&
+           even(a.z, a.zb, a.zt, V, sizeof(T)) && even(a.out, 0, 0, V, sizeof(T));
+  a.wide_bc = bc_even(a, sizeof(T));
+  if (a.nch > 1) {
+    hipLaunchKernelGGL((scan_fwd_kernel<T, S, true>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    if (const int32_t rc = pnp_check_launch("scan_fwd_kernel (chunks)")) return rc;
+    if (const int32_t rc = chain(a, a.state, S, 0, st)) return rc;
+  }
+  hipLaunchKernelGGL((scan_fwd_kernel<T, S, false>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+  return pnp_check_launch("scan_fwd_kernel");
+}
+
+template <typename T, int S> int32_t run_scan_bwd(ScanBwdArgs a, int64_t blocks, hipStream_t st) {
+  constexpr int E = tile_b(S) / S, V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
+  ScanArgs& f = a.f;
+  f.wide = f.per % V == 0 && f.dim % V == 0 && even(f.u, f.ub, f.ut, V, sizeof(T)) && even(f.delta, f.db, f.dt, V, sizeof(T)) &&
+           even(f.z, f.zb, f.zt, V, sizeof(T)) && even(a.dout, a.ob, a.ot, V, sizeof(T)) && even(a.du, 0, 0, V, sizeof(T)) &&
+           even(a.ddelta, 0, 0, V, sizeof(T)) && even(a.dz, 0, 0, V, sizeof(T));
+  f.wide_bc = bc_even(f, sizeof(T));
+  if (f.nch > 1) {
+    hipLaunchKernelGGL((scan_bwd_kernel<T, S, true>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    if (const int32_t rc = pnp_check_launch("scan_bwd_kernel (chunks)")) return rc;
+    if (const int32_t rc = chain(f, a.dlast, S, 1, st)) return rc;
+  }
+  hipLaunchKernelGGL((scan_bwd_kernel<T, S, false>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+  if (const int32_t rc = pnp_check_launch("scan_bwd_kernel")) return rc;
+  const int64_t rows = f.B * f.L * f.groups, n = ceil_div(rows * 8 * S, NT);
+  if (n) {
+    hipLaunchKernelGGL((scan_bc_kernel<T>), dim3((unsigned)(n < (1 << 22) ? n : (1 << 22))), dim3(NT), 0, st, a.bc, rows, f.N, 4 * S, f.tiles,
+                       (T*)a.dB, (T*)a.dC);
+    if (const int32_t rc = pnp_check_launch("scan_bc_kernel")) return rc;
+  }
+  hipLaunchKernelGGL(scan_sums_kernel, dim3((unsigned)ceil_div((int64_t)f.dim * (f.N + 2), 64)), dim3(1024), 0, st, a.part, f.B * f.nch, f.dim,
+                     f.N, a.dA, a.dD, a.dbias);
+  return pnp_check_launch("scan_sums_kernel");
+}
+
+template <typename T, int S> int32_t run_step(ScanArgs a, hipStream_t st) {
+  a.wide_bc = bc_even(a, sizeof(T));
+  const bool w4 = a.N == 4 * S && aligned_to(a.A, 16) && aligned_to(a.last, 16) && (!a.state || aligned_to(a.state, 16));
+  const int64_t n = ceil_div(a.B * a.dim * S, NT);
+  const unsigned grid = (unsigned)(n < (1 << 22) ? n : (1 << 22));
+  if (w4) hipLaunchKernelGGL((scan_step_kernel<T, S, true>), dim3(grid), dim3(NT), 0, st, a);
+  else hipLaunchKernelGGL((scan_step_kernel<T, S, false>), dim3(grid), dim3(NT), 0, st, a);
+  return pnp_check_launch("scan_step_kernel");
+}
+
+}  // namespace
+}  // namespace seq
+
+using namespace seq;
+
+extern "C" int64_t pnp_scan_ckpt_floats(const pnp_scan_desc* d) {
+  if (!scan_ok(d)) {
+    pnp_set_error("pnp_scan_ckpt_floats: bad shape or type");
+    return PNP_ERR_ARG;
+  }
+  const Plan p = plan(d);
+  return d->B * p.nck * d->dim * (int64_t)(4 * p.S);
+}
+
+extern "C" int64_t pnp_scan_workspace(const pnp_scan_desc* d) {
+  if (!scan_ok(d)) {
+    pnp_set_error("pnp_scan_workspace: bad shape or type");
+    return PNP_ERR_ARG;
+  }
+  return split_floats(d, plan(d));
+}
+
+static int32_t scan_check(const pnp_scan_desc* d, const Plan& p, const char* fn) {
+  if (!d->A || (d->B && d->L && (!d->u || !d->delta || !d->Bm || !d->Cm))) {
+    pnp_set_error("%s: null buffer", fn);
+    return PNP_ERR_ARG;
+  }
+  if (p.blocks >= (1 << 24) || d->B * (int64_t)d->dim * p.S >= ((int64_t)1 << 30)) {
+    pnp_set_error("%s: too many sequences for one launch", fn);
+    return PNP_ERR_ARG;
+  }
+  if (d->ckpt && d->ckpt_floats < pnp_scan_ckpt_floats(d)) {
+    pnp_set_error("%s: ckpt too small", fn);
+    return PNP_ERR_ARG;
+  }
+  if ((d->ckpt && !aligned_to(d->ckpt, 16)) || (d->workspace && !aligned_to(d->workspace, 16))) {
+    pnp_set_error("%s: ckpt and workspace are aligned to 16 bytes", fn);
+    return PNP_ERR_ARG;
+  }
+  return PNP_OK;
+}
+
+extern "C" int32_t pnp_selective_scan(const pnp_scan_desc* d, void* stream) {
+  const char* fn = "pnp_selective_scan";
+  if (!scan_ok(d)) {
+    pnp_set_error("%s: bad shape or type", fn);
+    return PNP_ERR_ARG;
+  }
+  if (!d->B || (!d->L && !d->last_state)) return PNP_OK;
+  const Plan p = plan(d);
+  if (const int32_t rc = scan_check(d, p, fn)) return rc;
+  if (d->L && !d->out) {
+    pnp_set_error("%s: null buffer", fn);
+    return PNP_ERR_ARG;
+  }
+  const int64_t need = split_floats(d, p);
+  if (need && (!d->workspace || d->workspace_floats < need)) {
+    pnp_set_error("%s: workspace too small", fn);
+    return PNP_ERR_ARG;
+  }
+  const ScanArgs a = scan_args(d, p, d->workspace);
+  const hipStream_t st = (hipStream_t)stream;
+  return SEQ_BY_TYPE(d->type, T, return BY_LANES(p.S, S, return (run_scan<T, S>(a, p.blocks, st))));
+}
+
+extern "C" int64_t pnp_scan_bwd_workspace(const pnp_scan_bwd_desc* d) {
+  if (!d || !scan_ok(&d->f)) {
+    pnp_set_error("pnp_scan_bwd_workspace: bad shape or type");
+    return PNP_ERR_ARG;
+  }
+  const pnp_scan_desc& f = d->f;
+  const Plan p = plan(&f);
+  return split_floats(&f, p) + f.B * p.nch * f.dim * (int64_t)(f.N + 2) + p.tiles * f.B * f.L * f.groups * (int64_t)(8 * p.S);
+}
+
+extern "C" int32_t pnp_selective_scan_bwd(const pnp_scan_bwd_desc* d, void* stream) {
+  const char* fn = "pnp_selective_scan_bwd";
+  if (!d || !scan_ok(&d->f)) {
+    pnp_set_error("%s: bad shape or type", fn);
+    return PNP_ERR_ARG;
+  }
+  const pnp_scan_desc& f = d->f;
+  const Plan p = plan(&f);
+  if (const int32_t rc = scan_check(&f, p, fn)) return rc;
+  if (!d->dA || (f.B && f.L && (!f.ckpt || !d->dout || !d->du || !d->ddelta || !d->dB || !d->dC || !f.z != !d->dz))) {
+    pnp_set_error("%s: null buffer", fn);
+    return PNP_ERR_ARG;
+  }
+  const int64_t need = pnp_scan_bwd_workspace(d);
+  if (need && (!d->workspace || !aligned_to(d->workspace, 16) || d->workspace_floats < need)) {
+    pnp_set_error("%s: workspace too small", fn);
+    return PNP_ERR_ARG;
+  }
+  const hipStream_t st = (hipStream_t)stream;
+  ScanBwdArgs a{};
+  a.f = scan_args(&f, p, d->workspace);
+  a.dout = d->dout; a.ob = d->dout_bstride; a.ot = d->dout_tstride; a.dlast = d->dlast;
+  a.du = d->du; a.ddelta = d->ddelta; a.dz = d->dz; a.dB = d->dB; a.dC = d->dC;
+  a.dA = d->dA; a.dD = d->dD; a.dbias = d->ddelta_bias; a.dstate = d->dstate;
+  a.part = d->workspace + split_floats(&f, p);
+  a.bc = a.part + f.B * p.nch * f.dim * (int64_t)(f.N + 2);
+  if (!f.B) {
+    hipLaunchKernelGGL(scan_sums_kernel, dim3((unsigned)ceil_div((int64_t)f.dim * (f.N + 2), 64)), dim3(1024), 0, st, (const float*)nullptr,
+                       (int64_t)0, f.dim, f.N, a.dA, a.dD, a.dbias);
+    return pnp_check_launch("scan_sums_kernel");
+  }
+  return SEQ_BY_TYPE(f.type, T, return BY_LANES(p.S, S, return (run_scan_bwd<T, S>(a, p.blocks, st))));
+}
+
+extern "C" int32_t pnp_selective_scan_step(const pnp_scan_desc* d, void* stream) {
+  const char* fn = "pnp_selective_scan_step";
+  if (!scan_ok(d) || d->L != 1) {
+    pnp_set_error("%s: bad shape or type", fn);
+    return PNP_ERR_ARG;
+  }
+  if (!d->B) return PNP_OK;
+  if (!d->A || !d->u || !d->delta || !d->Bm || !d->Cm || !d->out || !d->last_state) {
+    pnp_set_error("%s: null buffer", fn);
+    return PNP_ERR_ARG;
+  }
+  Plan p{};
+  p.S = lanes_of(d->N);
+  p.nch = 1;
+  const ScanArgs a = scan_args(d, p, nullptr);
+  const hipStream_t st = (hipStream_t)stream;
+  return SEQ_BY_TYPE(d->type, T, return BY_LANES(p.S, S, return (run_step<T, S>(a, st))));
+}

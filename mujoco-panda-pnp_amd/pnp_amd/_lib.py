@@ -22,6 +22,10 @@ EXPORTS = [
     "pnp_env_step", "pnp_env_step_f64", "pnp_env_evaluate", "pnp_env_evaluate_f64",
     "pnp_slerp_track_f64", "pnp_env_queue_status", "pnp_tqc_workspace_floats", "pnp_tqc_param_counts",
     "pnp_tqc_update", "pnp_tqc_update_phase", "pnp_tqc_sample", "pnp_tqc_sample_draw",
+    "pnp_rms_norm", "pnp_rms_norm_bwd", "pnp_rms_norm_bwd_workspace", "pnp_quantize_rows", "pnp_matmul_i8",
+    "pnp_causal_conv", "pnp_causal_conv_bwd", "pnp_causal_conv_bwd_workspace", "pnp_causal_conv_step",
+    "pnp_selective_scan", "pnp_selective_scan_bwd", "pnp_selective_scan_step", "pnp_scan_ckpt_floats",
+    "pnp_scan_workspace", "pnp_scan_bwd_workspace",
 ]
 
 STATE_FIELDS = ("qpos", "qvel", "ctrl", "mocap_pos", "mocap_quat", "qacc_warmstart", "time", "warn")
@@ -90,6 +94,60 @@ class PnpTqcReplay(C.Structure):
                [("rows", C.c_int32), ("n_envs", C.c_int32), ("obs_dim", C.c_int32), ("act_dim", C.c_int32),
                 ("n_keys", C.c_int32), ("key_dim", C.c_int32 * 4), ("mean", C.c_void_p * 4), ("var", C.c_void_p * 4),
                 ("clip_obs", C.c_double), ("norm_eps", C.c_double)]
+
+
+# ---- sequence operators (include/pnp.h; pnp_amd/seqops.py)
+_P, _I32, _I64 = C.c_void_p, C.c_int32, C.c_int64
+
+
+class PnpNormDesc(C.Structure):
+    """include/pnp.h pnp_norm_desc."""
+    _fields_ = [("rows", _I64), ("dim", _I32), ("type", _I32), ("res_type", _I32), ("eps", C.c_float), ("x", _P),
+                ("residual", _P), ("x_stride", _I64), ("r_stride", _I64), ("weight", _P), ("y", _P), ("s", _P),
+                ("rstd", _P), ("q", _P), ("q_stride", _I64), ("scale", _P)]
+
+
+class PnpNormBwdDesc(C.Structure):
+    """include/pnp.h pnp_norm_bwd_desc."""
+    _fields_ = [("rows", _I64), ("dim", _I32), ("type", _I32), ("res_type", _I32), ("dy", _P), ("ds", _P), ("s", _P),
+                ("dy_stride", _I64), ("ds_stride", _I64), ("s_stride", _I64), ("weight", _P), ("rstd", _P), ("dx", _P),
+                ("dres", _P), ("dweight", _P), ("workspace", _P), ("workspace_floats", _I64)]
+
+
+class PnpI8Desc(C.Structure):
+    """include/pnp.h pnp_i8_desc."""
+    _fields_ = [("M", _I64), ("N", _I32), ("K", _I32), ("out_type", _I32), ("pad", _I32), ("q", _P), ("wq", _P),
+                ("q_stride", _I64), ("wq_stride", _I64), ("scale", _P), ("wscale", _P), ("bias", _P), ("out", _P)]
+
+
+class PnpConvDesc(C.Structure):
+    """include/pnp.h pnp_conv_desc."""
+    _fields_ = [("B", _I64), ("L", _I64), ("dim", _I32), ("width", _I32), ("type", _I32), ("silu", _I32), ("x", _P),
+                ("x_bstride", _I64), ("x_tstride", _I64), ("weight", _P), ("bias", _P), ("starts", _P), ("state", _P),
+                ("y", _P), ("last_state", _P)]
+
+
+class PnpConvBwdDesc(C.Structure):
+    """include/pnp.h pnp_conv_bwd_desc."""
+    _fields_ = [("f", PnpConvDesc), ("dy", _P), ("dlast", _P), ("dy_bstride", _I64), ("dy_tstride", _I64), ("dx", _P),
+                ("dstate", _P), ("dweight", _P), ("dbias", _P), ("workspace", _P), ("workspace_floats", _I64)]
+
+
+class PnpScanDesc(C.Structure):
+    """include/pnp.h pnp_scan_desc."""
+    _fields_ = [("B", _I64), ("L", _I64), ("dim", _I32), ("N", _I32), ("groups", _I32), ("type", _I32)] + \
+               [(f, _P) for f in ("u", "delta", "z", "Bm", "Cm")] + \
+               [(f, _I64) for f in ("u_bstride", "u_tstride", "delta_bstride", "delta_tstride", "z_bstride", "z_tstride",
+                                    "B_bstride", "B_tstride", "C_bstride", "C_tstride")] + \
+               [(f, _P) for f in ("A", "D", "delta_bias", "state", "starts", "out", "last_state", "ckpt", "workspace")] + \
+               [("ckpt_floats", _I64), ("workspace_floats", _I64)]
+
+
+class PnpScanBwdDesc(C.Structure):
+    """include/pnp.h pnp_scan_bwd_desc."""
+    _fields_ = [("f", PnpScanDesc), ("dout", _P), ("dout_bstride", _I64), ("dout_tstride", _I64)] + \
+               [(f, _P) for f in ("dlast", "du", "ddelta", "dz", "dB", "dC", "dA", "dD", "ddelta_bias", "dstate", "workspace")] + \
+               [("workspace_floats", _I64)]
 
 
 # debug record layout (include/pnp.h PNP_DBG_*)
@@ -185,6 +243,23 @@ def load():
     L.pnp_tqc_sample.restype = I32
     L.pnp_tqc_sample_draw.argtypes = [C.POINTER(PnpTqcReplay), C.c_uint64, P, I32, P, P, P, P, P, P, P, P, P]
     L.pnp_tqc_sample_draw.restype = I32
+    for name, desc in (("pnp_rms_norm", PnpNormDesc), ("pnp_rms_norm_bwd", PnpNormBwdDesc), ("pnp_matmul_i8", PnpI8Desc),
+                       ("pnp_causal_conv", PnpConvDesc), ("pnp_causal_conv_bwd", PnpConvBwdDesc),
+                       ("pnp_selective_scan", PnpScanDesc), ("pnp_selective_scan_bwd", PnpScanBwdDesc),
+                       ("pnp_selective_scan_step", PnpScanDesc)):
+        f = getattr(L, name)
+        f.argtypes = [C.POINTER(desc), P]
+        f.restype = I32
+    for name, desc in (("pnp_rms_norm_bwd_workspace", PnpNormBwdDesc), ("pnp_causal_conv_bwd_workspace", PnpConvBwdDesc),
+                       ("pnp_scan_ckpt_floats", PnpScanDesc), ("pnp_scan_workspace", PnpScanDesc),
+                       ("pnp_scan_bwd_workspace", PnpScanBwdDesc)):
+        f = getattr(L, name)
+        f.argtypes = [C.POINTER(desc)]
+        f.restype = C.c_int64
+    L.pnp_quantize_rows.argtypes = [P, C.c_int64, I32, C.c_int64, I32, P, C.c_int64, P, P]
+    L.pnp_quantize_rows.restype = I32
+    L.pnp_causal_conv_step.argtypes = [P, C.c_int64, P, P, P, P, C.c_int64, I32, I32, I32, I32, P, P]
+    L.pnp_causal_conv_step.restype = I32
     if L.pnp_abi_version() != ABI_VERSION:
         raise PnpError(f"libpnp ABI {L.pnp_abi_version()} != binding ABI {ABI_VERSION}")
     if L.pnp_env_params_size() != C.sizeof(PnpEnvParams):
