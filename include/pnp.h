@@ -620,8 +620,9 @@ int32_t pnp_causal_conv_step(const void* x, int64_t x_stride, void* state, const
  * h[t] = a * h[t - 1] + dt * u * Bm[b][t][g][n]; y = sum_n Cm[b][t][g][n] * h + D[d] * u;
  * out = y * z * sigmoid(z) (y where z is NULL).  Channel d belongs to group g = d / (dim / groups).
  * h before t = 0: state [B][dim][N] (zeros where NULL); last_state the h after the last token.
- * N 1 .. 64.  ckpt (may be NULL; pnp_scan_ckpt_floats): the states the gradient starts its pieces
+ * N 1 .. 64; token strides up to PNP_SCAN_MAX_TSTRIDE elements.  ckpt (may be NULL; pnp_scan_ckpt_floats): the states the gradient starts its pieces
  * from.  workspace (pnp_scan_workspace floats) serves the split over the length. */
+#define PNP_SCAN_MAX_TSTRIDE (1 << 24)
 typedef struct pnp_scan_desc {
   int64_t B, L;
   int32_t dim, N, groups, type;

@@ -21,6 +21,8 @@
 // each chunk's state from a zero start and its decay (exp(A sum dt): one number a channel), a small
 // kernel chains them, and the main pass starts every chunk from its true state.  The gradient does the
 // same from the other end.
+#include <type_traits>
+
 #include "seq_dev.h"
 
 namespace seq {
@@ -28,9 +30,11 @@ namespace {
 
 constexpr int NT = 256;
 
-// tile of the forward, and tile of the gradient (its states stay in registers: 4 * 2 a token)
+// tokens of a tile, forward and gradient; the gradient's inner tile, whose states and decays stay in
+// registers (8 a token), is TR tokens: the forward keeps a state for each
 constexpr int tile_f(int S) { return S == 1 ? 8 : S == 2 ? 16 : 32; }
 constexpr int tile_b(int S) { return S == 1 ? 8 : 16; }
+constexpr int TR = 8;
 
 struct ScanArgs {
   int64_t B, L;
@@ -38,7 +42,7 @@ struct ScanArgs {
   int tiles;                     // workgroups across a group's channels
   int nch;                       // chunks of the length
   int64_t chunk;                 // tokens of a chunk, a multiple of the tile
-  int64_t nck;                   // states kept a sequence: one each tile_b tokens
+  int64_t nck;                   // states kept a sequence: one each TR tokens
   const void *u, *delta, *z, *Bm, *Cm;
   int64_t ub, ut, db, dt, zb, zt, Bb, Bt, Cb, Ct;
   const float *A, *D, *bias, *state;
@@ -47,8 +51,6 @@ struct ScanArgs {
   float *last, *ckpt;
   float *hin;                    // [B][nch][dim][4 S] states at the chunks' starts (nch > 1)
   float *dsum;                   // [B][nch][dim] sums of dt; NaN where the chunk holds a start
-  int wide;                      // packs of channels are aligned
-  int wide_bc;                   // packs of 4 states of B and C are aligned
 };
 
 struct Where { int64_t b, row; int chunk, g, c0, ch; };   // c0: first channel within the group; row: b * nch + chunk
@@ -66,43 +68,35 @@ template <int S> __device__ __forceinline__ Where where(const ScanArgs& a) {
   return w;
 }
 
-// E neighbouring channels of one token, as fp32; channels past the group's and tokens past the end as 0
-template <int E, typename T>
-__device__ __forceinline__ void load_channels(const T* p, int left, bool wide, float (&v)[E]) {
-  constexpr int V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
-  if (wide && left >= E) {
+// E neighbouring channels of one token; those past `left` as 0.  WIDE: packs of V are whole or past it,
+// and aligned.
+template <typename T, int E> struct Raw { T v[E]; };
+template <int E, bool WIDE, typename T> __device__ __forceinline__ void load_channels(const T* p, int left, Raw<T, E>& o) {
+  constexpr int V = !WIDE ? 1 : E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
 #pragma unroll
-    for (int i = 0; i < E; i += V) {
-      float w[V];
-      load_f<V>(p + i, w);
+  for (int i = 0; i < E; i += V) {
+    Pack<T, V> w;
 #pragma unroll
-      for (int k = 0; k < V; k++) v[i + k] = w[k];
-    }
-  } else {
+    for (int k = 0; k < V; k++) w.v[k] = (T)0.f;
+    if (i < left) w = *reinterpret_cast<const Pack<T, V>*>(p + i);
 #pragma unroll
-    for (int i = 0; i < E; i++) v[i] = i < left ? to_f(p[i]) : 0.f;
+    for (int k = 0; k < V; k++) o.v[i + k] = w.v[k];
   }
 }
-template <int E, typename T> __device__ __forceinline__ void store_channels(T* p, int left, bool wide, const float (&v)[E]) {
-  constexpr int V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
-  if (wide && left >= E) {
+template <int E, bool WIDE, typename T> __device__ __forceinline__ void store_channels(T* p, int left, const float (&v)[E]) {
+  constexpr int V = !WIDE ? 1 : E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
 #pragma unroll
-    for (int i = 0; i < E; i += V) {
-      float w[V];
+  for (int i = 0; i < E; i += V) {
+    float w[V];
 #pragma unroll
-      for (int k = 0; k < V; k++) w[k] = v[i + k];
-      store_f<V>(p + i, w);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; i++)
-      if (i < left) p[i] = from_f<T>(v[i]);
+    for (int k = 0; k < V; k++) w[k] = v[i + k];
+    if (i < left) store_f<V>(p + i, w);
   }
 }
 
 // 4 states of B or C of one token, zeros past N
-template <typename T> __device__ __forceinline__ float4 load_states(const T* p, int n, int N, bool wide) {
-  if (wide) {   // N is a multiple of 4: a pack is whole or not there
+template <bool WIDE, typename T> __device__ __forceinline__ float4 load_states(const T* p, int n, int N) {
+  if (WIDE) {   // N is a multiple of 4: a pack is whole or not there
     if (n >= N) return float4{0.f, 0.f, 0.f, 0.f};
     float v[4];
     load_f<4>(p + n, v);
@@ -120,6 +114,38 @@ __device__ __forceinline__ void load_state4(const float* p, int n, int N, float 
   for (int i = 0; i < 4; i++) h[i] = n + i < N ? p[n + i] : 0.f;
 }
 
+// p + elems (the same in the workgroup: a scalar address) + bytes (the thread's 32-bit offset): the form of
+// address that costs one register.  The compiler would add the offset to the tensor's base once and keep
+// that, two registers a tensor, if it saw through the scalar sum.
+#define SEQ_GLOBAL __attribute__((address_space(1)))
+template <typename T> __device__ __forceinline__ const T* at(const void* p, int64_t elems, uint32_t bytes) {
+  uint64_t base = (uint64_t)(static_cast<const T*>(p) + elems);
+  asm("" : "+s"(base));
+  return (const T*)(const SEQ_GLOBAL T*)((const SEQ_GLOBAL char*)base + bytes);
+}
+template <typename T> __device__ __forceinline__ T* at(void* p, int64_t elems, uint32_t bytes) {
+  uint64_t base = (uint64_t)(static_cast<T*>(p) + elems);
+  asm("" : "+s"(base));
+  return (T*)(SEQ_GLOBAL T*)((SEQ_GLOBAL char*)base + bytes);
+}
+
+// the thread's packs of 4 states of a tile's B, then C
+template <typename T, int S, int TT, int NBC, bool WIDE>
+__device__ __forceinline__ void load_bc(const ScanArgs& a, int64_t b, int g, int64_t t, int64_t t1, float4 (&o)[(NBC + NT - 1) / NT]) {
+  constexpr int H = TT * S;   // packs of B
+#pragma unroll
+  for (int k = 0; k < (NBC + NT - 1) / NT; k++) {
+    const int i = k * NT + threadIdx.x, r = i % H, n = 4 * (r % S);
+    const bool in = t + r / S < t1;
+    o[k] = float4{0.f, 0.f, 0.f, 0.f};
+    if (i < H) {
+      if (in) o[k] = load_states<WIDE>(at<T>(a.Bm, b * a.Bb + (int64_t)g * a.N + t * a.Bt, (uint32_t)(r / S * a.Bt) * sizeof(T)), n, a.N);
+    } else if (i < NBC) {
+      if (in) o[k] = load_states<WIDE>(at<T>(a.Cm, b * a.Cb + (int64_t)g * a.N + t * a.Ct, (uint32_t)(r / S * a.Ct) * sizeof(T)), n, a.N);
+    }
+  }
+}
+
 // the tile's tokens that start a sequence, a bit each (TT <= 32), the same in every wave
 template <int TT> __device__ __forceinline__ uint32_t start_bits(const ScanArgs& a, int64_t b, int64_t t0, int64_t t1) {
   if (!a.starts) return 0;
@@ -128,9 +154,13 @@ template <int TT> __device__ __forceinline__ uint32_t start_bits(const ScanArgs&
   return (uint32_t)__builtin_amdgcn_ballot_w64(s);
 }
 
+// Of G tokens' values, each the same in the S lanes of a channel, a lane keeps the one of token `ng`: G tokens
+// leave by one store of all lanes (G = S up to the inner tile).
+constexpr int group_of(int S) { return S < TR ? S : TR; }
+
 // STATE: the chunk's state from a zero start and its decay alone
-template <typename T, int S, bool STATE> __global__ __launch_bounds__(NT) void scan_fwd_kernel(ScanArgs a) {
-  constexpr int TT = tile_f(S), TB = tile_b(S), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S;
+template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__(NT) void scan_fwd_kernel(ScanArgs a) {
+  constexpr int TT = tile_f(S), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S, G = group_of(S);
   __shared__ float2 dd[TT][CW];
   __shared__ float4 sB[TT][S], sC[STATE ? 1 : TT][S];
   const Where w = where<S>(a);
@@ -140,11 +170,9 @@ template <typename T, int S, bool STATE> __global__ __launch_bounds__(NT) void s
   const int left = a.per - w.c0 - lc;                               // channels from there to the group's end
   const bool on = w.c0 + cl < a.per;
   const int64_t t0 = (int64_t)w.chunk * a.chunk, t1 = t0 + a.chunk < a.L ? t0 + a.chunk : a.L;
-  const T* u = (const T*)a.u + w.b * a.ub + w.ch + lc;
-  const T* dl = (const T*)a.delta + w.b * a.db + w.ch + lc;
-  const T* z = !STATE && a.z ? (const T*)a.z + w.b * a.zb + w.ch + lc : nullptr;
-  const T* Bm = (const T*)a.Bm + w.b * a.Bb + (int64_t)w.g * a.N;
-  const T* Cm = (const T*)a.Cm + w.b * a.Cb + (int64_t)w.g * a.N;
+  const bool z = !STATE && a.z;
+  const uint32_t ou = (uint32_t)(lt * a.ut + lc) * sizeof(T), od = (uint32_t)(lt * a.dt + lc) * sizeof(T),
+                 oz = (uint32_t)(lt * a.zt + lc) * sizeof(T), oo = (uint32_t)(lt * a.dim + lc) * sizeof(T);
 
   float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f}, dsum = 0.f;
   const int64_t ch = w.ch + (on ? cl : 0);
@@ -161,37 +189,27 @@ template <typename T, int S, bool STATE> __global__ __launch_bounds__(NT) void s
     Dv[i] = !STATE && a.D && i < left ? a.D[w.ch + lc + i] : 0.f;
     bias[i] = a.bias && i < left ? a.bias[w.ch + lc + i] : 0.f;
   }
-  float nu[E], nd[E], nz[E], cu[E], cz[E];
+  Raw<T, E> nu, nd, nz, cu, cz;
   constexpr int NBC = STATE ? TT * S : 2 * TT * S;                  // packs of 4 states a tile
   constexpr int PER = (NBC + NT - 1) / NT;
   float4 nbc[PER];
   auto fetch = [&](int64_t t) {
-    const int64_t tt = t + lt;
-    const int l = tt < t1 ? left : 0;
-    load_channels<E>(u + tt * a.ut, l, a.wide, nu);
-    load_channels<E>(dl + tt * a.dt, l, a.wide, nd);
-    if (z) load_channels<E>(z + tt * a.zt, l, a.wide, nz);
-#pragma unroll
-    for (int k = 0; k < PER; k++) {
-      const int i = k * NT + tid;
-      const bool isC = i >= TT * S;
-      const int r = isC ? i - TT * S : i;
-      const int64_t bt = t + r / S;
-      nbc[k] = float4{0.f, 0.f, 0.f, 0.f};
-      if (i < NBC && bt < t1)
-        nbc[k] = isC ? load_states(Cm + bt * a.Ct, 4 * (r % S), a.N, a.wide_bc) : load_states(Bm + bt * a.Bt, 4 * (r % S), a.N, a.wide_bc);
-    }
+    const int l = t + lt < t1 ? left : 0;
+    load_channels<E, WIDE>(at<T>(a.u, w.b * a.ub + t * a.ut + w.ch, ou), l, nu);
+    load_channels<E, WIDE>(at<T>(a.delta, w.b * a.db + t * a.dt + w.ch, od), l, nd);
+    if (z) load_channels<E, WIDE>(at<T>(a.z, w.b * a.zb + t * a.zt + w.ch, oz), l, nz);
+    load_bc<T, S, TT, NBC, WIDE>(a, w.b, w.g, t, t1, nbc);
   };
   if (t0 < t1) fetch(t0);
   for (int64_t t = t0; t < t1; t += TT) {
     const bool mine = t + lt < t1;
 #pragma unroll
     for (int i = 0; i < E; i++) {
-      const float d = mine && i < left ? softplus_f(nd[i] + bias[i]) : 0.f;
-      dd[lt][lc + i] = float2{d, d * nu[i]};
-      cu[i] = nu[i];
-      cz[i] = nz[i];
+      const float uv = to_f(nu.v[i]), d = mine && i < left ? softplus_f(to_f(nd.v[i]) + bias[i]) : 0.f;
+      dd[lt][lc + i] = float2{d, d * uv};
     }
+    cu = nu;
+    cz = nz;
 #pragma unroll
     for (int k = 0; k < PER; k++) {
       const int i = k * NT + tid;
@@ -201,15 +219,13 @@ template <typename T, int S, bool STATE> __global__ __launch_bounds__(NT) void s
     const uint32_t bits = start_bits<TT>(a, w.b, t, t1);
     __syncthreads();
     if (t + TT < t1) fetch(t + TT);
+    auto tokens = [&](auto starts, int p) {
+      float keep = 0.f;
 #pragma unroll
-    for (int p = 0; p < TT; p += TB) {
-      if (!STATE && a.ckpt && on && t + p < t1)
-        *reinterpret_cast<float4*>(a.ckpt + ((w.b * a.nck + (t + p) / TB) * a.dim + ch) * NP + 4 * ng) = float4{h[0], h[1], h[2], h[3]};
-#pragma unroll 4
-      for (int k = p; k < p + TB; k++) {
-        const float2 d = dd[k][cl];
-        const float4 b = sB[k][ng];
-        if (bits >> k & 1) {
+      for (int k = 0; k < TR; k++) {
+        const float2 d = dd[p + k][cl];
+        const float4 b = sB[p + k][ng];
+        if (starts.value && (bits >> (p + k) & 1)) {
           h[0] = h[1] = h[2] = h[3] = 0.f;
           if (STATE) dsum = __builtin_nanf("");
         }
@@ -220,21 +236,31 @@ template <typename T, int S, bool STATE> __global__ __launch_bounds__(NT) void s
         if (STATE) {
           dsum += d.x;
         } else {
-          const float4 c = sC[k][ng];
+          const float4 c = sC[p + k][ng];
           const float y = group_sum<S>(c.x * h[0] + c.y * h[1] + c.z * h[2] + c.w * h[3]);
-          if (ng == 0) dd[k][cl].x = y;   // (its dt has been read by every lane of the channel)
+          keep = ng == k % G ? y : keep;
+          // (dt of these tokens has been read by every lane of the channel)
+          if (k % G == G - 1 && (G == S || ng < G)) dd[p + k - (G - 1) + ng][cl].x = keep;
         }
       }
+    };
+#pragma unroll 1
+    for (int p = 0; p < TT; p += TR) {
+      if (!STATE && a.ckpt && on && t + p < t1)
+        *reinterpret_cast<float4*>(a.ckpt + ((w.b * a.nck + (t + p) / TR) * a.dim + ch) * NP + 4 * ng) = float4{h[0], h[1], h[2], h[3]};
+      if (bits) tokens(std::true_type(), p);
+      else tokens(std::false_type(), p);
     }
     __syncthreads();
     if (!STATE && mine) {
       float o[E];
 #pragma unroll
       for (int i = 0; i < E; i++) {
-        o[i] = dd[lt][lc + i].x + Dv[i] * cu[i];
-        if (z) o[i] *= cz[i] * sigmoid_f(cz[i]);
+        o[i] = dd[lt][lc + i].x + Dv[i] * to_f(cu.v[i]);
+        const float zv = to_f(cz.v[i]);
+        if (z) o[i] *= zv * sigmoid_f(zv);
       }
-      store_channels<E>((T*)a.out + (w.b * a.L + t + lt) * a.dim + w.ch + lc, left, a.wide, o);
+      store_channels<E, WIDE>(at<T>(a.out, (w.b * a.L + t) * a.dim + w.ch, oo), left, o);
     }
   }
   if (!on) return;
@@ -307,10 +333,10 @@ template <int S> __device__ __forceinline__ void channel_sums(float (&v)[8]) {
 }
 
 // STATE: the chunk's adjoint from a zero end and its decay alone
-template <typename T, int S, bool STATE> __global__ __launch_bounds__(NT, 2) void scan_bwd_kernel(ScanBwdArgs a) {
-  constexpr int TT = tile_b(S), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S;
+template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__(NT, 2) void scan_bwd_kernel(ScanBwdArgs a) {
+  constexpr int TT = tile_b(S), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S, G = group_of(S);
   const ScanArgs& f = a.f;
-  __shared__ float4 dd[TT][CW];                        // dt, u, dy, dt u; then sum g B, sum g (a h') A
+  __shared__ float4 dd[TT][CW];                        // dt, dy, u, dt u; then dt, dy, sum g B, sum g (a h') A
   __shared__ float yb[STATE ? 1 : TT][CW];             // sum C h
   __shared__ float4 sB[TT][S], sC[TT][S];
   __shared__ float bc[STATE ? 1 : 4][STATE ? 1 : TT][2 * NP];
@@ -321,12 +347,10 @@ template <typename T, int S, bool STATE> __global__ __launch_bounds__(NT, 2) voi
   const int left = f.per - w.c0 - lc;
   const bool on = w.c0 + cl < f.per;
   const int64_t t0 = (int64_t)w.chunk * f.chunk, t1 = t0 + f.chunk < f.L ? t0 + f.chunk : f.L;
-  const T* u = (const T*)f.u + w.b * f.ub + w.ch + lc;
-  const T* dl = (const T*)f.delta + w.b * f.db + w.ch + lc;
-  const T* z = f.z ? (const T*)f.z + w.b * f.zb + w.ch + lc : nullptr;
-  const T* dout = (const T*)a.dout + w.b * a.ob + w.ch + lc;
-  const T* Bm = (const T*)f.Bm + w.b * f.Bb + (int64_t)w.g * f.N;
-  const T* Cm = (const T*)f.Cm + w.b * f.Cb + (int64_t)w.g * f.N;
+  const bool z = f.z;
+  const uint32_t ou = (uint32_t)(lt * f.ut + lc) * sizeof(T), od = (uint32_t)(lt * f.dt + lc) * sizeof(T),
+                 oz = (uint32_t)(lt * f.zt + lc) * sizeof(T), oy = (uint32_t)(lt * a.ot + lc) * sizeof(T),
+                 oo = (uint32_t)(lt * f.dim + lc) * sizeof(T), ok = (uint32_t)(cl * NP + 4 * ng) * 4u;
 
   float A[4], A2[4], dA[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {0.f, 0.f, 0.f, 0.f}, dsum = 0.f;
   const int64_t ch = w.ch + (on ? cl : 0);
@@ -344,26 +368,15 @@ template <typename T, int S, bool STATE> __global__ __launch_bounds__(NT, 2) voi
     bias[i] = f.bias && i < left ? f.bias[w.ch + lc + i] : 0.f;
   }
   constexpr int NBC = 2 * TT * S, PER = (NBC + NT - 1) / NT;
-  float nu[E], nd[E], nz[E], no[E], cu[E], cd[E], cz[E], co[E];
-  float4 nbc[PER], nh = {0.f, 0.f, 0.f, 0.f};
+  Raw<T, E> nu, nd, nz, no, cu, cd, cz, co;
+  float4 nbc[PER];
   auto fetch = [&](int64_t t) {
-    const int64_t tt = t + lt;
-    const int l = tt < t1 ? left : 0;
-    load_channels<E>(u + tt * f.ut, l, f.wide, nu);
-    load_channels<E>(dl + tt * f.dt, l, f.wide, nd);
-    if (z) load_channels<E>(z + tt * f.zt, l, f.wide, nz);
-    load_channels<E>(dout + tt * a.ot, l, f.wide, no);
-#pragma unroll
-    for (int k = 0; k < PER; k++) {
-      const int i = k * NT + tid;
-      const bool isC = i >= TT * S;
-      const int r = isC ? i - TT * S : i;
-      const int64_t bt = t + r / S;
-      nbc[k] = float4{0.f, 0.f, 0.f, 0.f};
-      if (i < NBC && bt < t1)
-        nbc[k] = isC ? load_states(Cm + bt * f.Ct, 4 * (r % S), f.N, f.wide_bc) : load_states(Bm + bt * f.Bt, 4 * (r % S), f.N, f.wide_bc);
-    }
-    if (!STATE) nh = *reinterpret_cast<const float4*>(f.ckpt + ((w.b * f.nck + t / TT) * f.dim + ch) * NP + 4 * ng);
+    const int l = t + lt < t1 ? left : 0;
+    load_channels<E, WIDE>(at<T>(f.u, w.b * f.ub + t * f.ut + w.ch, ou), l, nu);
+    load_channels<E, WIDE>(at<T>(f.delta, w.b * f.db + t * f.dt + w.ch, od), l, nd);
+    if (z) load_channels<E, WIDE>(at<T>(f.z, w.b * f.zb + t * f.zt + w.ch, oz), l, nz);
+    load_channels<E, WIDE>(at<T>(a.dout, w.b * a.ob + t * a.ot + w.ch, oy), l, no);
+    load_bc<T, S, TT, NBC, WIDE>(f, w.b, w.g, t, t1, nbc);
   };
   const int64_t tiles = (t1 - t0 + TT - 1) / TT;
   if (tiles > 0) fetch(t0 + (tiles - 1) * TT);
@@ -372,15 +385,22 @@ template <typename T, int S, bool STATE> __global__ __launch_bounds__(NT, 2) voi
 #pragma unroll
     for (int i = 0; i < E; i++) {
       const bool in = mine && i < left;
-      const float d = in ? softplus_f(nd[i] + bias[i]) : 0.f;
-      cu[i] = nu[i];
-      cd[i] = nd[i] + bias[i];
-      cz[i] = nz[i];
-      co[i] = no[i];
-      const float dy = !in ? 0.f : z ? no[i] * nz[i] * sigmoid_f(nz[i]) : no[i];
-      dd[lt][lc + i] = float4{d, nu[i], dy, d * nu[i]};
+      const float uv = to_f(nu.v[i]), zv = to_f(nz.v[i]), ov = to_f(no.v[i]);
+      const float d = in ? softplus_f(to_f(nd.v[i]) + bias[i]) : 0.f;
+      const float dy = !in ? 0.f : z ? ov * zv * sigmoid_f(zv) : ov;
+      dd[lt][lc + i] = float4{d, dy, uv, d * uv};
     }
-    const float4 h0 = nh;
+    cu = nu;
+    cd = nd;
+    cz = nz;
+    co = no;
+    float4 hc[TT / TR];
+    if (!STATE)
+#pragma unroll
+      for (int p = 0; p < TT / TR; p++) {
+        hc[p] = float4{0.f, 0.f, 0.f, 0.f};
+        if (on && t + p * TR < t1) hc[p] = *reinterpret_cast<const float4*>(at<float>(f.ckpt, ((w.b * f.nck + t / TR + p) * f.dim + w.ch) * NP, ok));
+      }
 #pragma unroll
     for (int k = 0; k < PER; k++) {
       const int i = k * NT + tid;
@@ -395,10 +415,10 @@ template <typename T, int S, bool STATE> __global__ __launch_bounds__(NT, 2) voi
       for (int k = TT - 1; k >= 0; k--) {
         const float4 d = dd[k][cl];
         const float4 c = sC[k][ng];
-        g[0] = exp2_f(d.x * A2[0]) * (g[0] + c.x * d.z);
-        g[1] = exp2_f(d.x * A2[1]) * (g[1] + c.y * d.z);
-        g[2] = exp2_f(d.x * A2[2]) * (g[2] + c.z * d.z);
-        g[3] = exp2_f(d.x * A2[3]) * (g[3] + c.w * d.z);
+        g[0] = exp2_f(d.x * A2[0]) * (g[0] + c.x * d.y);
+        g[1] = exp2_f(d.x * A2[1]) * (g[1] + c.y * d.y);
+        g[2] = exp2_f(d.x * A2[2]) * (g[2] + c.z * d.y);
+        g[3] = exp2_f(d.x * A2[3]) * (g[3] + c.w * d.y);
         dsum += d.x;
         if (bits >> k & 1) {
           g[0] = g[1] = g[2] = g[3] = 0.f;
@@ -407,60 +427,74 @@ template <typename T, int S, bool STATE> __global__ __launch_bounds__(NT, 2) voi
       }
       __syncthreads();
     } else {
-      float e[TT][4], h[TT + 1][4];
-      h[0][0] = h0.x; h[0][1] = h0.y; h[0][2] = h0.z; h[0][3] = h0.w;
+      // the inner tile at p from the state h0: its states and decays forward, kept, then the adjoint back.
+      // starts: a start's decay is 0 whatever the state (0 times infinity is NaN)
+      auto tokens = [&](auto starts, int p, const float4 h0) {
+        constexpr bool ST = decltype(starts)::value;
+        const uint32_t marks = bits >> p;
+        float e[TR][4], h[TR + 1][4], keep = 0.f;
+        h[0][0] = h0.x; h[0][1] = h0.y; h[0][2] = h0.z; h[0][3] = h0.w;
 #pragma unroll
-      for (int k = 0; k < TT; k++) {
-        const float4 d = dd[k][cl];
-        const float4 b = sB[k][ng];
-        const float bv[4] = {b.x, b.y, b.z, b.w};
+        for (int k = 0; k < TR; k++) {
+          const float4 d = dd[p + k][cl];
+          const float4 b = sB[p + k][ng], c = sC[p + k][ng];
+          const float bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
+          const bool st = ST && (marks >> k & 1);
+          float y = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) e[k][i] = exp2_f(d.x * A2[i]);
-        float ah[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) ah[i] = e[k][i] * h[k][i];
-        if (bits >> k & 1) ah[0] = ah[1] = ah[2] = ah[3] = 0.f;   // (whatever the state: 0 times infinity is NaN)
-#pragma unroll
-        for (int i = 0; i < 4; i++) h[k + 1][i] = ah[i] + d.w * bv[i];
-        if (z) {
-          const float4 c = sC[k][ng];
-          const float y = group_sum<S>(c.x * h[k + 1][0] + c.y * h[k + 1][1] + c.z * h[k + 1][2] + c.w * h[k + 1][3]);
-          if (ng == 0) yb[k][cl] = y;
+          for (int i = 0; i < 4; i++) {
+            e[k][i] = exp2_f(d.x * A2[i]);
+            const float ah = e[k][i] * h[k][i];
+            h[k + 1][i] = (st ? 0.f : ah) + d.w * bv[i];
+            y += cv[i] * h[k + 1][i];
+          }
+          y = group_sum<S>(y);
+          keep = ng == k % G ? y : keep;
+          if (k % G == G - 1 && (G == S || ng < G)) yb[p + k - (G - 1) + ng][cl] = keep;
         }
-      }
+        // the tile is read again rather than held, 12 registers a token (the compiler must not see that it is the same)
+        asm volatile("" : "+s"(p));
+        float k1 = 0.f, k2 = 0.f;
 #pragma unroll
-      for (int k = TT - 1; k >= 0; k--) {
-        const float4 d = dd[k][cl];
-        const float4 b = sB[k][ng], c = sC[k][ng];
-        const float bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
-        float s1 = 0.f, s2 = 0.f, v[8], ah[4];
+        for (int k = TR - 1; k >= 0; k--) {
+          const float4 d = dd[p + k][cl];
+          const float4 b = sB[p + k][ng], c = sC[p + k][ng];
+          const float bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
+          const bool st = ST && (marks >> k & 1);
+          float s1 = 0.f, s2 = 0.f, v[8];
 #pragma unroll
-        for (int i = 0; i < 4; i++) ah[i] = e[k][i] * h[k][i];
-        if (bits >> k & 1) ah[0] = ah[1] = ah[2] = ah[3] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          g[i] += cv[i] * d.z;
-          v[4 + i] = h[k + 1][i] * d.z;
-          v[i] = g[i] * d.w;
-          s1 += g[i] * bv[i];
-          const float gah = g[i] * ah[i];
-          s2 += gah * A[i];
-          dA[i] += gah * d.x;
-          g[i] *= e[k][i];
-        }
-        if (bits >> k & 1) g[0] = g[1] = g[2] = g[3] = 0.f;
-        s1 = group_sum<S>(s1);
-        s2 = group_sum<S>(s2);
-        if (ng == 0) *reinterpret_cast<float2*>(&dd[k][cl]) = float2{s1, s2};
-        channel_sums<S>(v);
-        if (S >= 8 || (lane & 7) < S) {
-          const int at = (lane >> 5) * NP + 4 * ng + 2 * (lane >> 4 & 1);
-          if (S < 16) bc[wave][k][at + (lane >> 3 & 1)] = v[0];
-          else {
-            bc[wave][k][at] = v[0];
-            bc[wave][k][at + 1] = v[1];
+          for (int i = 0; i < 4; i++) {
+            g[i] += cv[i] * d.y;
+            v[4 + i] = h[k + 1][i] * d.y;
+            v[i] = g[i] * d.w;
+            s1 += g[i] * bv[i];
+            float ek = e[k][i];
+            asm("" : "+v"(ek));   // (e h is multiplied again: kept from above it would take 4 registers a token)
+            const float ah = ek * h[k][i], gah = g[i] * (st ? 0.f : ah);
+            s2 += gah * A[i];
+            dA[i] += gah * d.x;
+            g[i] = st ? 0.f : g[i] * ek;
+          }
+          s1 = group_sum<S>(s1);
+          s2 = group_sum<S>(s2);
+          k1 = ng == k % G ? s1 : k1;
+          k2 = ng == k % G ? s2 : k2;
+          if (k % G == 0 && (G == S || ng < G)) *reinterpret_cast<float2*>(&dd[p + k + ng][cl].z) = float2{k1, k2};
+          channel_sums<S>(v);
+          if (S >= 8 || (lane & 7) < S) {
+            const int o = (lane >> 5) * NP + 4 * ng + 2 * (lane >> 4 & 1);
+            if (S < 16) bc[wave][p + k][o + (lane >> 3 & 1)] = v[0];
+            else {
+              bc[wave][p + k][o] = v[0];
+              bc[wave][p + k][o + 1] = v[1];
+            }
           }
         }
+      };
+#pragma unroll
+      for (int q = TT / TR - 1; q >= 0; q--) {
+        if (bits) tokens(std::true_type(), q * TR, hc[q]);
+        else tokens(std::false_type(), q * TR, hc[q]);
       }
       __syncthreads();
       if (mine) {
@@ -468,20 +502,18 @@ template <typename T, int S, bool STATE> __global__ __launch_bounds__(NT, 2) voi
 #pragma unroll
         for (int i = 0; i < E; i++) {
           const float4 s = dd[lt][lc + i];
-          const float dy = s.z, dtv = softplus_f(cd[i]);
-          du[i] = Dv[i] * dy + dtv * s.x;
-          dr[i] = i < left ? (s.y + cu[i] * s.x) * sigmoid_f(cd[i]) : 0.f;
-          dD[i] += dy * cu[i];
+          const float dt = s.x, dy = s.y, uv = to_f(cu.v[i]);
+          du[i] = Dv[i] * dy + dt * s.z;
+          dr[i] = i < left ? (s.w + uv * s.z) * sigmoid_f(to_f(cd.v[i]) + bias[i]) : 0.f;
+          dD[i] += dy * uv;
           dbias[i] += dr[i];
-          if (z) {
-            const float sg = sigmoid_f(cz[i]);
-            dz[i] = co[i] * (yb[lt][lc + i] + Dv[i] * cu[i]) * (sg * (1.f + cz[i] * (1.f - sg)));
-          }
+          const float zv = to_f(cz.v[i]), sg = sigmoid_f(zv);
+          dz[i] = to_f(co.v[i]) * (yb[lt][lc + i] + Dv[i] * uv) * (sg * (1.f + zv * (1.f - sg)));
         }
-        const int64_t at = (w.b * f.L + t + lt) * f.dim + w.ch + lc;
-        store_channels<E>((T*)a.du + at, left, f.wide, du);
-        store_channels<E>((T*)a.ddelta + at, left, f.wide, dr);
-        if (z) store_channels<E>((T*)a.dz + at, left, f.wide, dz);
+        const int64_t o = (w.b * f.L + t) * f.dim + w.ch;
+        store_channels<E, WIDE>(at<T>(a.du, o, oo), left, du);
+        store_channels<E, WIDE>(at<T>(a.ddelta, o, oo), left, dr);
+        if (z) store_channels<E, WIDE>(at<T>(a.dz, o, oo), left, dz);
       }
       // this workgroup's share of dB and dC
       const int64_t tile = w.c0 / CW;
@@ -589,8 +621,8 @@ template <typename T, int S, bool W4> __global__ __launch_bounds__(NT) void scan
     const float raw = to_f(((const T*)a.delta)[b * a.db + d]) + (a.bias ? a.bias[d] : 0.f);
     const float zv = a.z ? to_f(((const T*)a.z)[b * a.zb + d]) : 0.f;
     const int g = d / a.per;
-    const float4 bm = load_states((const T*)a.Bm + b * a.Bb + (int64_t)g * a.N, 4 * ng, a.N, a.wide_bc);
-    const float4 cm = load_states((const T*)a.Cm + b * a.Cb + (int64_t)g * a.N, 4 * ng, a.N, a.wide_bc);
+    const float4 bm = load_states<W4>((const T*)a.Bm + b * a.Bb + (int64_t)g * a.N, 4 * ng, a.N);
+    const float4 cm = load_states<W4>((const T*)a.Cm + b * a.Cb + (int64_t)g * a.N, 4 * ng, a.N);
     const float dt = softplus_f(raw), dtu = dt * uv;
     if (a.starts && a.starts[b]) h[0] = h[1] = h[2] = h[3] = 0.f;
     const float bv[4] = {bm.x, bm.y, bm.z, bm.w}, cv[4] = {cm.x, cm.y, cm.z, cm.w};
@@ -618,7 +650,6 @@ template <typename T, int S, bool W4> __global__ __launch_bounds__(NT) void scan
 // ---- host
 int lanes_of(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 int host_tile_f(int S) { return tile_f(S); }
-int host_tile_b(int S) { return tile_b(S); }
 
 bool scan_ok(const pnp_scan_desc* d) {
   return d && d->B >= 0 && d->L >= 0 && d->dim > 0 && d->dim <= (1 << 24) && d->N >= 1 && d->N <= 64 && d->groups >= 1 &&
@@ -642,7 +673,7 @@ Plan plan(const pnp_scan_desc* d) {
   }
   p.chunk = ceil_div(ceil_div(d->L ? d->L : 1, nch), tt) * tt;
   p.nch = (int)(d->L ? ceil_div(d->L, p.chunk) : 1);
-  p.nck = ceil_div(d->L, host_tile_b(p.S));
+  p.nck = ceil_div(d->L, TR);
   p.blocks = base * p.nch;
   return p;
 }
@@ -694,32 +725,36 @@ int32_t chain(const ScanArgs& a, const float* first, int S, int back, hipStream_
 
 template <typename T, int S> int32_t run_scan(ScanArgs a, int64_t blocks, hipStream_t st) {
   constexpr int E = tile_f(S) / S, V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
-  a.wide = a.per % V == 0 && a.dim % V == 0 && even(a.u, a.ub, a.ut, V, sizeof(T)) && even(a.delta, a.db, a.dt, V, sizeof(T)) &&
+  const bool wide = bc_even(a, sizeof(T)) && a.per % V == 0 && a.dim % V == 0 && even(a.u, a.ub, a.ut, V, sizeof(T)) && even(a.delta, a.db, a.dt, V, sizeof(T)) &&
            even(a.z, a.zb, a.zt, V, sizeof(T)) && even(a.out, 0, 0, V, sizeof(T));
-  a.wide_bc = bc_even(a, sizeof(T));
-  if (a.nch > 1) {
-    hipLaunchKernelGGL((scan_fwd_kernel<T, S, true>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
-    if (const int32_t rc = pnp_check_launch("scan_fwd_kernel (chunks)")) return rc;
-    if (const int32_t rc = chain(a, a.state, S, 0, st)) return rc;
-  }
-  hipLaunchKernelGGL((scan_fwd_kernel<T, S, false>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
-  return pnp_check_launch("scan_fwd_kernel");
+  auto go = [&](auto w) -> int32_t {
+    if (a.nch > 1) {
+      hipLaunchKernelGGL((scan_fwd_kernel<T, S, true, w>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+      if (const int32_t rc = pnp_check_launch("scan_fwd_kernel (chunks)")) return rc;
+      if (const int32_t rc = chain(a, a.state, S, 0, st)) return rc;
+    }
+    hipLaunchKernelGGL((scan_fwd_kernel<T, S, false, w>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    return pnp_check_launch("scan_fwd_kernel");
+  };
+  return wide ? go(std::true_type()) : go(std::false_type());
 }
 
 template <typename T, int S> int32_t run_scan_bwd(ScanBwdArgs a, int64_t blocks, hipStream_t st) {
   constexpr int E = tile_b(S) / S, V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
   ScanArgs& f = a.f;
-  f.wide = f.per % V == 0 && f.dim % V == 0 && even(f.u, f.ub, f.ut, V, sizeof(T)) && even(f.delta, f.db, f.dt, V, sizeof(T)) &&
+  const bool wide = bc_even(f, sizeof(T)) && f.per % V == 0 && f.dim % V == 0 && even(f.u, f.ub, f.ut, V, sizeof(T)) && even(f.delta, f.db, f.dt, V, sizeof(T)) &&
            even(f.z, f.zb, f.zt, V, sizeof(T)) && even(a.dout, a.ob, a.ot, V, sizeof(T)) && even(a.du, 0, 0, V, sizeof(T)) &&
            even(a.ddelta, 0, 0, V, sizeof(T)) && even(a.dz, 0, 0, V, sizeof(T));
-  f.wide_bc = bc_even(f, sizeof(T));
-  if (f.nch > 1) {
-    hipLaunchKernelGGL((scan_bwd_kernel<T, S, true>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
-    if (const int32_t rc = pnp_check_launch("scan_bwd_kernel (chunks)")) return rc;
-    if (const int32_t rc = chain(f, a.dlast, S, 1, st)) return rc;
-  }
-  hipLaunchKernelGGL((scan_bwd_kernel<T, S, false>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
-  if (const int32_t rc = pnp_check_launch("scan_bwd_kernel")) return rc;
+  auto go = [&](auto w) -> int32_t {
+    if (f.nch > 1) {
+      hipLaunchKernelGGL((scan_bwd_kernel<T, S, true, w>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+      if (const int32_t rc = pnp_check_launch("scan_bwd_kernel (chunks)")) return rc;
+      if (const int32_t rc = chain(f, a.dlast, S, 1, st)) return rc;
+    }
+    hipLaunchKernelGGL((scan_bwd_kernel<T, S, false, w>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    return pnp_check_launch("scan_bwd_kernel");
+  };
+  if (const int32_t rc = wide ? go(std::true_type()) : go(std::false_type())) return rc;
   const int64_t rows = f.B * f.L * f.groups, n = ceil_div(rows * 8 * S, NT);
   if (n) {
     hipLaunchKernelGGL((scan_bc_kernel<T>), dim3((unsigned)(n < (1 << 22) ? n : (1 << 22))), dim3(NT), 0, st, a.bc, rows, f.N, 4 * S, f.tiles,
@@ -732,8 +767,7 @@ template <typename T, int S> int32_t run_scan_bwd(ScanBwdArgs a, int64_t blocks,
 }
 
 template <typename T, int S> int32_t run_step(ScanArgs a, hipStream_t st) {
-  a.wide_bc = bc_even(a, sizeof(T));
-  const bool w4 = a.N == 4 * S && aligned_to(a.A, 16) && aligned_to(a.last, 16) && (!a.state || aligned_to(a.state, 16));
+  const bool w4 = a.N == 4 * S && bc_even(a, sizeof(T)) && aligned_to(a.A, 16) && aligned_to(a.last, 16) && (!a.state || aligned_to(a.state, 16));
   const int64_t n = ceil_div(a.B * a.dim * S, NT);
   const unsigned grid = (unsigned)(n < (1 << 22) ? n : (1 << 22));
   if (w4) hipLaunchKernelGGL((scan_step_kernel<T, S, true>), dim3(grid), dim3(NT), 0, st, a);
@@ -763,7 +797,18 @@ extern "C" int64_t pnp_scan_workspace(const pnp_scan_desc* d) {
   return split_floats(d, plan(d));
 }
 
+// a tile's offsets are 32-bit: 32 tokens of a stride, in bytes
+static bool strides_ok(const pnp_scan_desc* d) {
+  for (int64_t s : {d->u_tstride, d->delta_tstride, d->z_tstride, d->B_tstride, d->C_tstride, (int64_t)d->dim})
+    if (s < 0 || s > PNP_SCAN_MAX_TSTRIDE) return false;
+  return true;
+}
+
 static int32_t scan_check(const pnp_scan_desc* d, const Plan& p, const char* fn) {
+  if (!strides_ok(d)) {
+    pnp_set_error("%s: a token stride is out of range", fn);
+    return PNP_ERR_ARG;
+  }
   if (!d->A || (d->B && d->L && (!d->u || !d->delta || !d->Bm || !d->Cm))) {
     pnp_set_error("%s: null buffer", fn);
     return PNP_ERR_ARG;
@@ -827,6 +872,10 @@ extern "C" int32_t pnp_selective_scan_bwd(const pnp_scan_bwd_desc* d, void* stre
   if (const int32_t rc = scan_check(&f, p, fn)) return rc;
   if (!d->dA || (f.B && f.L && (!f.ckpt || !d->dout || !d->du || !d->ddelta || !d->dB || !d->dC || !f.z != !d->dz))) {
     pnp_set_error("%s: null buffer", fn);
+    return PNP_ERR_ARG;
+  }
+  if (d->dout_tstride < 0 || d->dout_tstride > PNP_SCAN_MAX_TSTRIDE) {
+    pnp_set_error("%s: a token stride is out of range", fn);
     return PNP_ERR_ARG;
   }
   const int64_t need = pnp_scan_bwd_workspace(d);

@@ -435,6 +435,11 @@ Tensor packed_groups(const Tensor& t) {
   return ok ? t : t.contiguous();
 }
 
+// the scan's offsets within a tile are 32-bit: a tensor with tokens further apart is copied
+Tensor near(const Tensor& t, int64_t lead) {
+  return t.defined() && lead == 2 && t.stride(1) > PNP_SCAN_MAX_TSTRIDE ? t.contiguous() : t;
+}
+
 // lead: dimensions before the channels
 ScanIn scan_in(const Tensor& u, const Tensor& delta, const Tensor& A, Tensor B, Tensor C, const MaybeTensor& D, const MaybeTensor& z,
                const MaybeTensor& bias, int64_t lead) {
@@ -462,8 +467,8 @@ ScanIn scan_in(const Tensor& u, const Tensor& delta, const Tensor& A, Tensor B, 
   want.push_back(A.size(1));
   TORCH_CHECK_VALUE(groups >= 1 && dim % groups == 0 && B.sizes() == want && C.sizes() == want, "B ", B.sizes(), " and C ", C.sizes(),
                     ": expected ", u.sizes().slice(0, lead), " and then [groups,] ", A.size(1), ", groups dividing ", dim);
-  return {lines(u), lines(delta), A32, packed_groups(B), packed_groups(C), parameter(D, "D", {dim}, u),
-          z && z->defined() ? lines(*z) : Tensor(), parameter(bias, "delta_bias", {dim}, u)};
+  return {near(lines(u), lead), near(lines(delta), lead), A32, near(packed_groups(B), lead), near(packed_groups(C), lead),
+          parameter(D, "D", {dim}, u), z && z->defined() ? near(lines(*z), lead) : Tensor(), parameter(bias, "delta_bias", {dim}, u)};
 }
 
 pnp_scan_desc scan_desc(const ScanIn& v, const Tensor& starts, const Tensor& state, bool step) {
@@ -518,7 +523,7 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
     const ScanIn v{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]};
     const Tensor &starts = s[8], &state = s[9], &ckpt = s[10], &u = v.u;
     const ScalarType t = u.scalar_type();
-    const Tensor dout = grads[0].defined() ? lines(grads[0]) : at::zeros(u.sizes(), u.options());
+    const Tensor dout = grads[0].defined() ? near(lines(grads[0]), 2) : at::zeros(u.sizes(), u.options());
     const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
     pnp_scan_bwd_desc d{};
     d.f = scan_desc(v, starts, state, false);
