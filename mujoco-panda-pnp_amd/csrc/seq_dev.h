@@ -42,20 +42,17 @@ __device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f
 #define SEQ_LOG2E 1.44269504088896340736f
 __device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.f + exp2_f(-SEQ_LOG2E * x)); }
 
-// softplus(x) = max(x, 0) + log(1 + e) with e = exp(-|x|) in (0, 1]: no overflow.  The logarithm by its
-// series log(1 + e) = 2 (s + s^3 / 3 + s^5 / 5 + ...), s = e / (2 + e) <= 1 / 3: relative accuracy for small
-// results too (log of the rounded 1 + e would lose it: at x = -10 to 1e-3).  Seven terms past the first
-// leave (1/9)^8 / 17 = 1.4e-9.  A third of the library function's instructions.
+// softplus(x) = max(x, 0) + log(1 + e) with e = exp(-|x|) in (0, 1]: no overflow.  The logarithm as
+// log(1 + e) = 2 atanh(s), s = e / (2 + e) <= 1 / 3: relative accuracy for small results too (log of the
+// rounded 1 + e would lose it: at x = -10 to 1e-3).  atanh(s) / s is a polynomial in s^2, fitted to the
+// least largest relative error on [0, 1/9] (4e-9); in all within 5 steps of 2^-24 of the function.
 __device__ __forceinline__ float softplus_f(float x) {
   const float e = exp2_f(-SEQ_LOG2E * fabsf(x));
   const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
-  float p = 1.f / 15;
-  p = p * q + 1.f / 13;
-  p = p * q + 1.f / 11;
-  p = p * q + 1.f / 9;
-  p = p * q + 1.f / 7;
-  p = p * q + 1.f / 5;
-  p = p * q + 1.f / 3;
+  float p = 0.1408916711807251f;
+  p = p * q + 0.13980300724506378f;
+  p = p * q + 0.20012454688549042f;
+  p = p * q + 0.3333315849304199f;
   p = p * q + 1.f;
   return fmaxf(x, 0.f) + 2.f * s * p;   // (NaN: through e)
 }

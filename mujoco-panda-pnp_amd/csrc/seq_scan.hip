@@ -32,9 +32,13 @@ constexpr int NT = 256;
 
 // tokens of a tile, forward and gradient; the gradient's inner tile, whose states and decays stay in
 // registers (8 a token), is TR tokens: the forward keeps a state for each
-constexpr int tile_f(int S) { return S == 1 ? 8 : S == 2 ? 16 : 32; }
+constexpr int tile_f(int S, int bytes) {   // 4 or 8 channels a thread: registers for 4 waves a SIMD
+  return S == 1 ? 8 : S == 2 ? (bytes == 4 ? 8 : 16) : S == 4 ? (bytes == 4 ? 16 : 32) : 32;
+}
 constexpr int tile_b(int S) { return S == 1 ? 8 : 16; }
 constexpr int TR = 8;
+// waves a SIMD that the forward is built for: what its registers allow without spills
+constexpr int fwd_waves(int S, int bytes) { return S >= 8 || (S == 1 && bytes == 4) ? 3 : 4; }
 
 struct ScanArgs {
   int64_t B, L;
@@ -54,16 +58,15 @@ struct ScanArgs {
 };
 
 struct Where { int64_t b, row; int chunk, g, c0, ch; };   // c0: first channel within the group; row: b * nch + chunk
-template <int S> __device__ __forceinline__ Where where(const ScanArgs& a) {
-  const int per_row = a.groups * a.tiles;
-  const int64_t row = blockIdx.x / per_row;
-  const int r = (int)(blockIdx.x - row * per_row);
+// the workgroup's place among the sequences' chunks [first, first + chunks)
+template <int S> __device__ __forceinline__ Where where(const ScanArgs& a, int first, int chunks) {
+  const uint32_t per_row = a.groups * a.tiles, row = blockIdx.x / per_row, r = blockIdx.x - row * per_row;
   Where w;
-  w.row = row;
-  w.b = row / a.nch;
-  w.chunk = (int)(row - w.b * a.nch);
-  w.g = r / a.tiles;
-  w.c0 = (r - w.g * a.tiles) * (NT / S);
+  w.b = row / (uint32_t)chunks;
+  w.chunk = (int)(row - (uint32_t)w.b * chunks) + first;
+  w.row = w.b * a.nch + w.chunk;
+  w.g = (int)r / a.tiles;
+  w.c0 = ((int)r - w.g * a.tiles) * (NT / S);
   w.ch = w.g * a.per + w.c0;
   return w;
 }
@@ -146,29 +149,52 @@ __device__ __forceinline__ void load_bc(const ScanArgs& a, int64_t b, int g, int
   }
 }
 
-// the tile's tokens that start a sequence, a bit each (TT <= 32), the same in every wave
-template <int TT> __device__ __forceinline__ uint32_t start_bits(const ScanArgs& a, int64_t b, int64_t t0, int64_t t1) {
-  if (!a.starts) return 0;
+// the lane's byte of a tile's starts, and of all lanes' bytes the tile's tokens that start a sequence, a bit
+// each (TT <= 32), the same in every wave
+template <int TT> __device__ __forceinline__ uint32_t load_start(const ScanArgs& a, int64_t b, int64_t t, int64_t t1) {
   const int l = threadIdx.x & 63;
-  const bool s = l < TT && t0 + l < t1 && a.starts[b * a.L + t0 + l] != 0;
-  return (uint32_t)__builtin_amdgcn_ballot_w64(s);
+  return a.starts && l < TT && t + l < t1 ? *at<uint8_t>(a.starts, b * a.L + t, (uint32_t)l) : 0;
+}
+__device__ __forceinline__ uint32_t start_bits(uint32_t byte) { return (uint32_t)__builtin_amdgcn_ballot_w64(byte != 0); }
+
+// Where a thread's j-th unit (16 bytes) of a row of LDS goes, r: the thread's place in the row, U: units a
+// thread.  The threads' rows of units are 16 U bytes apart; the exchange of units within a thread's own
+// every 256 bytes lets 8 neighbouring threads' writes of one j fall into different banks.
+template <int U> __device__ __forceinline__ int unit(int r, int j) { return r * U + (j ^ (r * U >> 4 & (U - 1))); }
+
+// Sums over the S lanes of a channel of G tokens' values, token i's left in the lanes ng with ng % G = i:
+// G tokens leave by one store of all lanes (G = S up to the inner tile).  Of two tokens' values a lane
+// keeps one and gives the other away.
+constexpr int group_of(int S) { return S < TR ? S : TR; }
+__device__ __forceinline__ float xor4(float v) { return dpp<0x1B>(dpp<SEQ_DPP_HALF_MIRROR>(v)); }   // xor 7, then xor 3
+template <int S> __device__ __forceinline__ float token_sums(float (&q)[group_of(S)]) {
+  const int l = threadIdx.x;
+  constexpr int G = group_of(S);
+  if (S == 16)
+#pragma unroll
+    for (int i = 0; i < G; i++) q[i] += dpp<SEQ_DPP_ROR8>(q[i]);
+#pragma unroll
+  for (int i = 0; 2 * i < G; i++)
+    if (G > 1) q[i] = ((l & 1) ? q[2 * i + (G > 1)] : q[2 * i]) + dpp<SEQ_DPP_XOR1>((l & 1) ? q[2 * i] : q[2 * i + (G > 1)]);
+#pragma unroll
+  for (int i = 0; 4 * i < G; i++)
+    if (G > 2) q[i] = ((l & 2) ? q[2 * i + (G > 2)] : q[2 * i]) + dpp<SEQ_DPP_XOR2>((l & 2) ? q[2 * i] : q[2 * i + (G > 2)]);
+  if (G > 4) q[0] = ((l & 4) ? q[G > 4] : q[0]) + xor4((l & 4) ? q[0] : q[G > 4]);
+  return q[0];
 }
 
-// Of G tokens' values, each the same in the S lanes of a channel, a lane keeps the one of token `ng`: G tokens
-// leave by one store of all lanes (G = S up to the inner tile).
-constexpr int group_of(int S) { return S < TR ? S : TR; }
-
 // STATE: the chunk's state from a zero start and its decay alone
-template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__(NT) void scan_fwd_kernel(ScanArgs a) {
-  constexpr int TT = tile_f(S), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S, G = group_of(S);
-  __shared__ float2 dd[TT][CW];
+template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__(NT, fwd_waves(S, sizeof(T))) void scan_fwd_kernel(ScanArgs a) {
+  constexpr int TT = tile_f(S, sizeof(T)), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S, G = group_of(S), U = E / 2;
+  __shared__ float4 dd[TT][CW / 2];                                 // dt, dt u of two channels; then y in dt's place
   __shared__ float4 sB[TT][S], sC[STATE ? 1 : TT][S];
-  const Where w = where<S>(a);
+  const Where w = where<S>(a, 0, STATE ? a.nch - 1 : a.nch);
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int cl = wave * (64 / S) + lane / S, ng = lane % S;         // the lane's channel and states
   const int lt = tid / RT, lc = (tid % RT) * E;                     // the thread's part of a tile
   const int left = a.per - w.c0 - lc;                               // channels from there to the group's end
   const bool on = w.c0 + cl < a.per;
+  const int mine2 = 2 * unit<U>(cl / E, cl % E / 2) + cl % 2;       // the lane's channel in a row of dd, as float2
   const int64_t t0 = (int64_t)w.chunk * a.chunk, t1 = t0 + a.chunk < a.L ? t0 + a.chunk : a.L;
   const bool z = !STATE && a.z;
   const uint32_t ou = (uint32_t)(lt * a.ut + lc) * sizeof(T), od = (uint32_t)(lt * a.dt + lc) * sizeof(T),
@@ -193,8 +219,10 @@ template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__
   constexpr int NBC = STATE ? TT * S : 2 * TT * S;                  // packs of 4 states a tile
   constexpr int PER = (NBC + NT - 1) / NT;
   float4 nbc[PER];
+  uint32_t ns = 0;
   auto fetch = [&](int64_t t) {
     const int l = t + lt < t1 ? left : 0;
+    ns = load_start<TT>(a, w.b, t, t1);
     load_channels<E, WIDE>(at<T>(a.u, w.b * a.ub + t * a.ut + w.ch, ou), l, nu);
     load_channels<E, WIDE>(at<T>(a.delta, w.b * a.db + t * a.dt + w.ch, od), l, nd);
     if (z) load_channels<E, WIDE>(at<T>(a.z, w.b * a.zb + t * a.zt + w.ch, oz), l, nz);
@@ -204,9 +232,11 @@ template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__
   for (int64_t t = t0; t < t1; t += TT) {
     const bool mine = t + lt < t1;
 #pragma unroll
-    for (int i = 0; i < E; i++) {
-      const float uv = to_f(nu.v[i]), d = mine && i < left ? softplus_f(to_f(nd.v[i]) + bias[i]) : 0.f;
-      dd[lt][lc + i] = float2{d, d * uv};
+    for (int j = 0; j < U; j++) {
+      float d[2];
+#pragma unroll
+      for (int k = 0; k < 2; k++) d[k] = mine && 2 * j + k < left ? softplus_f(to_f(nd.v[2 * j + k]) + bias[2 * j + k]) : 0.f;
+      dd[lt][unit<U>(tid % RT, j)] = float4{d[0], d[0] * to_f(nu.v[2 * j]), d[1], d[1] * to_f(nu.v[2 * j + 1])};
     }
     cu = nu;
     cz = nz;
@@ -216,14 +246,14 @@ template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__
       if (i < TT * S) (&sB[0][0])[i] = nbc[k];
       else if (!STATE && i < 2 * TT * S) (&sC[0][0])[i - TT * S] = nbc[k];
     }
-    const uint32_t bits = start_bits<TT>(a, w.b, t, t1);
+    const uint32_t bits = start_bits(ns);
     __syncthreads();
     if (t + TT < t1) fetch(t + TT);
     auto tokens = [&](auto starts, int p) {
-      float keep = 0.f;
+      float q[G];
 #pragma unroll
       for (int k = 0; k < TR; k++) {
-        const float2 d = dd[p + k][cl];
+        const float2 d = reinterpret_cast<const float2*>(dd[p + k])[mine2];
         const float4 b = sB[p + k][ng];
         if (starts.value && (bits >> (p + k) & 1)) {
           h[0] = h[1] = h[2] = h[3] = 0.f;
@@ -237,10 +267,11 @@ template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__
           dsum += d.x;
         } else {
           const float4 c = sC[p + k][ng];
-          const float y = group_sum<S>(c.x * h[0] + c.y * h[1] + c.z * h[2] + c.w * h[3]);
-          keep = ng == k % G ? y : keep;
-          // (dt of these tokens has been read by every lane of the channel)
-          if (k % G == G - 1 && (G == S || ng < G)) dd[p + k - (G - 1) + ng][cl].x = keep;
+          q[k % G] = c.x * h[0] + c.y * h[1] + c.z * h[2] + c.w * h[3];
+          if (k % G == G - 1) {   // (dt of these tokens has been read by every lane of the channel)
+            const float y = token_sums<S>(q);
+            if (G == S || ng < G) reinterpret_cast<float2*>(dd[p + k - (G - 1) + ng])[mine2].x = y;
+          }
         }
       }
     };
@@ -255,8 +286,14 @@ template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__
     if (!STATE && mine) {
       float o[E];
 #pragma unroll
+      for (int j = 0; j < U; j++) {
+        const float4 y = dd[lt][unit<U>(tid % RT, j)];
+        o[2 * j] = y.x;
+        o[2 * j + 1] = y.z;
+      }
+#pragma unroll
       for (int i = 0; i < E; i++) {
-        o[i] = dd[lt][lc + i].x + Dv[i] * to_f(cu.v[i]);
+        o[i] += Dv[i] * to_f(cu.v[i]);
         const float zv = to_f(cz.v[i]);
         if (z) o[i] *= zv * sigmoid_f(zv);
       }
@@ -287,6 +324,10 @@ __global__ __launch_bounds__(NT) void scan_chain_kernel(ScanArgs a, const float*
   for (int i = 0; i < a.nch; i++) {
     const int64_t row = b * a.nch + (back ? a.nch - 1 - i : i);
     float* p = a.hin + (row * a.dim + d) * NP + n;
+    if (i == a.nch - 1) {   // (nothing follows it: its own state was not asked for)
+      *p = h;
+      return;
+    }
     const float own = *p, s = a.dsum[row * a.dim + d];
     *p = h;
     // a start in the chunk lets nothing through
@@ -327,40 +368,130 @@ template <int S> __device__ __forceinline__ void channel_sums(float (&v)[8]) {
     const float give = up ? v[0] : v[1], keep = up ? v[1] : v[0];
     v[0] = keep + dpp<SEQ_DPP_ROR8>(give);
   }
-  if (S < 8) v[0] += dpp<0x1B>(dpp<SEQ_DPP_HALF_MIRROR>(v[0]));   // xor 7, then quad_perm [3, 2, 1, 0]: xor 4
+  if (S < 8) v[0] += xor4(v[0]);
   if (S < 4) v[0] += dpp<SEQ_DPP_XOR2>(v[0]);
   if (S < 2) v[0] += dpp<SEQ_DPP_XOR1>(v[0]);
 }
 
-// STATE: the chunk's adjoint from a zero end and its decay alone
-template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__(NT, 2) void scan_bwd_kernel(ScanBwdArgs a) {
-  constexpr int TT = tile_b(S), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S, G = group_of(S);
+// a chunk's adjoint from a zero end, and its decay
+template <typename T, int S, bool WIDE> __global__ __launch_bounds__(NT) void scan_adjoint_kernel(ScanBwdArgs a) {
+  constexpr int TT = tile_f(S, sizeof(T)), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S, U = E / 2;
   const ScanArgs& f = a.f;
-  __shared__ float4 dd[TT][CW];                        // dt, dy, u, dt u; then dt, dy, sum g B, sum g (a h') A
-  __shared__ float yb[STATE ? 1 : TT][CW];             // sum C h
-  __shared__ float4 sB[TT][S], sC[TT][S];
-  __shared__ float bc[STATE ? 1 : 4][STATE ? 1 : TT][2 * NP];
-  const Where w = where<S>(f);
+  __shared__ float4 dd[TT][CW / 2];                    // dt, dy of two channels
+  __shared__ float4 sC[TT][S];
+  const Where w = where<S>(f, 1, f.nch - 1);
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int cl = wave * (64 / S) + lane / S, ng = lane % S;
   const int lt = tid / RT, lc = (tid % RT) * E;
   const int left = f.per - w.c0 - lc;
   const bool on = w.c0 + cl < f.per;
+  const int mine2 = 2 * unit<U>(cl / E, cl % E / 2) + cl % 2;
+  const int64_t t0 = (int64_t)w.chunk * f.chunk, t1 = t0 + f.chunk < f.L ? t0 + f.chunk : f.L;
+  const bool z = f.z;
+  const uint32_t od = (uint32_t)(lt * f.dt + lc) * sizeof(T), oz = (uint32_t)(lt * f.zt + lc) * sizeof(T),
+                 oy = (uint32_t)(lt * a.ot + lc) * sizeof(T);
+  float A2[4], g[4] = {0.f, 0.f, 0.f, 0.f}, dsum = 0.f;
+  const int64_t ch = w.ch + (on ? cl : 0);
+  load_state4(f.A + ch * f.N, 4 * ng, f.N, A2);
+#pragma unroll
+  for (int i = 0; i < 4; i++) A2[i] *= SEQ_LOG2E;
+  float bias[E];
+#pragma unroll
+  for (int i = 0; i < E; i++) bias[i] = f.bias && i < left ? f.bias[w.ch + lc + i] : 0.f;
+  constexpr int NBC = TT * S, PER = (NBC + NT - 1) / NT;
+  Raw<T, E> nd, nz, no;
+  float4 nc[PER];
+  uint32_t ns = 0;
+  ScanArgs fc = f;   // C in B's place: all of it that load_bc reads
+  fc.Bm = f.Cm;
+  fc.Bb = f.Cb;
+  fc.Bt = f.Ct;
+  auto fetch = [&](int64_t t) {
+    const int l = t + lt < t1 ? left : 0;
+    ns = load_start<TT>(f, w.b, t, t1);
+    load_channels<E, WIDE>(at<T>(f.delta, w.b * f.db + t * f.dt + w.ch, od), l, nd);
+    if (z) load_channels<E, WIDE>(at<T>(f.z, w.b * f.zb + t * f.zt + w.ch, oz), l, nz);
+    load_channels<E, WIDE>(at<T>(a.dout, w.b * a.ob + t * a.ot + w.ch, oy), l, no);
+    load_bc<T, S, TT, NBC, WIDE>(fc, w.b, w.g, t, t1, nc);
+  };
+  const int64_t tiles = (t1 - t0 + TT - 1) / TT;
+  if (tiles > 0) fetch(t0 + (tiles - 1) * TT);
+  for (int64_t t = t0 + (tiles - 1) * TT; t >= t0; t -= TT) {
+    const bool mine = t + lt < t1;
+#pragma unroll
+    for (int j = 0; j < U; j++) {
+      float d[4];
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const int i = 2 * j + k;
+        const bool in = mine && i < left;
+        const float zv = to_f(nz.v[i]), ov = to_f(no.v[i]);
+        d[2 * k] = in ? softplus_f(to_f(nd.v[i]) + bias[i]) : 0.f;
+        d[2 * k + 1] = !in ? 0.f : z ? ov * zv * sigmoid_f(zv) : ov;
+      }
+      dd[lt][unit<U>(tid % RT, j)] = float4{d[0], d[1], d[2], d[3]};
+    }
+#pragma unroll
+    for (int k = 0; k < PER; k++)
+      if (k * NT + tid < NBC) (&sC[0][0])[k * NT + tid] = nc[k];
+    const uint32_t bits = start_bits(ns);
+    __syncthreads();
+    if (t > t0) fetch(t - TT);
+    auto tokens = [&](auto starts, int p) {
+#pragma unroll
+      for (int k = TR - 1; k >= 0; k--) {
+        const float2 d = reinterpret_cast<const float2*>(dd[p + k])[mine2];
+        const float4 c = sC[p + k][ng];
+        g[0] = exp2_f(d.x * A2[0]) * (g[0] + c.x * d.y);
+        g[1] = exp2_f(d.x * A2[1]) * (g[1] + c.y * d.y);
+        g[2] = exp2_f(d.x * A2[2]) * (g[2] + c.z * d.y);
+        g[3] = exp2_f(d.x * A2[3]) * (g[3] + c.w * d.y);
+        dsum += d.x;
+        if (starts.value && (bits >> (p + k) & 1)) {
+          g[0] = g[1] = g[2] = g[3] = 0.f;
+          dsum = __builtin_nanf("");
+        }
+      }
+    };
+#pragma unroll 1
+    for (int p = TT - TR; p >= 0; p -= TR) {
+      if (bits) tokens(std::true_type(), p);
+      else tokens(std::false_type(), p);
+    }
+    __syncthreads();
+  }
+  if (!on) return;
+  *reinterpret_cast<float4*>(f.hin + (w.row * f.dim + ch) * NP + 4 * ng) = float4{g[0], g[1], g[2], g[3]};
+  if (ng == 0) f.dsum[w.row * f.dim + ch] = dsum;
+}
+
+template <typename T, int S, bool WIDE> __global__ __launch_bounds__(NT, 2) void scan_bwd_kernel(ScanBwdArgs a) {
+  constexpr int TT = tile_b(S), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S, G = group_of(S);
+  const ScanArgs& f = a.f;
+  __shared__ float4 dd[TT][CW];                        // dt, dy, u, dt u; then dt, dy, sum g B, sum g (a h') A
+  __shared__ float yb[TT][CW];                         // sum C h
+  __shared__ float4 sB[TT][S], sC[TT][S];
+  __shared__ float bc[4][TT][2 * NP];
+  const Where w = where<S>(f, 0, f.nch);
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int cl = wave * (64 / S) + lane / S, ng = lane % S;
+  const int lt = tid / RT, lc = (tid % RT) * E;
+  const int left = f.per - w.c0 - lc;
+  const bool on = w.c0 + cl < f.per;
+  const int mine4 = unit<E>(cl / E, cl % E);           // the lane's channel in a row of dd
   const int64_t t0 = (int64_t)w.chunk * f.chunk, t1 = t0 + f.chunk < f.L ? t0 + f.chunk : f.L;
   const bool z = f.z;
   const uint32_t ou = (uint32_t)(lt * f.ut + lc) * sizeof(T), od = (uint32_t)(lt * f.dt + lc) * sizeof(T),
                  oz = (uint32_t)(lt * f.zt + lc) * sizeof(T), oy = (uint32_t)(lt * a.ot + lc) * sizeof(T),
                  oo = (uint32_t)(lt * f.dim + lc) * sizeof(T), ok = (uint32_t)(cl * NP + 4 * ng) * 4u;
 
-  float A[4], A2[4], dA[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {0.f, 0.f, 0.f, 0.f}, dsum = 0.f;
+  float A[4], A2[4], dA[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {0.f, 0.f, 0.f, 0.f};
   const int64_t ch = w.ch + (on ? cl : 0);
   load_state4(f.A + ch * f.N, 4 * ng, f.N, A);
 #pragma unroll
   for (int i = 0; i < 4; i++) A2[i] = A[i] * SEQ_LOG2E;
-  if (!STATE) {
-    if (f.nch > 1) load_state4(f.hin + (w.row * f.dim + ch) * NP, 4 * ng, NP, g);
-    else if (a.dlast) load_state4(a.dlast + (w.b * f.dim + ch) * f.N, 4 * ng, f.N, g);
-  }
+  if (f.nch > 1) load_state4(f.hin + (w.row * f.dim + ch) * NP, 4 * ng, NP, g);
+  else if (a.dlast) load_state4(a.dlast + (w.b * f.dim + ch) * f.N, 4 * ng, f.N, g);
   float Dv[E], bias[E], dD[E] = {}, dbias[E] = {};
 #pragma unroll
   for (int i = 0; i < E; i++) {
@@ -370,8 +501,10 @@ template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__
   constexpr int NBC = 2 * TT * S, PER = (NBC + NT - 1) / NT;
   Raw<T, E> nu, nd, nz, no, cu, cd, cz, co;
   float4 nbc[PER];
+  uint32_t ns = 0;
   auto fetch = [&](int64_t t) {
     const int l = t + lt < t1 ? left : 0;
+    ns = load_start<TT>(f, w.b, t, t1);
     load_channels<E, WIDE>(at<T>(f.u, w.b * f.ub + t * f.ut + w.ch, ou), l, nu);
     load_channels<E, WIDE>(at<T>(f.delta, w.b * f.db + t * f.dt + w.ch, od), l, nd);
     if (z) load_channels<E, WIDE>(at<T>(f.z, w.b * f.zb + t * f.zt + w.ch, oz), l, nz);
@@ -388,147 +521,125 @@ template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__
       const float uv = to_f(nu.v[i]), zv = to_f(nz.v[i]), ov = to_f(no.v[i]);
       const float d = in ? softplus_f(to_f(nd.v[i]) + bias[i]) : 0.f;
       const float dy = !in ? 0.f : z ? ov * zv * sigmoid_f(zv) : ov;
-      dd[lt][lc + i] = float4{d, dy, uv, d * uv};
+      dd[lt][unit<E>(tid % RT, i)] = float4{d, dy, uv, d * uv};
     }
     cu = nu;
     cd = nd;
     cz = nz;
     co = no;
     float4 hc[TT / TR];
-    if (!STATE)
 #pragma unroll
-      for (int p = 0; p < TT / TR; p++) {
-        hc[p] = float4{0.f, 0.f, 0.f, 0.f};
-        if (on && t + p * TR < t1) hc[p] = *reinterpret_cast<const float4*>(at<float>(f.ckpt, ((w.b * f.nck + t / TR + p) * f.dim + w.ch) * NP, ok));
-      }
+    for (int p = 0; p < TT / TR; p++) {
+      hc[p] = float4{0.f, 0.f, 0.f, 0.f};
+      if (on && t + p * TR < t1) hc[p] = *reinterpret_cast<const float4*>(at<float>(f.ckpt, ((w.b * f.nck + t / TR + p) * f.dim + w.ch) * NP, ok));
+    }
 #pragma unroll
     for (int k = 0; k < PER; k++) {
       const int i = k * NT + tid;
       if (i < TT * S) (&sB[0][0])[i] = nbc[k];
       else if (i < 2 * TT * S) (&sC[0][0])[i - TT * S] = nbc[k];
     }
-    const uint32_t bits = start_bits<TT>(f, w.b, t, t1);
+    const uint32_t bits = start_bits(ns);
     __syncthreads();
     if (t > t0) fetch(t - TT);
-    if constexpr (STATE) {
-#pragma unroll 4
-      for (int k = TT - 1; k >= 0; k--) {
-        const float4 d = dd[k][cl];
-        const float4 c = sC[k][ng];
-        g[0] = exp2_f(d.x * A2[0]) * (g[0] + c.x * d.y);
-        g[1] = exp2_f(d.x * A2[1]) * (g[1] + c.y * d.y);
-        g[2] = exp2_f(d.x * A2[2]) * (g[2] + c.z * d.y);
-        g[3] = exp2_f(d.x * A2[3]) * (g[3] + c.w * d.y);
-        dsum += d.x;
-        if (bits >> k & 1) {
-          g[0] = g[1] = g[2] = g[3] = 0.f;
-          dsum = __builtin_nanf("");
+    // the inner tile at p from the state h0: its states and decays forward, kept, then the adjoint back.
+    // starts: a start's decay is 0 whatever the state (0 times infinity is NaN)
+    auto tokens = [&](auto starts, int p, const float4 h0) {
+      constexpr bool ST = decltype(starts)::value;
+      const uint32_t marks = bits >> p;
+      float e[TR][4], h[TR + 1][4], q[G];
+      h[0][0] = h0.x; h[0][1] = h0.y; h[0][2] = h0.z; h[0][3] = h0.w;
+#pragma unroll
+      for (int k = 0; k < TR; k++) {
+        const float4 d = dd[p + k][mine4];
+        const float4 b = sB[p + k][ng], c = sC[p + k][ng];
+        const float bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
+        const bool st = ST && (marks >> k & 1);
+        float y = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          e[k][i] = exp2_f(d.x * A2[i]);
+          const float ah = e[k][i] * h[k][i];
+          h[k + 1][i] = (st ? 0.f : ah) + d.w * bv[i];
+          y += cv[i] * h[k + 1][i];
+        }
+        q[k % G] = y;
+        if (k % G == G - 1) {
+          y = token_sums<S>(q);
+          if (G == S || ng < G) yb[p + k - (G - 1) + ng][cl] = y;
         }
       }
-      __syncthreads();
-    } else {
-      // the inner tile at p from the state h0: its states and decays forward, kept, then the adjoint back.
-      // starts: a start's decay is 0 whatever the state (0 times infinity is NaN)
-      auto tokens = [&](auto starts, int p, const float4 h0) {
-        constexpr bool ST = decltype(starts)::value;
-        const uint32_t marks = bits >> p;
-        float e[TR][4], h[TR + 1][4], keep = 0.f;
-        h[0][0] = h0.x; h[0][1] = h0.y; h[0][2] = h0.z; h[0][3] = h0.w;
+      // the tile is read again rather than held, 12 registers a token (the compiler must not see that it is the same)
+      asm volatile("" : "+s"(p));
+      float q1[G], q2[G];
 #pragma unroll
-        for (int k = 0; k < TR; k++) {
-          const float4 d = dd[p + k][cl];
-          const float4 b = sB[p + k][ng], c = sC[p + k][ng];
-          const float bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
-          const bool st = ST && (marks >> k & 1);
-          float y = 0.f;
+      for (int k = TR - 1; k >= 0; k--) {
+        const float4 d = dd[p + k][mine4];
+        const float4 b = sB[p + k][ng], c = sC[p + k][ng];
+        const float bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
+        const bool st = ST && (marks >> k & 1);
+        float s1 = 0.f, s2 = 0.f, v[8];
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            e[k][i] = exp2_f(d.x * A2[i]);
-            const float ah = e[k][i] * h[k][i];
-            h[k + 1][i] = (st ? 0.f : ah) + d.w * bv[i];
-            y += cv[i] * h[k + 1][i];
-          }
-          y = group_sum<S>(y);
-          keep = ng == k % G ? y : keep;
-          if (k % G == G - 1 && (G == S || ng < G)) yb[p + k - (G - 1) + ng][cl] = keep;
+        for (int i = 0; i < 4; i++) {
+          g[i] += cv[i] * d.y;
+          v[4 + i] = h[k + 1][i] * d.y;
+          v[i] = g[i] * d.w;
+          s1 += g[i] * bv[i];
+          float ek = e[k][i];
+          asm("" : "+v"(ek));   // (e h is multiplied again: kept from above it would take 4 registers a token)
+          const float ah = ek * h[k][i], gah = g[i] * (st ? 0.f : ah);
+          s2 += gah * A[i];
+          dA[i] += gah * d.x;
+          g[i] = st ? 0.f : g[i] * ek;
         }
-        // the tile is read again rather than held, 12 registers a token (the compiler must not see that it is the same)
-        asm volatile("" : "+s"(p));
-        float k1 = 0.f, k2 = 0.f;
-#pragma unroll
-        for (int k = TR - 1; k >= 0; k--) {
-          const float4 d = dd[p + k][cl];
-          const float4 b = sB[p + k][ng], c = sC[p + k][ng];
-          const float bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
-          const bool st = ST && (marks >> k & 1);
-          float s1 = 0.f, s2 = 0.f, v[8];
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            g[i] += cv[i] * d.y;
-            v[4 + i] = h[k + 1][i] * d.y;
-            v[i] = g[i] * d.w;
-            s1 += g[i] * bv[i];
-            float ek = e[k][i];
-            asm("" : "+v"(ek));   // (e h is multiplied again: kept from above it would take 4 registers a token)
-            const float ah = ek * h[k][i], gah = g[i] * (st ? 0.f : ah);
-            s2 += gah * A[i];
-            dA[i] += gah * d.x;
-            g[i] = st ? 0.f : g[i] * ek;
-          }
-          s1 = group_sum<S>(s1);
-          s2 = group_sum<S>(s2);
-          k1 = ng == k % G ? s1 : k1;
-          k2 = ng == k % G ? s2 : k2;
-          if (k % G == 0 && (G == S || ng < G)) *reinterpret_cast<float2*>(&dd[p + k + ng][cl].z) = float2{k1, k2};
-          channel_sums<S>(v);
-          if (S >= 8 || (lane & 7) < S) {
-            const int o = (lane >> 5) * NP + 4 * ng + 2 * (lane >> 4 & 1);
-            if (S < 16) bc[wave][p + k][o + (lane >> 3 & 1)] = v[0];
-            else {
-              bc[wave][p + k][o] = v[0];
-              bc[wave][p + k][o + 1] = v[1];
-            }
+        q1[k % G] = s1;
+        q2[k % G] = s2;
+        if (k % G == 0) {
+          const float2 s = {token_sums<S>(q1), token_sums<S>(q2)};
+          if (G == S || ng < G) *reinterpret_cast<float2*>(&dd[p + k + ng][mine4].z) = s;
+        }
+        channel_sums<S>(v);
+        if (S >= 8 || (lane & 7) < S) {
+          const int o = (lane >> 5) * NP + 4 * ng + 2 * (lane >> 4 & 1);
+          if (S < 16) bc[wave][p + k][o + (lane >> 3 & 1)] = v[0];
+          else {
+            bc[wave][p + k][o] = v[0];
+            bc[wave][p + k][o + 1] = v[1];
           }
         }
-      };
+      }
+    };
 #pragma unroll
-      for (int q = TT / TR - 1; q >= 0; q--) {
-        if (bits) tokens(std::true_type(), q * TR, hc[q]);
-        else tokens(std::false_type(), q * TR, hc[q]);
-      }
-      __syncthreads();
-      if (mine) {
-        float du[E], dr[E], dz[E];
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-          const float4 s = dd[lt][lc + i];
-          const float dt = s.x, dy = s.y, uv = to_f(cu.v[i]);
-          du[i] = Dv[i] * dy + dt * s.z;
-          dr[i] = i < left ? (s.w + uv * s.z) * sigmoid_f(to_f(cd.v[i]) + bias[i]) : 0.f;
-          dD[i] += dy * uv;
-          dbias[i] += dr[i];
-          const float zv = to_f(cz.v[i]), sg = sigmoid_f(zv);
-          dz[i] = to_f(co.v[i]) * (yb[lt][lc + i] + Dv[i] * uv) * (sg * (1.f + zv * (1.f - sg)));
-        }
-        const int64_t o = (w.b * f.L + t) * f.dim + w.ch;
-        store_channels<E, WIDE>(at<T>(a.du, o, oo), left, du);
-        store_channels<E, WIDE>(at<T>(a.ddelta, o, oo), left, dr);
-        if (z) store_channels<E, WIDE>(at<T>(a.dz, o, oo), left, dz);
-      }
-      // this workgroup's share of dB and dC
-      const int64_t tile = w.c0 / CW;
-      for (int i = tid; i < TT * 2 * NP; i += NT) {
-        const int k = i / (2 * NP), j = i - k * 2 * NP;
-        if (t + k < t1)
-          a.bc[(((tile * f.B + w.b) * f.L + t + k) * f.groups + w.g) * (2 * NP) + j] = bc[0][k][j] + bc[1][k][j] + bc[2][k][j] + bc[3][k][j];
-      }
+    for (int i = TT / TR - 1; i >= 0; i--) {
+      if (bits) tokens(std::true_type(), i * TR, hc[i]);
+      else tokens(std::false_type(), i * TR, hc[i]);
     }
-  }
-  if (STATE) {
-    if (!on) return;
-    *reinterpret_cast<float4*>(f.hin + (w.row * f.dim + ch) * NP + 4 * ng) = float4{g[0], g[1], g[2], g[3]};
-    if (ng == 0) f.dsum[w.row * f.dim + ch] = dsum;
-    return;
+    __syncthreads();
+    if (mine) {
+      float du[E], dr[E], dz[E];
+#pragma unroll
+      for (int i = 0; i < E; i++) {
+        const float4 s = dd[lt][unit<E>(tid % RT, i)];
+        const float dt = s.x, dy = s.y, uv = to_f(cu.v[i]);
+        du[i] = Dv[i] * dy + dt * s.z;
+        dr[i] = i < left ? (s.w + uv * s.z) * sigmoid_f(to_f(cd.v[i]) + bias[i]) : 0.f;
+        dD[i] += dy * uv;
+        dbias[i] += dr[i];
+        const float zv = to_f(cz.v[i]), sg = sigmoid_f(zv);
+        dz[i] = to_f(co.v[i]) * (yb[lt][lc + i] + Dv[i] * uv) * (sg * (1.f + zv * (1.f - sg)));
+      }
+      const int64_t o = (w.b * f.L + t) * f.dim + w.ch;
+      store_channels<E, WIDE>(at<T>(a.du, o, oo), left, du);
+      store_channels<E, WIDE>(at<T>(a.ddelta, o, oo), left, dr);
+      if (z) store_channels<E, WIDE>(at<T>(a.dz, o, oo), left, dz);
+    }
+    // this workgroup's share of dB and dC
+    const int64_t tile = w.c0 / CW;
+    for (int i = tid; i < TT * 2 * NP; i += NT) {
+      const int k = i / (2 * NP), j = i - k * 2 * NP;
+      if (t + k < t1)
+        a.bc[(((tile * f.B + w.b) * f.L + t + k) * f.groups + w.g) * (2 * NP) + j] = bc[0][k][j] + bc[1][k][j] + bc[2][k][j] + bc[3][k][j];
+    }
   }
   float* part = a.part + w.row * ((int64_t)f.dim * (f.N + 2));
   if (on) {
@@ -649,7 +760,6 @@ template <typename T, int S, bool W4> __global__ __launch_bounds__(NT) void scan
 
 // ---- host
 int lanes_of(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
-int host_tile_f(int S) { return tile_f(S); }
 
 bool scan_ok(const pnp_scan_desc* d) {
   return d && d->B >= 0 && d->L >= 0 && d->dim > 0 && d->dim <= (1 << 24) && d->N >= 1 && d->N <= 64 && d->groups >= 1 &&
@@ -661,7 +771,7 @@ struct Plan { int S, tiles, nch; int64_t chunk, nck, blocks; };
 Plan plan(const pnp_scan_desc* d) {
   Plan p;
   p.S = lanes_of(d->N);
-  const int per = d->dim / d->groups, tt = host_tile_f(p.S);
+  const int per = d->dim / d->groups, tt = 32;   // (a multiple of every tile)
   p.tiles = (int)ceil_div(per, NT / p.S);
   const int64_t base = d->B * d->groups * p.tiles;
   int64_t nch = 1;
@@ -724,12 +834,12 @@ int32_t chain(const ScanArgs& a, const float* first, int S, int back, hipStream_
 }
 
 template <typename T, int S> int32_t run_scan(ScanArgs a, int64_t blocks, hipStream_t st) {
-  constexpr int E = tile_f(S) / S, V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
+  constexpr int E = tile_f(S, sizeof(T)) / S, V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
   const bool wide = bc_even(a, sizeof(T)) && a.per % V == 0 && a.dim % V == 0 && even(a.u, a.ub, a.ut, V, sizeof(T)) && even(a.delta, a.db, a.dt, V, sizeof(T)) &&
            even(a.z, a.zb, a.zt, V, sizeof(T)) && even(a.out, 0, 0, V, sizeof(T));
   auto go = [&](auto w) -> int32_t {
     if (a.nch > 1) {
-      hipLaunchKernelGGL((scan_fwd_kernel<T, S, true, w>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+      hipLaunchKernelGGL((scan_fwd_kernel<T, S, true, w>), dim3((unsigned)(blocks / a.nch * (a.nch - 1))), dim3(NT), 0, st, a);
       if (const int32_t rc = pnp_check_launch("scan_fwd_kernel (chunks)")) return rc;
       if (const int32_t rc = chain(a, a.state, S, 0, st)) return rc;
     }
@@ -740,18 +850,19 @@ template <typename T, int S> int32_t run_scan(ScanArgs a, int64_t blocks, hipStr
 }
 
 template <typename T, int S> int32_t run_scan_bwd(ScanBwdArgs a, int64_t blocks, hipStream_t st) {
-  constexpr int E = tile_b(S) / S, V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
+  // the wider of the two kernels' packs
+  constexpr int E = tile_f(S, sizeof(T)) / S, V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
   ScanArgs& f = a.f;
   const bool wide = bc_even(f, sizeof(T)) && f.per % V == 0 && f.dim % V == 0 && even(f.u, f.ub, f.ut, V, sizeof(T)) && even(f.delta, f.db, f.dt, V, sizeof(T)) &&
            even(f.z, f.zb, f.zt, V, sizeof(T)) && even(a.dout, a.ob, a.ot, V, sizeof(T)) && even(a.du, 0, 0, V, sizeof(T)) &&
            even(a.ddelta, 0, 0, V, sizeof(T)) && even(a.dz, 0, 0, V, sizeof(T));
   auto go = [&](auto w) -> int32_t {
     if (f.nch > 1) {
-      hipLaunchKernelGGL((scan_bwd_kernel<T, S, true, w>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
-      if (const int32_t rc = pnp_check_launch("scan_bwd_kernel (chunks)")) return rc;
+      hipLaunchKernelGGL((scan_adjoint_kernel<T, S, w>), dim3((unsigned)(blocks / f.nch * (f.nch - 1))), dim3(NT), 0, st, a);
+      if (const int32_t rc = pnp_check_launch("scan_adjoint_kernel")) return rc;
       if (const int32_t rc = chain(f, a.dlast, S, 1, st)) return rc;
     }
-    hipLaunchKernelGGL((scan_bwd_kernel<T, S, false, w>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    hipLaunchKernelGGL((scan_bwd_kernel<T, S, w>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
     return pnp_check_launch("scan_bwd_kernel");
   };
   if (const int32_t rc = wide ? go(std::true_type()) : go(std::false_type())) return rc;
