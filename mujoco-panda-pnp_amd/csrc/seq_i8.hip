@@ -3,8 +3,11 @@
 //
 // Both operands run along k in memory, so a lane's 16 bytes of a row are its operand of
 // v_mfma_i32_16x16x64_i8 as they lie (any order of k serves, as long as both operands have the same).
-// The weights are the instruction's rows and the tokens its columns: a lane then holds 4 neighbouring
-// output channels of one token and stores them together.
+// The weights are the instruction's rows and the tokens its columns: a lane then holds 4 output channels
+// of one token.  The channels of a wave are dealt to its fragments so that a lane's 4 of each lie together:
+// fragment i's row 4 g + r is channel 4 WN g + 4 i + r, and a lane stores 4 WN neighbouring channels.
+#include <type_traits>
+
 #include "seq_dev.h"
 
 namespace seq {
@@ -18,6 +21,7 @@ struct I8Args {
   const int8_t *q, *w;
   const float *scale, *wscale, *bias;
   void* out;
+  int wide;   // rows of out start on 16-byte boundaries
 };
 
 // 16 bytes of a row from k on, zeros past its K elements; any alignment
@@ -35,88 +39,236 @@ __device__ __forceinline__ v4i load16(const int8_t* row, int k, int K) {
   return v;
 }
 
-// 4 neighbouring channels of one token
-template <typename T> __device__ __forceinline__ void store4(const I8Args& a, int64_t m, int n, v4i acc) {
-  if (m >= a.M) return;
+// 16 bytes a lane from memory to LDS, at `lds` + 16 * lane, without registers.  Written out, since the
+// compiler cannot tell the stages apart and would let every read of LDS wait for every such load: whoever
+// reads what it brings waits for it (s_waitcnt vmcnt) and for the other waves (a barrier) itself.
+__device__ __forceinline__ void load_to_lds(const int8_t* p, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
+// Workgroups go to the 8 XCDs in turn: each XCD gets a run of tiles of its own, and walks it in blocks of
+// 8 tiles along the tokens, so that its L2 holds the rows and columns that the tiles at work share.
+__device__ __forceinline__ void tile_of(int id, int tiles_n, int tiles_m, int& tn, int& tm) {
+  const int total = tiles_n * tiles_m, per = total / 8, rest = total % 8;
+  const int x = id % 8, k = id / 8;
+  const int t = x * per + (x < rest ? x : rest) + k;   // the x-th run: the first `rest` of them have one more
+  const int band = t / (8 * tiles_n), h = tiles_m - 8 * band < 8 ? tiles_m - 8 * band : 8, r = t - band * 8 * tiles_n;
+  tn = r / h;
+  tm = 8 * band + r % h;
+}
+
+// what a lane's channels n .. n + C - 1 are scaled by and get added
+template <int C> struct Channels {
+  float s[C], b[C];
+  __device__ __forceinline__ Channels(const I8Args& a, int n) {
+#pragma unroll
+    for (int i = 0; i < C; i++) {
+      s[i] = n + i < a.N ? a.wscale[n + i] : 0.f;
+      b[i] = a.bias && n + i < a.N ? a.bias[n + i] : 0.f;
+    }
+  }
+};
+template <typename T, int C>
+__device__ __forceinline__ void store_token(const I8Args& a, int64_t m, int n, const int (&acc)[C], const Channels<C>& ch) {
+  if (m >= a.M || n >= a.N) return;
   const float sm = a.scale[m];
   T* o = (T*)a.out + m * a.N + n;
-  float f[4];
+  float f[C];
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    f[i] = 0.f;
-    if (n + i < a.N) f[i] = (float)acc[i] * sm * a.wscale[n + i] + (a.bias ? a.bias[n + i] : 0.f);
-  }
-  if (n + 4 <= a.N && (a.N & 3) == 0) {
-    store_f<4>(o, f);
+  for (int i = 0; i < C; i++) f[i] = (float)acc[i] * sm * ch.s[i] + ch.b[i];
+  constexpr int V = C * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : C;
+  if (a.wide) {   // N is a multiple of the pack: a pack is whole or past the end
+#pragma unroll
+    for (int i = 0; i < C; i += V) {
+      float w[V];
+#pragma unroll
+      for (int k = 0; k < V; k++) w[k] = f[i + k];
+      if (n + i < a.N) store_f<V>(o + i, w);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < C; i++)
       if (n + i < a.N) o[i] = from_f<T>(f[i]);
   }
 }
 
-// A BN (channels) x BM (tokens) tile by 4 waves, 2 x 2, 128 bytes of k at a time through LDS.
-// A row of the tile is 128 bytes, 8 chunks; chunk c of row r lies at c ^ (r / 2 % 8), so the 16 rows
-// that a fragment's 16 lanes read lie in 16 different bank groups.
-template <typename T, int BM, int BN> __global__ __launch_bounds__(256) void i8_tile_kernel(I8Args a) {
-  constexpr int WM = BM / 2 / 16, WN = BN / 2 / 16;
-  __shared__ v4i sw[BN * 8], sq[BM * 8];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wn = (wave & 1) * (BN / 2), wm = (wave >> 1) * (BM / 2);
-  const int n0 = blockIdx.x * BN;
-  const int64_t m0 = (int64_t)blockIdx.y * BM;
+constexpr int BK = 64;   // bytes of k a stage
+
+// A BN (channels) x BM (tokens) tile by WGN x WGM waves, a stage of BK bytes of k of both operands at a time
+// through LDS.  A row of a stage is 4 chunks of 16 bytes; chunk c of row r lies at c ^ f(r), f the bits of r
+// in which the 4 groups of a fragment's 16 rows differ (r / 4 for tokens, r / (4 WN) for channels, mod 4): the 16 lanes
+// that read one chunk then meet 16 different bank groups.
+//
+// FAST (rows on 16-byte boundaries, K a multiple of 16): ST stages, filled ST - 1 ahead by loads into LDS; such
+// a load writes 64 lanes' chunks in a row, so the lane's global address carries the exchange; chunks past K come
+// from `zeros`.  Otherwise two stages, by way of registers.
+__device__ const v4i zeros[1] = {};
+
+template <typename T, int BM, int BN, int WGM, int WGN, bool FAST>
+__global__ __launch_bounds__(64 * WGM* WGN, 2) void i8_tile_kernel(I8Args a) {
+  constexpr int NT = 64 * WGM * WGN, ST = FAST ? 4 : 2, WM = BM / WGM / 16, WN = BN / WGN / 16, C = 4 * WN;
+  constexpr int LW = BN * 4 / NT, LQ = BM * 4 / NT;   // chunks of a stage a thread
+  static_assert(LW * NT == BN * 4 && LQ * NT == BM * 4, "whole chunks a thread");
+  __shared__ v4i sw[ST][BN * 4], sq[ST][BM * 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = (wave % WGN) * (BN / WGN), wm = (wave / WGN) * (BM / WGM);
+  int tn, tm;
+  tile_of(blockIdx.x, (a.N + BN - 1) / BN, (int)((a.M + BM - 1) / BM), tn, tm);
+  const int n0 = tn * BN;
+  const int64_t m0 = (int64_t)tm * BM;
+  const int nk = (a.K + BK - 1) / BK;
+  // the thread's rows and chunks; rows past the end are the last one's again, and their results are not stored
+  const int8_t *pw[LW], *pq[LQ];
+  int cw[LW], cq[LQ];
+#pragma unroll
+  for (int i = 0; i < LW; i++) {
+    const int r = (i * NT + tid) >> 2;
+    cw[i] = ((tid & 3) ^ (r / C & 3)) * 16;
+    pw[i] = a.w + (int64_t)(n0 + r < a.N ? n0 + r : a.N - 1) * a.ws;
+  }
+#pragma unroll
+  for (int i = 0; i < LQ; i++) {
+    const int r = (i * NT + tid) >> 2;
+    cq[i] = ((tid & 3) ^ (r >> 2 & 3)) * 16;
+    pq[i] = a.q + (m0 + r < a.M ? m0 + r : a.M - 1) * a.qs;
+  }
   v4i acc[WN][WM];
 #pragma unroll
   for (int i = 0; i < WN; i++)
 #pragma unroll
     for (int j = 0; j < WM; j++) acc[i][j] = v4i{0, 0, 0, 0};
-  for (int k0 = 0; k0 < a.K; k0 += 128) {
+  const int fr = lane & 15, fc = lane >> 4;
+  auto product = [&](int buf) {
+    v4i fw[WN], fq[WM];
 #pragma unroll
-    for (int i = 0; i < BN * 8 / 256; i++) {
-      const int s = i * 256 + tid, r = s >> 3, c = (s & 7) ^ ((r >> 1) & 7);
-      const int n = n0 + r < a.N ? n0 + r : a.N - 1;
-      sw[s] = load16(a.w + n * a.ws, k0 + c * 16, a.K);
+    for (int i = 0; i < WN; i++) {
+      const int r = wn + (fr >> 2) * C + i * 4 + (fr & 3);
+      fw[i] = sw[buf][r * 4 + (fc ^ (r / C & 3))];
     }
 #pragma unroll
-    for (int i = 0; i < BM * 8 / 256; i++) {
-      const int s = i * 256 + tid, r = s >> 3, c = (s & 7) ^ ((r >> 1) & 7);
-      const int64_t m = m0 + r < a.M ? m0 + r : a.M - 1;
-      sq[s] = load16(a.q + m * a.qs, k0 + c * 16, a.K);
+    for (int j = 0; j < WM; j++) {
+      const int r = wm + j * 16 + fr;
+      fq[j] = sq[buf][r * 4 + (fc ^ (r >> 2 & 3))];
     }
-    __syncthreads();
-#pragma unroll
-    for (int kk = 0; kk < 2; kk++) {
-      v4i fw[WN], fq[WM];
-      const int c = kk * 4 + (lane >> 4);
-#pragma unroll
-      for (int i = 0; i < WN; i++) {
-        const int r = wn + i * 16 + (lane & 15);
-        fw[i] = sw[r * 8 + (c ^ ((r >> 1) & 7))];
-      }
-#pragma unroll
-      for (int j = 0; j < WM; j++) {
-        const int r = wm + j * 16 + (lane & 15);
-        fq[j] = sq[r * 8 + (c ^ ((r >> 1) & 7))];
-      }
-#pragma unroll
-      for (int i = 0; i < WN; i++)
-#pragma unroll
-        for (int j = 0; j < WM; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i], fq[j], acc[i][j], 0, 0, 0);
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < WN; i++)
 #pragma unroll
     for (int j = 0; j < WM; j++)
-      store4<T>(a, m0 + wm + j * 16 + (lane & 15), n0 + wn + i * 16 + (lane >> 4) * 4, acc[i][j]);
+#pragma unroll
+      for (int i = 0; i < WN; i++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i], fq[j], acc[i][j], 0, 0, 0);
+  };
+  if constexpr (FAST) {
+    const uint32_t lw = lds_address(&sw[0][wave * 64]), lq = lds_address(&sq[0][wave * 64]);
+    auto fetch = [&](int s) {   // stage s; past the last one: zeros that nobody reads, so that every wave counts the same loads
+      const int buf = s % ST, k = s * BK;
+#pragma unroll
+      for (int i = 0; i < LW; i++)
+        load_to_lds(k + cw[i] < a.K ? pw[i] + k + cw[i] : (const int8_t*)zeros, lw + (buf * BN * 4 + i * NT) * 16);
+#pragma unroll
+      for (int i = 0; i < LQ; i++)
+        load_to_lds(k + cq[i] < a.K ? pq[i] + k + cq[i] : (const int8_t*)zeros, lq + (buf * BM * 4 + i * NT) * 16);
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; s++) fetch(s);
+    for (int s = 0; s < nk; s++) {
+      // this wave's loads of stage s have arrived
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 2) * (LW + LQ)) : "memory");
+      __builtin_amdgcn_s_barrier();   // everybody's have, and everybody has read stage s - 1
+      fetch(s + ST - 1);
+      product(s % ST);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the workgroup
+  } else {
+    v4i rw[LW], rq[LQ];
+    auto fetch = [&](int s) {
+#pragma unroll
+      for (int i = 0; i < LW; i++) rw[i] = load16(pw[i], s * BK + cw[i], a.K);
+#pragma unroll
+      for (int i = 0; i < LQ; i++) rq[i] = load16(pq[i], s * BK + cq[i], a.K);
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+      for (int i = 0; i < LW; i++) sw[buf][i * NT + tid] = rw[i];
+#pragma unroll
+      for (int i = 0; i < LQ; i++) sq[buf][i * NT + tid] = rq[i];
+    };
+    fetch(0);
+    put(0);
+    for (int s = 0; s < nk; s++) {
+      __syncthreads();   // stage s is there, and everybody has read stage s - 1
+      if (s + 1 < nk) fetch(s + 1);
+      product(s & 1);
+      if (s + 1 < nk) put((s + 1) & 1);
+    }
+  }
+  const int n = n0 + wn + fc * C;
+  const Channels<C> ch(a, n);
+#pragma unroll
+  for (int j = 0; j < WM; j++) {
+    int o[C];
+#pragma unroll
+    for (int i = 0; i < WN; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) o[4 * i + r] = acc[i][j][r];
+    store_token<T, C>(a, m0 + wm + j * 16 + fr, n, o, ch);
+  }
 }
 
-template <typename T> int32_t run_i8(const I8Args& a, hipStream_t st) {
-  constexpr int BM = 128, BN = 128;
-  const dim3 grid((unsigned)ceil_div(a.N, BN), (unsigned)ceil_div(a.M, BM));
-  hipLaunchKernelGGL((i8_tile_kernel<T, BM, BN>), grid, dim3(256), 0, st, a);
+// Few tokens (16 MT at most): the weights' bytes are what counts.  A workgroup has 16 channels, its 4 waves the
+// stages of k in turn, straight from memory to registers; their sums meet in LDS.
+template <typename T, int MT> __global__ __launch_bounds__(256) void i8_rows_kernel(I8Args a) {
+  __shared__ v4i part[3][MT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fc = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const int8_t* w = a.w + (int64_t)(n0 + fr < a.N ? n0 + fr : a.N - 1) * a.ws;
+  const int8_t* q[MT];
+#pragma unroll
+  for (int j = 0; j < MT; j++) q[j] = a.q + (j * 16 + fr < a.M ? j * 16 + fr : a.M - 1) * a.qs;
+  v4i acc[MT];
+#pragma unroll
+  for (int j = 0; j < MT; j++) acc[j] = v4i{0, 0, 0, 0};
+#pragma unroll 4
+  for (int k = wave * BK + fc * 16; k - fc * 16 < a.K; k += 4 * BK) {
+    const v4i fw = load16(w, k, a.K);
+#pragma unroll
+    for (int j = 0; j < MT; j++) acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw, load16(q[j], k, a.K), acc[j], 0, 0, 0);
+  }
+  if (wave)
+#pragma unroll
+    for (int j = 0; j < MT; j++) part[wave - 1][j][lane] = acc[j];
+  __syncthreads();
+  if (wave) return;
+  const Channels<4> ch(a, n0 + fc * 4);
+#pragma unroll
+  for (int j = 0; j < MT; j++) {
+    const v4i s = acc[j] + part[0][j][lane] + part[1][j][lane] + part[2][j][lane];
+    const int o[4] = {s[0], s[1], s[2], s[3]};
+    store_token<T, 4>(a, j * 16 + fr, n0 + fc * 4, o, ch);
+  }
+}
+
+// ---- host
+template <typename T, int BM, int BN, int WGM, int WGN> int32_t launch_tile(const I8Args& a, bool fast, hipStream_t st) {
+  const dim3 grid((unsigned)(ceil_div(a.M, BM) * ceil_div(a.N, BN))), block(64 * WGM * WGN);
+  if (fast) hipLaunchKernelGGL((i8_tile_kernel<T, BM, BN, WGM, WGN, true>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((i8_tile_kernel<T, BM, BN, WGM, WGN, false>), grid, block, 0, st, a);
   return pnp_check_launch("i8_tile_kernel");
+}
+
+template <typename T> int32_t run_i8(I8Args a, hipStream_t st) {
+  a.wide = a.N % (16 / (int)sizeof(T)) == 0 && aligned_to(a.out, 16);
+  const bool fast = a.K % 16 == 0 && a.qs % 16 == 0 && a.ws % 16 == 0 && aligned_to(a.q, 16) && aligned_to(a.w, 16);
+  const dim3 rows((unsigned)ceil_div(a.N, 16)), block(256);
+  if (a.M <= 16) hipLaunchKernelGGL((i8_rows_kernel<T, 1>), rows, block, 0, st, a);
+  else if (a.M <= 32) hipLaunchKernelGGL((i8_rows_kernel<T, 2>), rows, block, 0, st, a);
+  else if (a.M <= 64) hipLaunchKernelGGL((i8_rows_kernel<T, 4>), rows, block, 0, st, a);
+  if (a.M <= 64) return pnp_check_launch("i8_rows_kernel");
+  // the largest tile that still gives most of the 256 CUs one
+  const auto tiles = [&](int b) { return ceil_div(a.M, b) * ceil_div(a.N, b); };
+  if (tiles(256) >= 192) return launch_tile<T, 256, 256, 2, 4>(a, fast, st);
+  if (tiles(128) >= 192) return launch_tile<T, 128, 128, 2, 2>(a, fast, st);
+  return launch_tile<T, 64, 64, 2, 2>(a, fast, st);
 }
 
 }  // namespace
@@ -126,10 +278,14 @@ using namespace seq;
 
 extern "C" int32_t pnp_matmul_i8(const pnp_i8_desc* d, void* stream) {
   const char* fn = "pnp_matmul_i8";
-  // 65535 * 64 tokens: a grid's second dimension; 131071 * 127 * 127 < 2^31
-  if (!d || d->M < 0 || d->M > 65535 * (int64_t)64 || d->N <= 0 || d->N > (1 << 24) || d->K <= 0 || d->K > 131071 ||
+  // 131071 * 128 * 128 < 2^31
+  if (!d || d->M < 0 || d->M > ((int64_t)1 << 31) || d->N <= 0 || d->N > (1 << 24) || d->K <= 0 || d->K > 131071 ||
       !type_bytes(d->out_type) || d->q_stride < d->K || d->wq_stride < d->K) {
     pnp_set_error("%s: bad shape or type", fn);
+    return PNP_ERR_ARG;
+  }
+  if (ceil_div(d->M, 64) * ceil_div(d->N, 64) >= ((int64_t)1 << 23)) {
+    pnp_set_error("%s: too many tiles for one launch", fn);
     return PNP_ERR_ARG;
   }
   if (!d->M) return PNP_OK;
@@ -137,7 +293,7 @@ extern "C" int32_t pnp_matmul_i8(const pnp_i8_desc* d, void* stream) {
     pnp_set_error("%s: null buffer", fn);
     return PNP_ERR_ARG;
   }
-  I8Args a{d->M, d->q_stride, d->wq_stride, d->N, d->K, d->q, d->wq, d->scale, d->wscale, d->bias, d->out};
+  I8Args a{d->M, d->q_stride, d->wq_stride, d->N, d->K, d->q, d->wq, d->scale, d->wscale, d->bias, d->out, 0};
   const hipStream_t st = (hipStream_t)stream;
   return SEQ_BY_TYPE(d->out_type, T, return run_i8<T>(a, st));
 }

@@ -134,7 +134,8 @@ def test_rows_in_8_bits(S, dtype):
 
 # ---------------------------------------------------------------------------------- product
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 1000, 512), (3, 17, 15), (16, 64, 16), (33, 40, 100), (65, 130, 257), (128, 128, 128),
-                                   (200, 300, 1000), (257, 512, 640), (500, 260, 2064), (64, 1024, 4096), (7, 4099, 129)])
+                                   (200, 300, 1000), (257, 512, 640), (500, 260, 2064), (64, 1024, 4096), (7, 4099, 129), (2100, 2060, 208),
+                                   (4096, 1030, 1040), (1025, 4609, 16)])
 def test_product(S, M, N, K):
     d = Draw(M + N + K)
     q = torch.randint(-128, 128, (M, K), generator=d.g, dtype=torch.int8)
