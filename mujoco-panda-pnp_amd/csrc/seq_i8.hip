@@ -96,11 +96,14 @@ __device__ __forceinline__ void store_token(const I8Args& a, int64_t m, int n, c
 }
 
 constexpr int BK = 64;   // bytes of k a stage
+__device__ __forceinline__ int k_of(int g) { return g == 0 ? 0 : g == 1 ? 3 : g == 2 ? 1 : 2; }
 
 // A BN (channels) x BM (tokens) tile by WGN x WGM waves, a stage of BK bytes of k of both operands at a time
 // through LDS.  A row of a stage is 4 chunks of 16 bytes; chunk c of row r lies at c ^ f(r), f the bits of r
-// in which the 4 groups of a fragment's 16 rows differ (r / 4 for tokens, r / (4 WN) for channels, mod 4): the 16 lanes
-// that read one chunk then meet 16 different bank groups.
+// in which the 4 groups of a fragment's 16 rows differ (r / 4 for tokens, r / (4 WN) for channels, mod 4).  LDS
+// serves a 16-byte read 16 lanes at a time, of the first 32 lanes 0 .. 3, 12 .. 15, 20 .. 27 and then the others;
+// with chunk k_of(g) for the lanes' g-th sixteen (any order of k serves) each such set meets 16 different bank
+// groups: 2.0 -> 1.0 cycles of LDS a read against the order 0, 1, 2, 3.
 //
 // FAST (rows on 16-byte boundaries, K a multiple of 16): ST stages, filled ST - 1 ahead by loads into LDS; such
 // a load writes 64 lanes' chunks in a row, so the lane's global address carries the exchange; chunks past K come
@@ -140,18 +143,18 @@ __global__ __launch_bounds__(64 * WGM* WGN, 2) void i8_tile_kernel(I8Args a) {
   for (int i = 0; i < WN; i++)
 #pragma unroll
     for (int j = 0; j < WM; j++) acc[i][j] = v4i{0, 0, 0, 0};
-  const int fr = lane & 15, fc = lane >> 4;
+  const int fr = lane & 15, fc = lane >> 4, kc = k_of(fc);
   auto product = [&](int buf) {
     v4i fw[WN], fq[WM];
 #pragma unroll
     for (int i = 0; i < WN; i++) {
       const int r = wn + (fr >> 2) * C + i * 4 + (fr & 3);
-      fw[i] = sw[buf][r * 4 + (fc ^ (r / C & 3))];
+      fw[i] = sw[buf][r * 4 + (kc ^ (r / C & 3))];
     }
 #pragma unroll
     for (int j = 0; j < WM; j++) {
       const int r = wm + j * 16 + fr;
-      fq[j] = sq[buf][r * 4 + (fc ^ (r >> 2 & 3))];
+      fq[j] = sq[buf][r * 4 + (kc ^ (r >> 2 & 3))];
     }
 #pragma unroll
     for (int j = 0; j < WM; j++)
