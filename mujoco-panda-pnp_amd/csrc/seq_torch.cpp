@@ -154,6 +154,9 @@ variable_list once(variable_list grads, const char* name) {
 }
 
 // ---- norm
+// [..., dim] as rows
+Tensor rows_of(const Tensor& t) { return t.defined() ? lines(t.dim() == 2 ? t : t.reshape({-1, t.size(-1)})) : t; }
+
 pnp_norm_desc norm_desc(const Tensor& x, const Tensor& r, const Tensor& w, double eps) {
   pnp_norm_desc d{};
   d.rows = x.size(0); d.dim = (int32_t)x.size(1); d.type = code_of(x.scalar_type()); d.eps = (float)eps;
@@ -165,9 +168,10 @@ pnp_norm_desc norm_desc(const Tensor& x, const Tensor& r, const Tensor& w, doubl
 
 struct NormRun { Tensor y, s, rstd; };
 NormRun norm_run(const Tensor& x, const Tensor& r, const Tensor& w, double eps, bool train) {
-  NormRun o{fresh(x.sizes(), x.scalar_type(), x), x, train ? fresh({x.size(0)}, at::kFloat, x) : Tensor()};
+  const Tensor x2 = rows_of(x), r2 = rows_of(r);
+  NormRun o{fresh(x.sizes(), x.scalar_type(), x), x, train ? fresh({x2.size(0)}, at::kFloat, x) : Tensor()};
   if (r.defined()) o.s = fresh(x.sizes(), r.scalar_type(), x);
-  pnp_norm_desc d = norm_desc(x, r, w, eps);
+  pnp_norm_desc d = norm_desc(x2, r2, w, eps);
   d.y = mptr(o.y); d.rstd = mfloat(o.rstd);
   if (r.defined()) d.s = mptr(o.s);
   CALL(rms_norm, x, &d);
@@ -180,36 +184,35 @@ struct NormFn : torch::autograd::Function<NormFn> {
     const NormRun o = norm_run(x, r, w, eps, true);
     ctx->save_for_backward({o.s, w, o.rstd});
     ctx->saved_data["type"] = (int64_t)x.scalar_type();
-    ctx->saved_data["added"] = r.defined();
-    ctx->saved_data["dw"] = w.requires_grad();
+    ctx->saved_data["flags"] = (int64_t)(r.defined() | (w.requires_grad() << 1));
     ctx->set_materialize_grads(false);
     return {o.y, o.s};   // without a residual s is x: the stream goes on through here, one rounding of dx + ds
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &s = saved[0], &w = saved[1], &rstd = saved[2];
+    const Tensor &s0 = saved[0], &w = saved[1], &rstd = saved[2];
     const ScalarType type = (ScalarType)ctx->saved_data["type"].toInt();
-    const bool added = ctx->saved_data["added"].toBool();
-    Tensor dy = grads[0], ds = grads[1];
-    if (!dy.defined()) {
+    const int64_t flags = ctx->saved_data["flags"].toInt();
+    const bool added = flags & 1;
+    if (!grads[0].defined()) {
+      const Tensor& ds = grads[1];
       if (!ds.defined()) return variable_list(4);
       return once({ds.to(type), added ? ds : Tensor(), Tensor(), Tensor()}, "add_rms_norm");
     }
-    dy = lines(dy);
-    ds = lines(ds);
+    const Tensor s = rows_of(s0), dy = rows_of(grads[0]), ds = rows_of(grads[1]);
     pnp_norm_bwd_desc d{};
     d.rows = s.size(0); d.dim = (int32_t)s.size(1); d.type = code_of(type); d.res_type = code_of(s.scalar_type());
     d.dy = cptr(dy); d.dy_stride = dy.stride(0); d.s = cptr(s); d.s_stride = s.stride(0);
     if (ds.defined()) { d.ds = cptr(ds); d.ds_stride = ds.stride(0); }
     d.weight = cfloat(w); d.rstd = cfloat(rstd);
-    const Tensor dx = fresh(s.sizes(), type, s);
+    const Tensor dx = fresh(s0.sizes(), type, s);
     Tensor dres = dx, dw, ws;
     d.dx = mptr(dx);
     if (s.scalar_type() != type) {
-      dres = fresh(s.sizes(), s.scalar_type(), s);
+      dres = fresh(s0.sizes(), s.scalar_type(), s);
       d.dres = mptr(dres);
     }
-    if (ctx->saved_data["dw"].toBool()) {
+    if (flags & 2) {
       dw = fresh(w.sizes(), at::kFloat, s);
       d.workspace_floats = FLOATS(rms_norm_bwd_workspace, d);
       ws = scratch(d.workspace_floats, s);
@@ -220,34 +223,32 @@ struct NormFn : torch::autograd::Function<NormFn> {
   }
 };
 
-struct NormIn { Tensor x, w, r; };
+struct NormIn { Tensor w, r; };
 NormIn norm_in(const Tensor& x, const MaybeTensor& w, const MaybeTensor& r, double eps) {
   activation(x, "x");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "x: shape ", x.sizes(), ", expected [..., dim] with dim > 0");
   TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative (got ", eps, ")");
-  const int64_t dim = x.size(-1);
   NormIn o;
-  o.w = required(w, "weight", {dim}, x);
+  o.w = required(w, "weight", {x.size(-1)}, x);
   if (r && r->defined()) {
     activation(*r, "residual");
     TORCH_CHECK_TYPE(r->scalar_type() == x.scalar_type() || r->scalar_type() == at::kFloat, "residual: dtype ", r->scalar_type(), ", expected ",
                      x.scalar_type(), " or float32");
     same_device(*r, "residual", x);
     shaped(*r, "residual", x.sizes());
-    o.r = lines(r->reshape({-1, dim}));
+    o.r = *r;
   }
-  o.x = lines(x.reshape({-1, dim}));
   return o;
 }
 
 std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& residual, double eps) {
   const NormIn in = norm_in(x, weight, residual, eps);
-  if (training(in.x, in.w, in.r)) {
-    const variable_list o = NormFn::apply(in.x, maybe(in.r), in.w, eps);
-    return {o[0].view(x.sizes()), o[1].view(x.sizes())};
+  if (training(x, in.w, in.r)) {
+    const variable_list o = NormFn::apply(x, maybe(in.r), in.w, eps);
+    return {o[0], o[1]};
   }
-  const NormRun o = norm_run(in.x, in.r, in.w, eps, false);
-  return {o.y.view(x.sizes()), in.r.defined() ? o.s.view(x.sizes()) : x};
+  const NormRun o = norm_run(x, in.r, in.w, eps, false);
+  return {o.y, o.s};
 }
 
 // 8-bit rows, a multiple of 16 bytes apart: the product's loads want rows on such boundaries
@@ -256,6 +257,7 @@ Q8 q8_out(const Tensor& x) {
   return {fresh({x.size(0), (x.size(1) + 15) / 16 * 16}, at::kChar, x), fresh({x.size(0)}, at::kFloat, x)};
 }
 Q8 q8_view(const Q8& o, at::IntArrayRef shape) {
+  if (shape.size() == 2) return {o.q.size(1) == shape[1] ? o.q : o.q.narrow(1, 0, shape[1]), o.scale};
   std::vector<int64_t> s = shape.vec();
   const Tensor scale = o.scale.view(shape.slice(0, shape.size() - 1));
   s.back() = o.q.size(1);
@@ -265,8 +267,9 @@ Q8 q8_view(const Q8& o, at::IntArrayRef shape) {
 std::tuple<Tensor, Tensor, Tensor> add_rms_norm_q8(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& residual, double eps) {
   serving("add_rms_norm_q8", x, weight, residual);
   const NormIn in = norm_in(x, weight, residual, eps);
-  const Q8 o = q8_out(in.x);
-  pnp_norm_desc d = norm_desc(in.x, in.r, in.w, eps);
+  const Tensor x2 = rows_of(x), r2 = rows_of(in.r);
+  const Q8 o = q8_out(x2);
+  pnp_norm_desc d = norm_desc(x2, r2, in.w, eps);
   d.q = (int8_t*)mptr(o.q); d.q_stride = o.q.stride(0); d.scale = mfloat(o.scale);
   Tensor s = x;
   if (in.r.defined()) {
@@ -282,7 +285,7 @@ std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
   serving("quantize_rows", x);
   activation(x, "x");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "x: shape ", x.sizes(), ", expected [..., dim] with dim > 0");
-  const Tensor x2 = lines(x.reshape({-1, x.size(-1)}));
+  const Tensor x2 = rows_of(x);
   const Q8 o = q8_out(x2);
   CALL(quantize_rows, x, cptr(x2), x2.stride(0), code_of(x.scalar_type()), x2.size(0), (int32_t)x2.size(1), (int8_t*)mptr(o.q), o.q.stride(0),
        mfloat(o.scale));
@@ -348,10 +351,7 @@ struct ConvFn : torch::autograd::Function<ConvFn> {
     const Tensor b = value(b_), starts = value(starts_), state = value(state_);
     const auto [y, last] = conv_run(x, w, b, silu, starts, state);
     ctx->save_for_backward({x, w, b, starts, state});
-    ctx->saved_data["silu"] = silu;
-    ctx->saved_data["dw"] = wants(w);
-    ctx->saved_data["db"] = wants(b);
-    ctx->saved_data["ds"] = wants(state);
+    ctx->saved_data["flags"] = (int64_t)(silu | (wants(w) << 1) | (wants(b) << 2) | (wants(state) << 3));
     ctx->set_materialize_grads(false);
     return {y, last};
   }
@@ -361,14 +361,15 @@ struct ConvFn : torch::autograd::Function<ConvFn> {
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(6);
     const Tensor dy = grads[0].defined() ? lines(grads[0]) : at::zeros(x.sizes(), x.options());
     const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const int64_t flags = ctx->saved_data["flags"].toInt();
     pnp_conv_bwd_desc d{};
-    d.f = conv_desc(x, w, b, ctx->saved_data["silu"].toBool(), starts, state);
+    d.f = conv_desc(x, w, b, flags & 1, starts, state);
     d.dy = cptr(dy); d.dy_bstride = dy.stride(0); d.dy_tstride = dy.stride(1); d.dlast = cptr(dlast);
     const Tensor dx = fresh(x.sizes(), x.scalar_type(), x);
     Tensor dw, db, ds, ws;
-    if (ctx->saved_data["dw"].toBool()) dw = fresh(w.sizes(), at::kFloat, x);
-    if (ctx->saved_data["db"].toBool()) db = fresh(b.sizes(), at::kFloat, x);
-    if (ctx->saved_data["ds"].toBool()) ds = fresh(state.sizes(), x.scalar_type(), x);
+    if (flags & 2) dw = fresh(w.sizes(), at::kFloat, x);
+    if (flags & 4) db = fresh(b.sizes(), at::kFloat, x);
+    if (flags & 8) ds = fresh(state.sizes(), x.scalar_type(), x);
     d.dx = mptr(dx); d.dweight = mfloat(dw); d.dbias = mfloat(db); d.dstate = mptr(ds);
     if (dw.defined() || db.defined()) {
       d.workspace_floats = FLOATS(causal_conv_bwd_workspace, d);
@@ -429,9 +430,9 @@ Tensor causal_conv_step(const Tensor& x_, const Tensor& state, const Tensor& wei
 // ---- selective scan
 struct ScanIn { Tensor u, delta, A, B, C, D, z, bias; };
 
-// [..., groups, N] with both of the last dimensions contiguous
-Tensor packed_groups(const Tensor& t) {
-  const bool ok = (t.size(-1) == 1 || t.stride(-1) == 1) && (t.size(-2) == 1 || t.stride(-2) == t.size(-1));
+// [..., N] or [..., groups, N] with what follows the leading dimensions contiguous
+Tensor packed_groups(const Tensor& t, int64_t lead) {
+  const bool ok = (t.size(-1) == 1 || t.stride(-1) == 1) && (t.dim() == lead + 1 || t.size(-2) == 1 || t.stride(-2) == t.size(-1));
   return ok ? t : t.contiguous();
 }
 
@@ -441,7 +442,7 @@ Tensor near(const Tensor& t, int64_t lead) {
 }
 
 // lead: dimensions before the channels
-ScanIn scan_in(const Tensor& u, const Tensor& delta, const Tensor& A, Tensor B, Tensor C, const MaybeTensor& D, const MaybeTensor& z,
+ScanIn scan_in(const Tensor& u, const Tensor& delta, const Tensor& A, const Tensor& B, const Tensor& C, const MaybeTensor& D, const MaybeTensor& z,
                const MaybeTensor& bias, int64_t lead) {
   activation(u, "u");
   dims(u, "u", lead + 1);
@@ -457,24 +458,20 @@ ScanIn scan_in(const Tensor& u, const Tensor& delta, const Tensor& A, Tensor B, 
   const Tensor A32 = parameter(A, "A", {dim, A.size(1)}, u);
   activation(B, "B", &u);
   activation(C, "C", &u);
-  if (B.dim() == lead + 1 && C.dim() == lead + 1) {
-    B = B.unsqueeze(-2);
-    C = C.unsqueeze(-2);
-  }
-  const int64_t groups = B.dim() == lead + 2 ? B.size(-2) : 0;
+  const int64_t groups = B.dim() == lead + 2 ? B.size(-2) : B.dim() == lead + 1 ? 1 : 0;
   std::vector<int64_t> want = u.sizes().slice(0, lead).vec();
-  want.push_back(groups);
+  if (B.dim() == lead + 2) want.push_back(groups);
   want.push_back(A.size(1));
   TORCH_CHECK_VALUE(groups >= 1 && dim % groups == 0 && B.sizes() == want && C.sizes() == want, "B ", B.sizes(), " and C ", C.sizes(),
                     ": expected ", u.sizes().slice(0, lead), " and then [groups,] ", A.size(1), ", groups dividing ", dim);
-  return {near(lines(u), lead), near(lines(delta), lead), A32, near(packed_groups(B), lead), near(packed_groups(C), lead),
+  return {near(lines(u), lead), near(lines(delta), lead), A32, near(packed_groups(B, lead), lead), near(packed_groups(C, lead), lead),
           parameter(D, "D", {dim}, u), z && z->defined() ? near(lines(*z), lead) : Tensor(), parameter(bias, "delta_bias", {dim}, u)};
 }
 
 pnp_scan_desc scan_desc(const ScanIn& v, const Tensor& starts, const Tensor& state, bool step) {
   pnp_scan_desc d{};
   d.B = v.u.size(0); d.L = step ? 1 : v.u.size(1); d.dim = (int32_t)v.u.size(-1); d.N = (int32_t)v.A.size(1);
-  d.groups = (int32_t)v.B.size(-2); d.type = code_of(v.u.scalar_type());
+  d.groups = v.B.dim() == (step ? 3 : 4) ? (int32_t)v.B.size(-2) : 1; d.type = code_of(v.u.scalar_type());
   auto put = [&](const Tensor& t, const void*& p, int64_t& sb, int64_t& st) {
     if (!t.defined()) return;
     p = cptr(t);
