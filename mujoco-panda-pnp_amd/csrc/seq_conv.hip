@@ -88,7 +88,9 @@ __device__ __forceinline__ void tap_sum(const float (&wt)[W][V], const float (&b
   }
 }
 
-// a lane: V channels of one run.  Lanes of a wave lie along the channels first.
+// A lane: V channels of one run.  Lanes of a wave lie along the channels first.  The next TB tokens are
+// loaded before the first of these is used: the stores between would hold their loads back.
+constexpr int TB = 4;
 template <typename T, int W, int V> __global__ __launch_bounds__(NT) void conv_fwd_kernel(ConvArgs a) {
   const int64_t packs = a.dim / V, id = (int64_t)blockIdx.x * NT + threadIdx.x;
   const int64_t k = id / packs;
@@ -96,24 +98,45 @@ template <typename T, int W, int V> __global__ __launch_bounds__(NT) void conv_f
   const int c = (int)(id - k * packs) * V;
   const int64_t b = k / a.runs, t0 = (k - b * a.runs) * a.run, t1 = t0 + a.run < a.L ? t0 + a.run : a.L;
   const T *x = (const T*)a.x, *state = (const T*)a.state;
-  T* y = (T*)a.y;
   float wt[W][V], bs[V], h[W - 1][V];
   taps<W, V>(a.w, a.bias, c, wt, bs);
   history<W, V>(a, x, state, b, t0, c, h);
   const T* px = x + b * a.xb + t0 * a.xt + c;
-  T* py = y + (b * a.L + t0) * a.dim + c;
+  T* py = (T*)a.y + (b * a.L + t0) * a.dim + c;
   const uint8_t* ps = a.starts ? a.starts + b * a.L : nullptr;
-#pragma unroll 4
-  for (int64_t t = t0; t < t1; t++, px += a.xt, py += a.dim) {
-    float v[V], pre[V];
-    load_f<V>(px, v);
-    if (ps && ps[t]) clear<W, V>(h);
-    tap_sum<W, V>(wt, bs, h, v, pre);
-    if (a.silu)
+  Pack<T, V> next[TB], raw[TB];
+  bool ns[TB], st[TB];
+  auto fetch = [&](int64_t t) {
 #pragma unroll
-      for (int i = 0; i < V; i++) pre[i] *= sigmoid_f(pre[i]);
-    store_f<V>(py, pre);
-    push<W, V>(h, v);
+    for (int k = 0; k < TB; k++)
+      if (t + k < t1) {
+        next[k] = *reinterpret_cast<const Pack<T, V>*>(px + k * a.xt);
+        ns[k] = ps && ps[t + k];
+      }
+    px += TB * a.xt;
+  };
+  fetch(t0);
+  for (int64_t t = t0; t < t1; t += TB, py += (int64_t)TB * a.dim) {
+#pragma unroll
+    for (int k = 0; k < TB; k++) {
+      raw[k] = next[k];
+      st[k] = ns[k];
+    }
+    fetch(t + TB);
+#pragma unroll
+    for (int k = 0; k < TB; k++) {
+      if (t + k >= t1) break;
+      float v[V], pre[V];
+#pragma unroll
+      for (int i = 0; i < V; i++) v[i] = to_f(raw[k].v[i]);
+      if (st[k]) clear<W, V>(h);
+      tap_sum<W, V>(wt, bs, h, v, pre);
+      if (a.silu)
+#pragma unroll
+        for (int i = 0; i < V; i++) pre[i] *= sigmoid_f(pre[i]);
+      store_f<V>(py + (int64_t)k * a.dim, pre);
+      push<W, V>(h, v);
+    }
   }
   if (a.last && t1 == a.L)
 #pragma unroll
@@ -135,9 +158,9 @@ struct ConvBwdArgs {
 // A token's dx needs the dpre of the W - 1 tokens after it: the walk goes W - 1 tokens past the run's
 // end, and dx is written W - 1 tokens behind.  acc[k] holds the sum for token t - k; tokens before the
 // start of t's sequence get nothing from it (age: tokens since the start).
-template <typename T, int W, int V> __global__ __launch_bounds__(NT) void conv_bwd_kernel(ConvBwdArgs a) {
+template <typename T, int W, int V> __global__ __launch_bounds__(NT, 2) void conv_bwd_kernel(ConvBwdArgs a) {
   const ConvArgs& f = a.f;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // (a wave's run, its marks and its age are scalars)
   const int npack = f.dim / V;
   const int pk = blockIdx.x * 64 + lane;
   const bool on = pk < npack;
@@ -161,67 +184,97 @@ template <typename T, int W, int V> __global__ __launch_bounds__(NT) void conv_b
 #pragma unroll
       for (int j = W - 1; j >= 1; j--)
         if (t0 - j >= 0 && ps[t0 - j]) age = j - 1;
-    for (int64_t t = t0; t < t1 + W - 1; t++) {
-      const bool in = t < f.L;
-      if (in) {
-        float v[V], g[V], pre[V];
-        load_f<V>(x + b * f.xb + t * f.xt + c, v);
-        load_f<V>(dy + b * a.dyb + t * a.dyt + c, g);
-        if (ps && ps[t]) {
-          clear<W, V>(h);
-          age = 0;
+    const T *px = x + b * f.xb + t0 * f.xt + c, *pg = dy + b * a.dyb + t0 * a.dyt + c;
+    const int64_t end = t1 + W - 1, held = end < f.L ? end : f.L;   // the walk's end, and the last token there is for it
+    Pack<T, V> nx[TB], ng[TB], rx[TB], rg[TB];
+    bool nm[TB], mark[TB];
+    auto fetch = [&](int64_t tb) {
+#pragma unroll
+      for (int k = 0; k < TB; k++)
+        if (tb + k < held) {
+          nx[k] = *reinterpret_cast<const Pack<T, V>*>(px + k * f.xt);
+          ng[k] = *reinterpret_cast<const Pack<T, V>*>(pg + k * a.dyt);
+          nm[k] = ps && ps[tb + k];
+        }
+      px += TB * f.xt;
+      pg += TB * a.dyt;
+    };
+    fetch(t0);
+    for (int64_t tb = t0; tb < end; tb += TB) {
+#pragma unroll
+      for (int k = 0; k < TB; k++) {
+        rx[k] = nx[k];
+        rg[k] = ng[k];
+        mark[k] = nm[k];
+      }
+      fetch(tb + TB);
+#pragma unroll
+      for (int k = 0; k < TB; k++) {
+        const int64_t t = tb + k;
+        if (t >= end) break;
+        if (t < f.L) {
+          float v[V], g[V], pre[V];
+#pragma unroll
+          for (int i = 0; i < V; i++) {
+            v[i] = to_f(rx[k].v[i]);
+            g[i] = to_f(rg[k].v[i]);
+          }
+          if (mark[k]) {
+            clear<W, V>(h);
+            age = 0;
+          } else if (age < W - 1) {
+            age++;
+          }
+          if (f.silu) {
+            tap_sum<W, V>(wt, bs, h, v, pre);
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+              const float s = sigmoid_f(pre[i]);
+              g[i] *= s * (1.f + pre[i] * (1.f - s));
+            }
+          }
+          if (t < t1) {
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+#pragma unroll
+              for (int j = 0; j < W - 1; j++) dw[j][i] += g[i] * h[j][i];
+              dw[W - 1][i] += g[i] * v[i];
+              db[i] += g[i];
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < W; j++)
+            if (j <= age)
+#pragma unroll
+              for (int i = 0; i < V; i++) acc[j][i] += wt[W - 1 - j][i] * g[i];
+          push<W, V>(h, v);
         } else if (age < W - 1) {
           age++;
         }
-        if (f.silu) {
-          tap_sum<W, V>(wt, bs, h, v, pre);
+        // what last_state's gradient brings, at the walk's first token past the last: its row W - 1 - j is token L - j,
+        // held in acc[j], if that still belongs to the sequence
+        if (dlast && t == f.L) {
 #pragma unroll
-          for (int i = 0; i < V; i++) {
-            const float s = sigmoid_f(pre[i]);
-            g[i] *= s * (1.f + pre[i] * (1.f - s));
-          }
+          for (int j = 1; j < W; j++)
+            if (j <= age) {
+              float g[V];
+              load_f<V>(dlast + (b * (W - 1) + W - 1 - j) * f.dim + c, g);
+#pragma unroll
+              for (int i = 0; i < V; i++) acc[j][i] += g[i];
+            }
         }
-        if (t < t1) {
-#pragma unroll
-          for (int i = 0; i < V; i++) {
-#pragma unroll
-            for (int j = 0; j < W - 1; j++) dw[j][i] += g[i] * h[j][i];
-            dw[W - 1][i] += g[i] * v[i];
-            db[i] += g[i];
-          }
+        const int64_t o = t - (W - 1);
+        if (on && o >= first && o < t1) {
+          if (o >= 0) store_f<V>((T*)a.dx + (b * f.L + o) * f.dim + c, acc[W - 1]);
+          else if (a.dstate) store_f<V>((T*)a.dstate + (b * (W - 1) + o + W - 1) * f.dim + c, acc[W - 1]);
         }
 #pragma unroll
-        for (int j = 0; j < W; j++)
-          if (j <= age)
+        for (int j = W - 1; j > 0; j--)
 #pragma unroll
-            for (int i = 0; i < V; i++) acc[j][i] += wt[W - 1 - j][i] * g[i];
-        push<W, V>(h, v);
-      } else if (age < W - 1) {
-        age++;
+          for (int i = 0; i < V; i++) acc[j][i] = acc[j - 1][i];
+#pragma unroll
+        for (int i = 0; i < V; i++) acc[0][i] = 0.f;
       }
-      // what last_state's gradient brings: its row j is token L - W + 1 + j.  All of it is added at the
-      // walk's first token at or past L (or at its last one of L), where `age` says what still belongs to the sequence
-      if (dlast && t == f.L) {
-#pragma unroll
-        for (int j = 1; j < W; j++)   // token L - j: row W - 1 - j, held in acc[j]
-          if (j <= age) {
-            float g[V];
-            load_f<V>(dlast + (b * (W - 1) + W - 1 - j) * f.dim + c, g);
-#pragma unroll
-            for (int i = 0; i < V; i++) acc[j][i] += g[i];
-          }
-      }
-      const int64_t o = t - (W - 1);
-      if (on && o >= first && o < t1) {
-        if (o >= 0) store_f<V>((T*)a.dx + (b * f.L + o) * f.dim + c, acc[W - 1]);
-        else if (a.dstate) store_f<V>((T*)a.dstate + (b * (W - 1) + o + W - 1) * f.dim + c, acc[W - 1]);
-      }
-#pragma unroll
-      for (int j = W - 1; j > 0; j--)
-#pragma unroll
-        for (int i = 0; i < V; i++) acc[j][i] = acc[j - 1][i];
-#pragma unroll
-      for (int i = 0; i < V; i++) acc[0][i] = 0.f;
     }
   }
   if (!a.part) return;
@@ -309,11 +362,12 @@ template <typename F> int32_t by_width(int W, F f) {
 bool on_pack(const void* p, size_t bytes) { return !p || aligned_to(p, bytes); }
 
 constexpr int VB = 4;         // channels a lane of the gradient: the filters, their sums and the tokens under them in registers
-// tokens of a run: long enough that the W - 1 tokens a run reads twice are few, short enough to fill the chip
+// tokens of a run: long enough that the W - 1 tokens a run reads twice are few, short enough for 2 waves a SIMD,
+// a sequence's runs of one length
 int run_length(int64_t B, int64_t L, int64_t packs) {
   int run = 64;
-  while (run > 8 && B * ceil_div(L, run) * packs < 256 * 1024) run /= 2;
-  return run;
+  while (run > 8 && B * ceil_div(L, run) * packs < 128 * 1024) run /= 2;
+  return L ? (int)ceil_div(L, ceil_div(L, run)) : run;
 }
 int64_t bwd_parts(int64_t B, int64_t L, int64_t packs, int run) {
   const int64_t cols = ceil_div(packs, 64), rows = ceil_div(B * ceil_div(L, run), 4);
