@@ -28,6 +28,9 @@ Multi-GPU: one process per GPU, each with its own env batch and re
 gradients are averaged with one all-reduce per optimiser (a single flattened bucket over RCCL /
 xGMI), parameters start from rank 0's, and obs statistics are merged as above, so the ranks stay
 in lockstep (data-parallel learner).
+
+A policy with memory (``TQCConfig(history=H)``; not in the reference): actor and critics see, next to the
+observation, features of the last H steps from ``pnp_amd.history.HistoryEncoder``.
 """
 from __future__ import annotations
 
@@ -80,6 +83,14 @@ class TQCConfig:
     # graph's generator bookkeeping less per gradient step.  Same distributions, other numbers
     # than the generator's; False draws from the generator (the tests' bit-exact comparisons)
     device_rng: bool = True
+    # a policy with memory: features of the last `history` steps (pnp_amd.history.HistoryEncoder, trained by
+    # the critics' loss, with a Polyak-averaged target copy) appended to the observation of the actor and the
+    # critics; the replay samples windows, the rollout carries a state per env.  0: none (the reference's policy)
+    history: int = 0
+    history_dim: int = 256               # features, and the blocks' width
+    history_layers: int = 1
+    # the rollout's and the evaluation's encoder with its products in 8 bits (weights quantised after updates)
+    rollout_int8: bool = False
 
 
 def _world():
@@ -166,7 +177,7 @@ class DictReplayBuffer:
     """sb3 DictReplayBuffer (optimize_memory_usage=False, handle_timeout_termination=True) on the
     device; the dict keys are stored flattened (flat_obs order)."""
 
-    def __init__(self, buffer_size, n_envs, obs_dim, act_dim, device):
+    def __init__(self, buffer_size, n_envs, obs_dim, act_dim, device, windows=False):
         self.size = max(buffer_size // n_envs, 1)
         self.n_envs = n_envs
         z = lambda *s: torch.zeros(*s, dtype=torch.float32, device=device)
@@ -180,8 +191,13 @@ class DictReplayBuffer:
         # rows filled so far, on the device: sample() draws indices from it without a host value,
         # so the captured learner step samples the buffer as it grows
         self.upper = torch.zeros((), dtype=torch.float32, device=device)
+        # sample_windows: which rows begin an episode, and the oldest row there is (on the device, as upper)
+        self.starts = torch.zeros(self.size, n_envs, dtype=torch.uint8, device=device) if windows else None
+        self.oldest = torch.zeros((), dtype=torch.int64, device=device)
 
-    def add(self, obs, next_obs, action, reward, done):
+    def add(self, obs, next_obs, action, reward, done, start=None):
+        if self.starts is not None:
+            self.starts[self.pos].copy_(start)
         self.obs[self.pos].copy_(obs)
         self.next_obs[self.pos].copy_(next_obs)
         self.actions[self.pos].copy_(action)
@@ -191,13 +207,31 @@ class DictReplayBuffer:
         if self.pos == self.size:
             self.full, self.pos = True, 0
         self.upper.fill_(float(self.size if self.full else self.pos))
+        if self.full:
+            self.oldest.fill_(self.pos)
+
+    def _draw(self, batch_size, generator):
+        u = torch.rand(2, batch_size, device=self.device, generator=generator)
+        return (torch.clamp((u[0] * self.upper).long(), max=self.size - 1),
+                torch.clamp((u[1] * self.n_envs).long(), max=self.n_envs - 1))
+
+    def sample_windows(self, batch_size, length, generator=None):
+        """``length`` steps that end in a uniform (row, env) pair, oldest first: observations and the actions taken
+        before them ([B, length, .], zero where an episode begins), starts [B, length] (where one begins, or where the
+        buffer does: earlier tokens of the window are not part of it), and the last step's transition as sample()'s."""
+        bi, ei = self._draw(batch_size, generator)
+        back = torch.arange(length - 1, -1, -1, device=self.device)
+        age = ((bi - self.oldest) % self.size)[:, None] - back          # rows since the oldest; below 0: not there
+        row, env = (bi[:, None] - back) % self.size, ei[:, None].expand(-1, length)
+        starts = (self.starts[row, env] != 0) | (age <= 0)
+        prev = self.actions[(row - 1) % self.size, env] * (~starts)[..., None]
+        return (self.obs[row, env], prev, starts, self.actions[bi, ei], self.next_obs[bi, ei], self.dones[bi, ei, None],
+                self.rewards[bi, ei, None])
 
     def sample(self, batch_size, generator=None):
         """Uniform (row, env) pairs over the filled rows: floor(U[0, 1) * upper), the row count read
         on the device (sb3 samples the same distribution with randint on the host's upper bound)."""
-        u = torch.rand(2, batch_size, device=self.device, generator=generator)
-        bi = torch.clamp((u[0] * self.upper).long(), max=self.size - 1)
-        ei = torch.clamp((u[1] * self.n_envs).long(), max=self.n_envs - 1)
+        bi, ei = self._draw(batch_size, generator)
         return (self.obs[bi, ei], self.actions[bi, ei], self.next_obs[bi, ei], self.dones[bi, ei, None],
                 self.rewards[bi, ei, None])
 
@@ -297,17 +331,28 @@ class TQC:
         self.obs_dim = sum(dims.values())
         self.rank = dist.get_rank() if _world() > 1 else 0
         torch.manual_seed(c.seed)             # same initial weights on every rank (broadcast below too)
-        self.actor = Actor(self.obs_dim, self.act_dim, c.net_arch).to(self.device)
-        self.critic = QuantileCritics(self.obs_dim, self.act_dim, c.net_arch, c.n_critics,
-                                      c.n_quantiles).to(self.device)
-        self.critic_target = QuantileCritics(self.obs_dim, self.act_dim, c.net_arch, c.n_critics,
-                                             c.n_quantiles).to(self.device)
+        if c.history < 0:
+            raise ValueError(f"history must not be negative (got {c.history})")
+        if c.history and self.device.type != "cuda":
+            raise ValueError("history: the sequence operators need a HIP device (there is no CPU path)")
+        in_dim = self.obs_dim + (c.history_dim if c.history else 0)
+        self.actor = Actor(in_dim, self.act_dim, c.net_arch).to(self.device)
+        self.critic = QuantileCritics(in_dim, self.act_dim, c.net_arch, c.n_critics, c.n_quantiles).to(self.device)
+        self.critic_target = QuantileCritics(in_dim, self.act_dim, c.net_arch, c.n_critics, c.n_quantiles).to(self.device)
+        self.encoder = self.encoder_target = None
+        if c.history:
+            from .history import HistoryEncoder
+            make = lambda: HistoryEncoder(self.obs_dim + self.act_dim, c.history_dim, c.history_layers).to(self.device)
+            self.encoder, self.encoder_target = make(), make()
         self.log_ent_coef = torch.full((1,), math.log(c.ent_coef_init), device=self.device, requires_grad=True)
         if _world() > 1:
-            for p in list(self.actor.parameters()) + list(self.critic.parameters()):
+            for p in list(self.actor.parameters()) + self._critic_params():
                 dist.broadcast(p.data, 0)
         self.critic_target.load_state_dict(self.critic.state_dict())
         self.critic_target.requires_grad_(False)
+        if self.encoder is not None:
+            self.encoder_target.load_state_dict(self.encoder.state_dict())
+            self.encoder_target.requires_grad_(False)
         self.target_entropy = -float(self.act_dim)
         # fused Adam with the learning rate as a device tensor (the linear schedule writes it in place,
         # so a captured step follows it); capturable: step counts on the device
@@ -315,7 +360,7 @@ class TQC:
         self._lr = torch.full((), c.learning_rate, dtype=torch.float32, device=self.device) if cuda else c.learning_rate
         kw = dict(lr=self._lr, fused=True, capturable=True) if cuda else dict(lr=c.learning_rate)
         self.actor_opt = torch.optim.Adam(self.actor.parameters(), **kw)
-        self.critic_opt = torch.optim.Adam(self.critic.parameters(), **kw)
+        self.critic_opt = torch.optim.Adam(self._critic_params(), **kw)
         self.ent_opt = torch.optim.Adam([self.log_ent_coef], **kw)
         self._graph = None          # the captured gradient step (TQC._capture)
         self._graph_out = None
@@ -326,7 +371,10 @@ class TQC:
         self._fctr = torch.zeros(2, dtype=torch.int64, device=self.device) if cuda else None
         self._eager_updates = 0     # steps run eagerly before the capture (allocator / optimiser state)
         self.vecnorm = VecNormalize(dims, self.device, c.clip_obs, c.norm_eps)
-        self.buffer = DictReplayBuffer(c.buffer_size, self.n_envs, self.obs_dim, self.act_dim, self.device)
+        self.buffer = DictReplayBuffer(c.buffer_size, self.n_envs, self.obs_dim, self.act_dim, self.device,
+                                       windows=bool(c.history))
+        self._mem = None                # the rollout's memory (TQC._recall): encoder state, previous action, starts
+        self._int8 = (None, -1)         # the encoder's 8-bit weights, and the update that they were taken after
         # per-rank sampling streams (exploration, replay indices); identical init weights
         self.gen = torch.Generator(device=self.device)
         self.gen.manual_seed(c.seed * 1000003 + self.rank + 1)
@@ -338,6 +386,10 @@ class TQC:
         self.ep_reward = torch.zeros(self.n_envs, device=self.device)
         self.stats = {"episodes": 0, "ep_reward_sum": 0.0, "success_sum": 0.0}
         self.logs = {}
+
+    def _critic_params(self):
+        """What the critics' loss trains: the critics, and the encoder of their history."""
+        return list(self.critic.parameters()) + (list(self.encoder.parameters()) if self.encoder is not None else [])
 
     # ------------------------------------------------------------------ schedule / optimisers
     def _progress_remaining(self):
@@ -379,12 +431,30 @@ class TQC:
     def _norm(self, raw):
         return flat_obs(self.vecnorm.normalize(raw))
 
+    def _memory(self, n):
+        """The memory of n envs at their episodes' start."""
+        return {"state": self.encoder.new_state(n), "act": torch.zeros(n, self.act_dim, device=self.device),
+                "start": torch.ones(n, dtype=torch.bool, device=self.device)}
+
+    @torch.no_grad()
+    def _recall(self, obs_norm, mem):
+        """The policy's input: the observation with its history's features, the memory advanced by this step
+        (the state carried over episodes' lengths and over updates of the weights, not recomputed)."""
+        if self.encoder is None:
+            return obs_norm
+        if self.cfg.rollout_int8 and self._int8[1] != self.n_updates:
+            self._int8 = (self.encoder.int8_weights(), self.n_updates)
+        x = torch.cat([obs_norm, mem["act"] * (~mem["start"])[:, None]], dim=1)
+        return torch.cat([obs_norm, self.encoder.step(x, mem["state"], reset=mem["start"], int8=self._int8[0])], dim=1)
+
     def reset(self):
         obs = self.env.reset()
         raw = {k: obs[k].clone() for k in OBS_KEYS}
         self.vecnorm.update(raw)
         self._last_raw = raw
         self._last_norm = self._norm(raw)
+        if self.encoder is not None:
+            self._mem = self._memory(self.n_envs)
 
     @torch.no_grad()
     def predict(self, obs_norm, deterministic=False):
@@ -393,10 +463,11 @@ class TQC:
     @torch.no_grad()
     def collect_step(self):
         """One vector step of every env (sb3 collect_rollouts with train_freq = 1 step)."""
+        seen = self._recall(self._last_norm, self._mem)
         if self.num_timesteps < self.cfg.learning_starts:
             act = torch.rand(self.n_envs, self.act_dim, device=self.device, generator=self.gen) * 2 - 1
         else:
-            act = self.predict(self._last_norm)
+            act = self.predict(seen)
         obs, reward, term, trunc, info = self.env.step(act)
         done = term | trunc
         new_raw = {k: obs[k] for k in OBS_KEYS}
@@ -405,7 +476,10 @@ class TQC:
             fin = {"observation": info["final_observation"], "achieved_goal": info["final_achieved_goal"],
                    "desired_goal": info["final_desired_goal"]}
             next_raw = {k: torch.where(done[:, None], fin[k], new_raw[k]) for k in OBS_KEYS}
-        self.buffer.add(flat_obs(self._last_raw), flat_obs(next_raw), act, reward, term.float())
+        self.buffer.add(flat_obs(self._last_raw), flat_obs(next_raw), act, reward, term.float(),
+                        None if self._mem is None else self._mem["start"])
+        if self._mem is not None:
+            self._mem["act"], self._mem["start"] = act.clone(), done.clone()
         self.vecnorm.update(new_raw)
         self._last_raw = {k: v.clone() for k, v in new_raw.items()}
         self._last_norm = self._norm(self._last_raw)
@@ -427,6 +501,23 @@ class TQC:
             return flat_obs(self.vecnorm.normalize(dict(zip(OBS_KEYS, parts))))
         return norm(o), a, norm(no), d, r
 
+    def _sample_history(self):
+        """_sample_norm with the history's features: (obs, act, next obs, next obs for the targets, done, reward).
+        One pass over the window and the step after it; gradients flow through obs alone."""
+        H = self.cfg.history
+        o, prev, starts, a, no, d, r = self.buffer.sample_windows(self.cfg.batch_size, H, self.gen)
+        def norm(x):
+            parts = torch.split(x.reshape(-1, self.obs_dim), [3, 3, 19], dim=1)
+            return flat_obs(self.vecnorm.normalize(dict(zip(OBS_KEYS, parts)))).view(x.shape)
+        o, no = norm(o), norm(no)
+        x = torch.cat([torch.cat([o, prev], dim=2), torch.cat([no, a], dim=1)[:, None]], dim=1)
+        starts = torch.cat([starts, torch.zeros_like(starts[:, :1])], dim=1)
+        f = self.encoder(x, starts)
+        with torch.no_grad():
+            nt = torch.cat([no, self.encoder_target(x, starts)[:, H]], dim=1)
+            nobs = torch.cat([no, f[:, H]], dim=1)
+        return torch.cat([o[:, H - 1], f[:, H - 1]], dim=1), a, nobs, nt, d, r
+
     def _update(self):
         """One gradient step (sb3-contrib tqc.py train() order) on device tensors, no host sync:
         entropy coefficient, critics, actor, Polyak target update.  Returns the logged values as
@@ -442,15 +533,19 @@ class TQC:
         rc = ra = None
         if record is not None:
             rc, ra = record.setdefault("critic", []), record.setdefault("actor", [])
-        obs, act, nobs, done, rew = self._sample_norm()
-        a_pi, lp = self.actor.action_log_prob(obs, self.gen)
+        if c.history:
+            obs, act, nobs, tobs, done, rew = self._sample_history()
+        else:
+            obs, act, nobs, done, rew = self._sample_norm()
+            tobs = nobs
+        a_pi, lp = self.actor.action_log_prob(obs.detach(), self.gen)
         lp = lp.reshape(-1, 1)
         ent_coef = torch.exp(self.log_ent_coef.detach())
         ent_loss = -(self.log_ent_coef * (lp + self.target_entropy).detach()).mean()
         self._step_opt(self.ent_opt, ent_loss, [self.log_ent_coef])
         with torch.no_grad():
             na, nlp = self.actor.action_log_prob(nobs, self.gen)
-            nq = self.critic_target(nobs, na)
+            nq = self.critic_target(tobs, na)
             keep = c.n_quantiles * c.n_critics - c.top_quantiles_to_drop_per_net * c.n_critics
             nq, _ = torch.sort(nq.reshape(c.batch_size, -1))
             nq = nq[:, :keep]
@@ -459,13 +554,15 @@ class TQC:
             tq = tq.unsqueeze(1)
         cq = self.critic(obs, act)
         critic_loss = quantile_huber_loss(cq, tq, sum_over_quantiles=False)
-        self._step_opt(self.critic_opt, critic_loss, list(self.critic.parameters()), rc)
-        qpi = self.critic(obs, a_pi).mean(dim=2).mean(dim=1, keepdim=True)
+        self._step_opt(self.critic_opt, critic_loss, self._critic_params(), rc)
+        qpi = self.critic(obs.detach(), a_pi).mean(dim=2).mean(dim=1, keepdim=True)
         actor_loss = (ent_coef * lp - qpi).mean()
         self._step_opt(self.actor_opt, actor_loss, list(self.actor.parameters()), ra)
         if (self.n_updates + 1) % c.target_update_interval == 0:
             with torch.no_grad():
-                tps, ps = list(self.critic_target.parameters()), list(self.critic.parameters())
+                tps, ps = list(self.critic_target.parameters()), self._critic_params()
+                if self.encoder is not None:
+                    tps += list(self.encoder_target.parameters())
                 torch._foreach_mul_(tps, 1 - c.tau)
                 torch._foreach_add_(tps, ps, alpha=c.tau)
         self.n_updates += 1
@@ -474,7 +571,7 @@ class TQC:
     # ------------------------------------------------------------------ the fused gradient step
     def _fused_ok(self):
         c = self.cfg
-        return (c.fused and self.device.type == "cuda" and tuple(c.net_arch) == (256, 256, 256)
+        return (c.fused and not c.history and self.device.type == "cuda" and tuple(c.net_arch) == (256, 256, 256)
                 and c.n_critics == 2 and c.n_quantiles == 25 and c.top_quantiles_to_drop_per_net == 2
                 and c.batch_size % 16 == 0 and self.obs_dim == 25 and self.act_dim == 7
                 and c.target_update_interval == 1)
@@ -726,7 +823,9 @@ class TQC:
 
     # ------------------------------------------------------------------ checkpoints
     def state_dict(self):
-        return {"actor": self.actor.state_dict(), "critic": self.critic.state_dict(),
+        mem = {} if self.encoder is None else {"encoder": self.encoder.state_dict(),
+                                               "encoder_target": self.encoder_target.state_dict()}
+        return {**mem, "actor": self.actor.state_dict(), "critic": self.critic.state_dict(),
                 "critic_target": self.critic_target.state_dict(), "log_ent_coef": self.log_ent_coef.detach(),
                 "actor_opt": self.actor_opt.state_dict(), "critic_opt": self.critic_opt.state_dict(),
                 "ent_opt": self.ent_opt.state_dict(), "vecnormalize": self.vecnorm.state_dict(),
@@ -737,6 +836,10 @@ class TQC:
         self.actor.load_state_dict(d["actor"])
         self.critic.load_state_dict(d["critic"])
         self.critic_target.load_state_dict(d["critic_target"])
+        if self.encoder is not None:
+            self.encoder.load_state_dict(d["encoder"])
+            self.encoder_target.load_state_dict(d["encoder_target"])
+            self._int8 = (None, -1)
         with torch.no_grad():
             self.log_ent_coef.copy_(d["log_ent_coef"])
         self.actor_opt.load_state_dict(d["actor_opt"])
@@ -775,9 +878,12 @@ class TQC:
         live = torch.ones(n, dtype=torch.bool, device=self.device)
         succ = torch.zeros(n, device=self.device)
         steps = 0
+        mem = None if self.encoder is None else self._memory(n)
         while bool(live[:n_episodes].any()):
-            a = self.actor(self._norm({k: obs[k] for k in OBS_KEYS}), deterministic=True)
+            a = self.actor(self._recall(self._norm({k: obs[k] for k in OBS_KEYS}), mem), deterministic=True)
             obs, r, term, trunc, info = eval_env.step(a)
+            if mem is not None:
+                mem["act"], mem["start"] = a.clone(), term | trunc
             ret += r * live
             done = (term | trunc) & live
             succ[done] = info["is_success"][done]

@@ -45,7 +45,14 @@ def main(argv=None):
     ap.add_argument("--gradient-steps", type=int, default=-1,
                     help="gradient steps per vector step (default -1: envs // 4, the reference's "
                          "one update per 4 transitions)")
+    ap.add_argument("--history", type=int, default=0,
+                    help="steps of history that the policy sees (TQCConfig.history; default 0: none)")
+    ap.add_argument("--history-dim", type=int, default=256, help="features of the history")
+    ap.add_argument("--history-layers", type=int, default=1)
+    ap.add_argument("--rollout-int8", action="store_true", help="the rollout's history encoder with 8-bit products")
     args = ap.parse_args(argv)
+    if args.rollout_int8 and not args.history:
+        ap.error("--rollout-int8 needs --history")
 
     world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = int(os.environ.get("RANK", "0"))
@@ -60,7 +67,8 @@ def main(argv=None):
     eval_env = BatchedFrankaShelfPNPEnv(args.eval_episodes, reward_type=reward_type, config=cfg,
                                         env_offset=10 ** 8 + rank * args.eval_episodes)
     gsteps = args.gradient_steps if args.gradient_steps > 0 else max(1, args.envs // 4)
-    model = TQC(env, TQCConfig(seed=args.seed, gradient_steps=gsteps))
+    model = TQC(env, TQCConfig(seed=args.seed, gradient_steps=gsteps, history=args.history, history_dim=args.history_dim,
+                               history_layers=args.history_layers, rollout_int8=args.rollout_int8))
     if rank == 0:
         print(f"==> Training on {env_id} | device=cuda:{local} | {args.envs} envs x {world} GPU(s) | "
               f"{gsteps} gradient steps per vector step", flush=True)
