@@ -79,9 +79,16 @@ __device__ __forceinline__ void norm_fwd_row(const NormArgs& a, int64_t row, flo
       for (int k = 0; k < V; k++) v[k] = to_f(from_f<R>(v[k] + b[k]));
     }
   };
+  // short rows take their weights along with the row, not after its sum
+  constexpr bool EARLY = NV == 1;
+  float early[V];
+  if (EARLY && a.w && lane * V < a.dim) load_f<V>(a.w + lane * V, early);
   auto scaled = [&](int i, float rho, float (&v)[V]) {
     float w[V];
-    if (a.w) load_f<V>(a.w + i, w);
+    if (EARLY)
+#pragma unroll
+      for (int k = 0; k < V; k++) w[k] = early[k];
+    else if (a.w) load_f<V>(a.w + i, w);
 #pragma unroll
     for (int k = 0; k < V; k++) v[k] = a.w ? v[k] * rho * w[k] : v[k] * rho;
   };

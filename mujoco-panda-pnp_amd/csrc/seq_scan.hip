@@ -200,6 +200,19 @@ template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__
   const uint32_t ou = (uint32_t)(lt * a.ut + lc) * sizeof(T), od = (uint32_t)(lt * a.dt + lc) * sizeof(T),
                  oz = (uint32_t)(lt * a.zt + lc) * sizeof(T), oo = (uint32_t)(lt * a.dim + lc) * sizeof(T);
 
+  Raw<T, E> nu, nd, nz, cu, cz;
+  constexpr int NBC = STATE ? TT * S : 2 * TT * S;                  // packs of 4 states a tile
+  constexpr int PER = (NBC + NT - 1) / NT;
+  float4 nbc[PER];
+  uint32_t ns = 0;
+  auto fetch = [&](int64_t t) {
+    const int l = t + lt < t1 ? left : 0;
+    ns = load_start<TT>(a, w.b, t, t1);
+    load_channels<E, WIDE>(at<T>(a.u, w.b * a.ub + t * a.ut + w.ch, ou), l, nu);
+    load_channels<E, WIDE>(at<T>(a.delta, w.b * a.db + t * a.dt + w.ch, od), l, nd);
+    if (z) load_channels<E, WIDE>(at<T>(a.z, w.b * a.zb + t * a.zt + w.ch, oz), l, nz);
+    load_bc<T, S, TT, NBC, WIDE>(a, w.b, w.g, t, t1, nbc);
+  };
   float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f}, dsum = 0.f;
   const int64_t ch = w.ch + (on ? cl : 0);
   load_state4(a.A + ch * a.N, 4 * ng, a.N, A2);
@@ -215,19 +228,6 @@ template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__
     Dv[i] = !STATE && a.D && i < left ? a.D[w.ch + lc + i] : 0.f;
     bias[i] = a.bias && i < left ? a.bias[w.ch + lc + i] : 0.f;
   }
-  Raw<T, E> nu, nd, nz, cu, cz;
-  constexpr int NBC = STATE ? TT * S : 2 * TT * S;                  // packs of 4 states a tile
-  constexpr int PER = (NBC + NT - 1) / NT;
-  float4 nbc[PER];
-  uint32_t ns = 0;
-  auto fetch = [&](int64_t t) {
-    const int l = t + lt < t1 ? left : 0;
-    ns = load_start<TT>(a, w.b, t, t1);
-    load_channels<E, WIDE>(at<T>(a.u, w.b * a.ub + t * a.ut + w.ch, ou), l, nu);
-    load_channels<E, WIDE>(at<T>(a.delta, w.b * a.db + t * a.dt + w.ch, od), l, nd);
-    if (z) load_channels<E, WIDE>(at<T>(a.z, w.b * a.zb + t * a.zt + w.ch, oz), l, nz);
-    load_bc<T, S, TT, NBC, WIDE>(a, w.b, w.g, t, t1, nbc);
-  };
   if (t0 < t1) fetch(t0);
   for (int64_t t = t0; t < t1; t += TT) {
     const bool mine = t + lt < t1;
@@ -249,13 +249,16 @@ template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__
     const uint32_t bits = start_bits(ns);
     __syncthreads();
     if (t + TT < t1) fetch(t + TT);
-    auto tokens = [&](auto starts, int p) {
-      float q[G];
+    // ANY: some of the n tokens start a sequence, or there are fewer than TR
+    auto tokens = [&](auto any, int p, int n) {
+      constexpr bool ANY = decltype(any)::value;
+      float q[G] = {};
 #pragma unroll
       for (int k = 0; k < TR; k++) {
+        if (ANY && k >= n) break;
         const float2 d = reinterpret_cast<const float2*>(dd[p + k])[mine2];
         const float4 b = sB[p + k][ng];
-        if (starts.value && (bits >> (p + k) & 1)) {
+        if (ANY && (bits >> (p + k) & 1)) {
           h[0] = h[1] = h[2] = h[3] = 0.f;
           if (STATE) dsum = __builtin_nanf("");
         }
@@ -268,19 +271,31 @@ template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__
         } else {
           const float4 c = sC[p + k][ng];
           q[k % G] = c.x * h[0] + c.y * h[1] + c.z * h[2] + c.w * h[3];
-          if (k % G == G - 1) {   // (dt of these tokens has been read by every lane of the channel)
+          if (k % G == G - 1 || (ANY && k == n - 1)) {   // (dt of these tokens has been read by every lane of the channel)
             const float y = token_sums<S>(q);
-            if (G == S || ng < G) reinterpret_cast<float2*>(dd[p + k - (G - 1) + ng])[mine2].x = y;
+            if (G == S || ng < G) reinterpret_cast<float2*>(dd[p + k / G * G + ng])[mine2].x = y;
           }
         }
       }
     };
-#pragma unroll 1
-    for (int p = 0; p < TT; p += TR) {
-      if (!STATE && a.ckpt && on && t + p < t1)
+    auto keep = [&](int p) {
+      if (!STATE && a.ckpt && on)
         *reinterpret_cast<float4*>(a.ckpt + ((w.b * a.nck + (t + p) / TR) * a.dim + ch) * NP + 4 * ng) = float4{h[0], h[1], h[2], h[3]};
-      if (bits) tokens(std::true_type(), p);
-      else tokens(std::false_type(), p);
+    };
+    if (!bits && t + TT <= t1) {
+#pragma unroll 1
+      for (int p = 0; p < TT; p += TR) {
+        keep(p);
+        tokens(std::false_type(), p, TR);
+      }
+    } else {
+      const int held = t1 - t < TT ? (int)(t1 - t) : TT;
+#pragma unroll 1
+      for (int p = 0; p < held; p += TR) {
+        keep(p);
+        if (bits >> p & ((1u << TR) - 1) || p + TR > held) tokens(std::true_type(), p, held - p);
+        else tokens(std::false_type(), p, TR);
+      }
     }
     __syncthreads();
     if (!STATE && mine) {
@@ -321,17 +336,25 @@ __global__ __launch_bounds__(NT) void scan_chain_kernel(ScanArgs a, const float*
   const int d = (int)(bd - b * a.dim);
   const float A2 = n < a.N ? a.A[(int64_t)d * a.N + n] * SEQ_LOG2E : 0.f;
   float h = first && n < a.N ? first[bd * a.N + n] : 0.f;
-  for (int i = 0; i < a.nch; i++) {
-    const int64_t row = b * a.nch + (back ? a.nch - 1 - i : i);
-    float* p = a.hin + (row * a.dim + d) * NP + n;
-    if (i == a.nch - 1) {   // (nothing follows it: its own state was not asked for)
-      *p = h;
-      return;
+  float* p = a.hin + ((b * a.nch + (back ? a.nch - 1 : 0)) * a.dim + d) * NP + n;
+  const float* q = a.dsum + (b * a.nch + (back ? a.nch - 1 : 0)) * a.dim + d;
+  const int64_t stride = back ? -(int64_t)a.dim : a.dim;
+  constexpr int C = 8;   // chunks whose states are loaded together
+  for (int i = 0; i < a.nch; i += C, p += C * stride * NP, q += C * stride) {
+    float own[C], s[C];
+#pragma unroll
+    for (int k = 0; k < C; k++)
+      if (i + k < a.nch - 1) {   // (nothing follows the last one: its own state was not asked for)
+        own[k] = p[k * stride * NP];
+        s[k] = q[k * stride];
+      }
+#pragma unroll
+    for (int k = 0; k < C; k++) {
+      if (i + k >= a.nch) return;
+      p[k * stride * NP] = h;
+      // a start in the chunk lets nothing through
+      if (i + k < a.nch - 1) h = s[k] == s[k] ? own[k] + exp2_f(A2 * s[k]) * h : own[k];
     }
-    const float own = *p, s = a.dsum[row * a.dim + d];
-    *p = h;
-    // a start in the chunk lets nothing through
-    h = s == s ? own + exp2_f(A2 * s) * h : own;
   }
 }
 
@@ -437,9 +460,11 @@ template <typename T, int S, bool WIDE> __global__ __launch_bounds__(NT) void sc
     const uint32_t bits = start_bits(ns);
     __syncthreads();
     if (t > t0) fetch(t - TT);
-    auto tokens = [&](auto starts, int p) {
+    auto tokens = [&](auto any, int p, int n) {
+      constexpr bool ANY = decltype(any)::value;
 #pragma unroll
       for (int k = TR - 1; k >= 0; k--) {
+        if (ANY && k >= n) continue;
         const float2 d = reinterpret_cast<const float2*>(dd[p + k])[mine2];
         const float4 c = sC[p + k][ng];
         g[0] = exp2_f(d.x * A2[0]) * (g[0] + c.x * d.y);
@@ -447,16 +472,19 @@ template <typename T, int S, bool WIDE> __global__ __launch_bounds__(NT) void sc
         g[2] = exp2_f(d.x * A2[2]) * (g[2] + c.z * d.y);
         g[3] = exp2_f(d.x * A2[3]) * (g[3] + c.w * d.y);
         dsum += d.x;
-        if (starts.value && (bits >> (p + k) & 1)) {
+        if (ANY && (bits >> (p + k) & 1)) {
           g[0] = g[1] = g[2] = g[3] = 0.f;
           dsum = __builtin_nanf("");
         }
       }
     };
+    if (!bits && t + TT <= t1) {
 #pragma unroll 1
-    for (int p = TT - TR; p >= 0; p -= TR) {
-      if (bits) tokens(std::true_type(), p);
-      else tokens(std::false_type(), p);
+      for (int p = TT - TR; p >= 0; p -= TR) tokens(std::false_type(), p, TR);
+    } else {
+      const int held = t1 - t < TT ? (int)(t1 - t) : TT;
+#pragma unroll 1
+      for (int p = (held - 1) / TR * TR; p >= 0; p -= TR) tokens(std::true_type(), p, held - p);
     }
     __syncthreads();
   }
@@ -485,19 +513,6 @@ template <typename T, int S, bool WIDE> __global__ __launch_bounds__(NT, 2) void
                  oz = (uint32_t)(lt * f.zt + lc) * sizeof(T), oy = (uint32_t)(lt * a.ot + lc) * sizeof(T),
                  oo = (uint32_t)(lt * f.dim + lc) * sizeof(T), ok = (uint32_t)(cl * NP + 4 * ng) * 4u;
 
-  float A[4], A2[4], dA[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {0.f, 0.f, 0.f, 0.f};
-  const int64_t ch = w.ch + (on ? cl : 0);
-  load_state4(f.A + ch * f.N, 4 * ng, f.N, A);
-#pragma unroll
-  for (int i = 0; i < 4; i++) A2[i] = A[i] * SEQ_LOG2E;
-  if (f.nch > 1) load_state4(f.hin + (w.row * f.dim + ch) * NP, 4 * ng, NP, g);
-  else if (a.dlast) load_state4(a.dlast + (w.b * f.dim + ch) * f.N, 4 * ng, f.N, g);
-  float Dv[E], bias[E], dD[E] = {}, dbias[E] = {};
-#pragma unroll
-  for (int i = 0; i < E; i++) {
-    Dv[i] = f.D && i < left ? f.D[w.ch + lc + i] : 0.f;
-    bias[i] = f.bias && i < left ? f.bias[w.ch + lc + i] : 0.f;
-  }
   constexpr int NBC = 2 * TT * S, PER = (NBC + NT - 1) / NT;
   Raw<T, E> nu, nd, nz, no, cu, cd, cz, co;
   float4 nbc[PER];
@@ -512,7 +527,21 @@ template <typename T, int S, bool WIDE> __global__ __launch_bounds__(NT, 2) void
     load_bc<T, S, TT, NBC, WIDE>(f, w.b, w.g, t, t1, nbc);
   };
   const int64_t tiles = (t1 - t0 + TT - 1) / TT;
-  if (tiles > 0) fetch(t0 + (tiles - 1) * TT);
+  if (tiles > 0) fetch(t0 + (tiles - 1) * TT);   // (under way while the rest is loaded)
+
+  float A[4], A2[4], dA[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {0.f, 0.f, 0.f, 0.f};
+  const int64_t ch = w.ch + (on ? cl : 0);
+  load_state4(f.A + ch * f.N, 4 * ng, f.N, A);
+#pragma unroll
+  for (int i = 0; i < 4; i++) A2[i] = A[i] * SEQ_LOG2E;
+  if (f.nch > 1) load_state4(f.hin + (w.row * f.dim + ch) * NP, 4 * ng, NP, g);
+  else if (a.dlast) load_state4(a.dlast + (w.b * f.dim + ch) * f.N, 4 * ng, f.N, g);
+  float Dv[E], bias[E], dD[E] = {}, dbias[E] = {};
+#pragma unroll
+  for (int i = 0; i < E; i++) {
+    Dv[i] = f.D && i < left ? f.D[w.ch + lc + i] : 0.f;
+    bias[i] = f.bias && i < left ? f.bias[w.ch + lc + i] : 0.f;
+  }
   for (int64_t t = t0 + (tiles - 1) * TT; t >= t0; t -= TT) {
     const bool mine = t + lt < t1;
 #pragma unroll
@@ -542,19 +571,21 @@ template <typename T, int S, bool WIDE> __global__ __launch_bounds__(NT, 2) void
     const uint32_t bits = start_bits(ns);
     __syncthreads();
     if (t > t0) fetch(t - TT);
-    // the inner tile at p from the state h0: its states and decays forward, kept, then the adjoint back.
-    // starts: a start's decay is 0 whatever the state (0 times infinity is NaN)
-    auto tokens = [&](auto starts, int p, const float4 h0) {
-      constexpr bool ST = decltype(starts)::value;
+    // The inner tile at p from the state h0: its states and decays forward, kept, then the adjoint back.  ANY: some
+    // of the n tokens start a sequence, or there are fewer than TR.  A start's decay is 0 whatever the state (0 times
+    // infinity is NaN).
+    auto tokens = [&](auto any, int p, int n, const float4 h0) {
+      constexpr bool ANY = decltype(any)::value;
       const uint32_t marks = bits >> p;
-      float e[TR][4], h[TR + 1][4], q[G];
+      float e[TR][4], h[TR + 1][4], q[G] = {};
       h[0][0] = h0.x; h[0][1] = h0.y; h[0][2] = h0.z; h[0][3] = h0.w;
 #pragma unroll
       for (int k = 0; k < TR; k++) {
+        if (ANY && k >= n) break;
         const float4 d = dd[p + k][mine4];
         const float4 b = sB[p + k][ng], c = sC[p + k][ng];
         const float bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
-        const bool st = ST && (marks >> k & 1);
+        const bool st = ANY && (marks >> k & 1);
         float y = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -564,20 +595,21 @@ template <typename T, int S, bool WIDE> __global__ __launch_bounds__(NT, 2) void
           y += cv[i] * h[k + 1][i];
         }
         q[k % G] = y;
-        if (k % G == G - 1) {
+        if (k % G == G - 1 || (ANY && k == n - 1)) {
           y = token_sums<S>(q);
-          if (G == S || ng < G) yb[p + k - (G - 1) + ng][cl] = y;
+          if (G == S || ng < G) yb[p + k / G * G + ng][cl] = y;
         }
       }
       // the tile is read again rather than held, 12 registers a token (the compiler must not see that it is the same)
       asm volatile("" : "+s"(p));
-      float q1[G], q2[G];
+      float q1[G] = {}, q2[G] = {};
 #pragma unroll
       for (int k = TR - 1; k >= 0; k--) {
+        if (ANY && k >= n) continue;
         const float4 d = dd[p + k][mine4];
         const float4 b = sB[p + k][ng], c = sC[p + k][ng];
         const float bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
-        const bool st = ST && (marks >> k & 1);
+        const bool st = ANY && (marks >> k & 1);
         float s1 = 0.f, s2 = 0.f, v[8];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -609,10 +641,12 @@ template <typename T, int S, bool WIDE> __global__ __launch_bounds__(NT, 2) void
         }
       }
     };
+    const int held = t1 - t < TT ? (int)(t1 - t) : TT;
 #pragma unroll
     for (int i = TT / TR - 1; i >= 0; i--) {
-      if (bits) tokens(std::true_type(), i * TR, hc[i]);
-      else tokens(std::false_type(), i * TR, hc[i]);
+      if (i * TR >= held) continue;
+      if (bits >> (i * TR) & ((1u << TR) - 1) || i * TR + TR > held) tokens(std::true_type(), i * TR, held - i * TR, hc[i]);
+      else tokens(std::false_type(), i * TR, TR, hc[i]);
     }
     __syncthreads();
     if (mine) {
