@@ -744,19 +744,28 @@ __global__ __launch_bounds__(1024) void scan_sums_kernel(const float* part, int6
   else if (dbias) dbias[c - na - dim] = s;
 }
 
-// one token: a lane holds 4 states of a channel
-template <typename T, int S, bool W4> __global__ __launch_bounds__(NT) void scan_step_kernel(ScanArgs a) {
-  const int64_t n = a.B * a.dim * S;
-  for (int64_t base = (int64_t)blockIdx.x * NT; base < n; base += (int64_t)gridDim.x * NT) {
-    const int64_t id = base + threadIdx.x, bd = id < n ? id / S : 0;
-    const int ng = threadIdx.x % S;
-    const int64_t b = bd / a.dim;
-    const int d = (int)(bd - b * a.dim);
-    const bool on = id < n;
+// One token: a lane holds 4 states of a channel, a workgroup NT / S channels of one sequence (so that the
+// sequence is a scalar).  Bound by the states' way from and to memory.  STREAM: states that outgrow the 256 MB
+// of cache before HBM go past the caches: at 8192 x 512 x 16 (268 MB) 98 against 102 us, 113 against 127 us with
+// the rest of a step's inputs; where they fit it is the other way (134 MB: 51 against 45 us).
+template <typename T, int S, bool W4, bool STREAM> __global__ __launch_bounds__(NT) void scan_step_kernel(ScanArgs a) {
+  typedef float V4 __attribute__((ext_vector_type(4)));
+  const int ng = threadIdx.x % S;
+  const int64_t n = a.B * a.tiles;
+  for (int64_t at = blockIdx.x; at < n; at += gridDim.x) {
+    const int64_t b = (uint64_t)at < (1ull << 32) ? (uint32_t)at / (uint32_t)a.tiles : at / a.tiles;
+    const int d0 = (int)(at - b * a.tiles) * (NT / S) + threadIdx.x / S;
+    const bool on = d0 < a.dim;
+    const int d = on ? d0 : 0;
+    const int64_t bd = b * a.dim + d;
     float h[4] = {0.f, 0.f, 0.f, 0.f}, A2[4];
     const float* hp = a.state ? a.state + bd * a.N + 4 * ng : nullptr;
     if (W4) {
-      if (hp) load_f<4>(hp, h);
+      if (hp) {
+        const V4 v = STREAM ? __builtin_nontemporal_load((const V4*)hp) : *(const V4*)hp;
+#pragma unroll
+        for (int i = 0; i < 4; i++) h[i] = v[i];
+      }
       load_f<4>(a.A + (int64_t)d * a.N + 4 * ng, A2);
     } else {
       if (hp) load_state4(hp - 4 * ng, 4 * ng, a.N, h);
@@ -779,8 +788,11 @@ template <typename T, int S, bool W4> __global__ __launch_bounds__(NT) void scan
     }
     y = group_sum<S>(y);
     if (!on) continue;
-    if (W4) store_f<4>(a.last + bd * a.N + 4 * ng, h);
-    else
+    if (W4) {
+      const V4 v = {h[0], h[1], h[2], h[3]};
+      if (STREAM) __builtin_nontemporal_store(v, (V4*)(a.last + bd * a.N + 4 * ng));
+      else *(V4*)(a.last + bd * a.N + 4 * ng) = v;
+    } else
 #pragma unroll
       for (int i = 0; i < 4; i++)
         if (4 * ng + i < a.N) a.last[bd * a.N + 4 * ng + i] = h[i];
@@ -913,10 +925,13 @@ template <typename T, int S> int32_t run_scan_bwd(ScanBwdArgs a, int64_t blocks,
 
 template <typename T, int S> int32_t run_step(ScanArgs a, hipStream_t st) {
   const bool w4 = a.N == 4 * S && bc_even(a, sizeof(T)) && aligned_to(a.A, 16) && aligned_to(a.last, 16) && (!a.state || aligned_to(a.state, 16));
-  const int64_t n = ceil_div(a.B * a.dim * S, NT);
+  a.tiles = (int)ceil_div(a.dim, NT / S);
+  const int64_t n = a.B * a.tiles;
   const unsigned grid = (unsigned)(n < (1 << 22) ? n : (1 << 22));
-  if (w4) hipLaunchKernelGGL((scan_step_kernel<T, S, true>), dim3(grid), dim3(NT), 0, st, a);
-  else hipLaunchKernelGGL((scan_step_kernel<T, S, false>), dim3(grid), dim3(NT), 0, st, a);
+  const bool stream = a.B * a.dim * a.N >= 50 * 1000 * 1000;   // 200 MB of states
+  if (w4 && stream) hipLaunchKernelGGL((scan_step_kernel<T, S, true, true>), dim3(grid), dim3(NT), 0, st, a);
+  else if (w4) hipLaunchKernelGGL((scan_step_kernel<T, S, true, false>), dim3(grid), dim3(NT), 0, st, a);
+  else hipLaunchKernelGGL((scan_step_kernel<T, S, false, false>), dim3(grid), dim3(NT), 0, st, a);
   return pnp_check_launch("scan_step_kernel");
 }
 

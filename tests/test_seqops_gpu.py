@@ -410,6 +410,21 @@ def test_scan_step(S, dtype, B, D, N, G):
     P.close(g["state"], rl, el, 1, "state")
 
 
+def test_scan_step_of_more_states_than_the_cache_holds(S):
+    """The way past the caches gives the bits of the way through them."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    B, D, N = 6272, 512, 16
+    rnd = lambda *s: torch.randn(*s, device="cuda", generator=g)   # noqa: E731
+    u, dl, z, Bm, Cm, A, h = rnd(B, D), rnd(B, D), rnd(B, D), rnd(B, N), rnd(B, N), -rnd(D, N).abs(), rnd(B, D, N)
+    assert h.numel() >= 50 * 1000 * 1000
+    part, outs = [h[k:k + 448].clone() for k in range(0, B, 448)], []
+    whole = S.selective_scan_step(u, h, dl, A, Bm, Cm, z=z)
+    for i, p in enumerate(part):
+        k = slice(448 * i, 448 * i + 448)
+        outs.append(S.selective_scan_step(u[k], p, dl[k], A, Bm[k], Cm[k], z=z[k]))
+    assert torch.equal(whole, torch.cat(outs)) and torch.equal(h, torch.cat(part))
+
+
 def test_scan_empty(S):
     d = Draw(2)
     v = {k: dev(t, k != "starts") for k, t in scan_inputs(d, 2, 4, 8, 4, 1, torch.float32).items()}
