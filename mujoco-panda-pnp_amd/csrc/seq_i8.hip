@@ -175,9 +175,9 @@ __global__ __launch_bounds__(64 * WGM* WGN, 2) void i8_tile_kernel(I8Args a) {
 #pragma unroll
     for (int s = 0; s < ST - 1; s++) fetch(s);
     for (int s = 0; s < nk; s++) {
-      // this wave's loads of stage s have arrived
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 2) * (LW + LQ)) : "memory");
-      __builtin_amdgcn_s_barrier();   // everybody's have, and everybody has read stage s - 1
+      // this wave's loads of stage s have arrived, and what it read of stage s - 1 is in registers
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((ST - 2) * (LW + LQ)) : "memory");
+      __builtin_amdgcn_s_barrier();   // everybody's have and is: the buffer of stage s - 1 is free
       fetch(s + ST - 1);
       product(s % ST);
     }

@@ -352,8 +352,12 @@ __global__ __launch_bounds__(NT) void scan_chain_kernel(ScanArgs a, const float*
     for (int k = 0; k < C; k++) {
       if (i + k >= a.nch) return;
       p[k * stride * NP] = h;
-      // a start in the chunk lets nothing through
-      if (i + k < a.nch - 1) h = s[k] == s[k] ? own[k] + exp2_f(A2 * s[k]) * h : own[k];
+      // a start in the chunk lets nothing through, and a zero nothing of a growing state (A > 0) whose factor
+      // outgrows fp32; a factor that does on its way to a product that does not: in four parts
+      if (i + k < a.nch - 1) {
+        const float e = exp2_f(0.25f * A2 * s[k]);
+        h = s[k] == s[k] && h != 0.f ? own[k] + e * (e * (e * (e * h))) : own[k];
+      }
     }
   }
 }
@@ -1030,6 +1034,10 @@ extern "C" int32_t pnp_selective_scan_bwd(const pnp_scan_bwd_desc* d, void* stre
   const pnp_scan_desc& f = d->f;
   const Plan p = plan(&f);
   if (const int32_t rc = scan_check(&f, p, fn)) return rc;
+  if ((int64_t)f.dim * (f.N + 2) >= ((int64_t)1 << 28)) {
+    pnp_set_error("%s: too many channels for one launch", fn);
+    return PNP_ERR_ARG;
+  }
   if (!d->dA || (f.B && f.L && (!f.ckpt || !d->dout || !d->du || !d->ddelta || !d->dB || !d->dC || !f.z != !d->dz))) {
     pnp_set_error("%s: null buffer", fn);
     return PNP_ERR_ARG;

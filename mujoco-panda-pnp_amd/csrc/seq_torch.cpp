@@ -78,16 +78,24 @@ void activation(const Tensor& t, const char* name, const Tensor* like = nullptr)
 void dims(const Tensor& t, const char* name, int64_t n) {
   TORCH_CHECK_VALUE(t.dim() == n, name, ": shape ", t.sizes(), ", expected ", n, " dimensions");
 }
+// what the entry points hold in 32 bits
+void channels(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.dim() >= 1 && t.size(-1) > 0 && t.size(-1) <= (1 << 24), name, ": shape ", t.sizes(),
+                    ", expected a last dimension from 1 to ", 1 << 24);
+}
 void shaped(const Tensor& t, const char* name, at::IntArrayRef want) {
   TORCH_CHECK_VALUE(t.sizes() == want, name, ": shape ", t.sizes(), ", expected ", want);
 }
+// values as they lie in memory (not a view that stands for their negative)
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+Tensor whole(const Tensor& t) { return plain(t).contiguous(); }
 // a parameter, used in fp32 and contiguous (a differentiable cast: its gradient comes back in its own type)
 Tensor parameter(const MaybeTensor& t, const char* name, at::IntArrayRef want, const Tensor& like) {
   if (!t || !t->defined()) return Tensor();
   TORCH_CHECK_TYPE(at::isFloatingType(t->scalar_type()), name, " must be a floating tensor");
   same_device(*t, name, like);
   shaped(*t, name, want);
-  return t->to(at::kFloat).contiguous();
+  return whole(t->to(at::kFloat));
 }
 Tensor required(const MaybeTensor& t, const char* name, at::IntArrayRef want, const Tensor& like) {
   TORCH_CHECK_TYPE(t && t->defined(), name, " must be a floating tensor");
@@ -102,7 +110,18 @@ Tensor marks(const MaybeTensor& t, const char* name, at::IntArrayRef want, const
   return t->contiguous();
 }
 // a contiguous last dimension
-Tensor lines(const Tensor& t) { return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+Tensor lines(const Tensor& t_) {
+  const Tensor t = plain(t_);
+  return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+// a state that a call advances in place, which autograd has to hear of as of torch's own in-place calls: a graph
+// that holds the state as it was refuses to go back through it
+void in_place(const Tensor& state) {
+  TORCH_CHECK_VALUE(state.is_contiguous() && !state.is_neg(), "state must be contiguous: it is advanced in place");
+}
+void advanced(const Tensor& state) {
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+}
 
 // autograd nodes take what may be missing as an optional (an undefined tensor among their inputs is an error)
 MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
@@ -226,7 +245,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
 struct NormIn { Tensor w, r; };
 NormIn norm_in(const Tensor& x, const MaybeTensor& w, const MaybeTensor& r, double eps) {
   activation(x, "x");
-  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "x: shape ", x.sizes(), ", expected [..., dim] with dim > 0");
+  channels(x, "x");
   TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative (got ", eps, ")");
   NormIn o;
   o.w = required(w, "weight", {x.size(-1)}, x);
@@ -284,7 +303,7 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_q8(const Tensor& x, const MaybeT
 std::tuple<Tensor, Tensor> quantize_rows(const Tensor& x) {
   serving("quantize_rows", x);
   activation(x, "x");
-  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "x: shape ", x.sizes(), ", expected [..., dim] with dim > 0");
+  channels(x, "x");
   const Tensor x2 = rows_of(x);
   const Q8 o = q8_out(x2);
   CALL(quantize_rows, x, cptr(x2), x2.stride(0), code_of(x.scalar_type()), x2.size(0), (int32_t)x2.size(1), (int8_t*)mptr(o.q), o.q.stride(0),
@@ -360,7 +379,7 @@ struct ConvFn : torch::autograd::Function<ConvFn> {
     const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &starts = saved[3], &state = saved[4];
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(6);
     const Tensor dy = grads[0].defined() ? lines(grads[0]) : at::zeros(x.sizes(), x.options());
-    const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const Tensor dlast = grads[1].defined() ? whole(grads[1]) : Tensor();
     const int64_t flags = ctx->saved_data["flags"].toInt();
     pnp_conv_bwd_desc d{};
     d.f = conv_desc(x, w, b, flags & 1, starts, state);
@@ -394,7 +413,7 @@ std::tuple<Tensor, Tensor> causal_conv(const Tensor& x_, const Tensor& weight, c
                                        const MaybeTensor& starts_, const MaybeTensor& state_) {
   activation(x_, "x");
   dims(x_, "x", 3);
-  TORCH_CHECK_VALUE(x_.size(2) > 0, "x: no channels");
+  channels(x_, "x");
   const bool silu = is_silu(act);
   const Tensor w = conv_weight(weight, x_.size(2), x_), b = parameter(bias, "bias", {x_.size(2)}, x_);
   const Tensor starts = marks(starts_, "starts", x_.sizes().slice(0, 2), x_);
@@ -402,7 +421,7 @@ std::tuple<Tensor, Tensor> causal_conv(const Tensor& x_, const Tensor& weight, c
   if (state_ && state_->defined()) {
     activation(*state_, "state", &x_);
     shaped(*state_, "state", {x_.size(0), w.size(1) - 1, x_.size(2)});
-    state = state_->contiguous();
+    state = whole(*state_);
   }
   const Tensor x = lines(x_);
   if (!training(x, w, b, state)) return conv_run(x, w, b, silu, starts, state);
@@ -415,15 +434,16 @@ Tensor causal_conv_step(const Tensor& x_, const Tensor& state, const Tensor& wei
   serving("causal_conv_step", x_, state, weight, bias);
   activation(x_, "x");
   dims(x_, "x", 2);
-  TORCH_CHECK_VALUE(x_.size(1) > 0, "x: no channels");
+  channels(x_, "x");
   const bool silu = is_silu(act);
   const Tensor w = conv_weight(weight, x_.size(1), x_), b = parameter(bias, "bias", {x_.size(1)}, x_);
   activation(state, "state", &x_);
   shaped(state, "state", {x_.size(0), w.size(1) - 1, x_.size(1)});
-  TORCH_CHECK_VALUE(state.is_contiguous(), "state must be contiguous: it is advanced in place");
+  in_place(state);
   const Tensor reset = marks(reset_, "reset", x_.sizes().slice(0, 1), x_), x = lines(x_), y = fresh(x.sizes(), x.scalar_type(), x);
   CALL(causal_conv_step, x, cptr(x), x.stride(0), mptr(state), cfloat(w), cfloat(b), cbyte(reset), x.size(0), (int32_t)x.size(1),
        (int32_t)w.size(1), code_of(x.scalar_type()), (int32_t)silu, mptr(y));
+  advanced(state);
   return y;
 }
 
@@ -431,7 +451,8 @@ Tensor causal_conv_step(const Tensor& x_, const Tensor& state, const Tensor& wei
 struct ScanIn { Tensor u, delta, A, B, C, D, z, bias; };
 
 // [..., N] or [..., groups, N] with what follows the leading dimensions contiguous
-Tensor packed_groups(const Tensor& t, int64_t lead) {
+Tensor packed_groups(const Tensor& t_, int64_t lead) {
+  const Tensor t = plain(t_);
   const bool ok = (t.size(-1) == 1 || t.stride(-1) == 1) && (t.dim() == lead + 1 || t.size(-2) == 1 || t.stride(-2) == t.size(-1));
   return ok ? t : t.contiguous();
 }
@@ -447,7 +468,7 @@ ScanIn scan_in(const Tensor& u, const Tensor& delta, const Tensor& A, const Tens
   activation(u, "u");
   dims(u, "u", lead + 1);
   const int64_t dim = u.size(-1);
-  TORCH_CHECK_VALUE(dim > 0, "u: no channels");
+  channels(u, "u");
   activation(delta, "delta", &u);
   shaped(delta, "delta", u.sizes());
   if (z && z->defined()) {
@@ -521,7 +542,7 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
     const Tensor &starts = s[8], &state = s[9], &ckpt = s[10], &u = v.u;
     const ScalarType t = u.scalar_type();
     const Tensor dout = grads[0].defined() ? near(lines(grads[0]), 2) : at::zeros(u.sizes(), u.options());
-    const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const Tensor dlast = grads[1].defined() ? whole(grads[1]) : Tensor();
     pnp_scan_bwd_desc d{};
     d.f = scan_desc(v, starts, state, false);
     d.f.ckpt = mfloat(ckpt); d.f.ckpt_floats = ckpt.defined() ? ckpt.numel() : 0;
@@ -554,7 +575,7 @@ std::tuple<Tensor, Tensor> selective_scan(const Tensor& u, const Tensor& delta, 
   Tensor state;
   if (state_ && state_->defined()) {
     state32(*state_, {u.size(0), u.size(2), A.size(1)}, u);
-    state = state_->contiguous();
+    state = whole(*state_);
   }
   if (!training(v.u, v.delta, v.A, v.B, v.C, v.D, v.z, v.bias, state)) {
     const ScanRun o = scan_run(v, starts, state, false);
@@ -569,11 +590,12 @@ Tensor selective_scan_step(const Tensor& u, const Tensor& state, const Tensor& d
   serving("selective_scan_step", u, state, delta, A, B, C, D, z, bias);
   const ScanIn v = scan_in(u, delta, A, B, C, D, z, bias, 1);
   state32(state, {u.size(0), u.size(1), A.size(1)}, u);
-  TORCH_CHECK_VALUE(state.is_contiguous(), "state must be contiguous: it is advanced in place");
+  in_place(state);
   const Tensor reset = marks(reset_, "reset", u.sizes().slice(0, 1), u), out = fresh(u.sizes(), u.scalar_type(), u);
   pnp_scan_desc d = scan_desc(v, reset, state, true);
   d.out = mptr(out); d.last_state = mfloat(state);
   CALL(selective_scan_step, u, &d);
+  advanced(state);
   return out;
 }
 

@@ -22,7 +22,12 @@ call gives the same bits.  There is no CPU path: a CPU tensor is a ``ValueError`
 Sequences that end inside a batch: ``starts`` [B, L] (uint8 or bool) marks tokens that begin a new
 sequence; they and what follows see nothing from before, whatever it holds (infinities and NaN
 included).  Sequences of different lengths go padded on the left, with a start at the first real token;
-packed sequences go one after the other in a row.
+packed sequences go one after the other in a row.  Padding is a sequence of its own, with outputs of its
+own: where weights are trained it holds finite values, since a gradient of zero times NaN is NaN.
+
+A captured graph may hold any call, its backward pass too; as everywhere in torch, no eager graph of the
+same leaves may live while a backward pass is captured (capture over detached copies of the leaves, or
+after the eager graphs are gone).
 """
 from __future__ import annotations
 
@@ -70,7 +75,8 @@ def add_rms_norm(x, weight, residual=None, eps=1e-6):
     returns ``(y, s)``.  ``s`` is held in the residual's type (x's, or fp32 under 16-bit activations:
     a residual stream that many layers add to), and what is held is what is normalised; without a
     residual ``s`` is ``x`` (take the stream's gradient through it: the two paths then meet in one
-    rounding).  A row that holds infinity or NaN is NaN in ``y``."""
+    rounding).  A row that holds NaN is NaN in ``y``; in one whose squares outgrow fp32 (infinity among
+    them) what is finite is 0 and infinity NaN, as by the formula."""
     return _ext.add_rms_norm(x, weight, residual, eps)
 
 

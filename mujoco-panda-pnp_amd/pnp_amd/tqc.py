@@ -333,6 +333,8 @@ class TQC:
         torch.manual_seed(c.seed)             # same initial weights on every rank (broadcast below too)
         if c.history < 0:
             raise ValueError(f"history must not be negative (got {c.history})")
+        if c.rollout_int8 and not c.history:
+            raise ValueError("rollout_int8 is of the history's encoder: set history")
         if c.history and self.device.type != "cuda":
             raise ValueError("history: the sequence operators need a HIP device (there is no CPU path)")
         in_dim = self.obs_dim + (c.history_dim if c.history else 0)

@@ -59,3 +59,8 @@ def test_train_refuses_8_bits_without_history():
     from pnp_amd import train
     with pytest.raises(SystemExit):
         train.main(["--rollout-int8"])
+
+
+def test_learner_refuses_8_bits_without_history():
+    with pytest.raises(ValueError, match="set history"):
+        T.TQC(ToyReach(4), T.TQCConfig(rollout_int8=True))

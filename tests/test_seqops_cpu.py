@@ -186,6 +186,27 @@ def test_c_gradients_refuse_small_workspaces():
     assert L.pnp_selective_scan(C.byref(f), None) == -1 and b"workspace" in L.pnp_last_error()
 
 
+def test_c_scan_refuses_strides_and_channels_out_of_range():
+    """Offsets within a tile are 32-bit; the gradient's last sums are one launch over dim * (N + 2) columns."""
+    from pnp_amd import _lib
+    L = _lib.load()
+    for field in ("u_tstride", "delta_tstride", "z_tstride", "B_tstride", "C_tstride"):
+        for value in ((1 << 24) + 1, -1):
+            f = _scan()
+            setattr(f, field, value)
+            assert L.pnp_selective_scan(C.byref(f), None) == -1 and b"stride" in L.pnp_last_error()
+    s = _lib.PnpScanBwdDesc()
+    s.f = _scan()
+    s.f.B, s.f.L = 1, 1
+    s.f.ckpt = s.dout = s.du = s.ddelta = s.dB = s.dC = s.dA = s.workspace = 4096
+    s.f.ckpt_floats = s.workspace_floats = 1 << 60
+    s.dout_tstride = (1 << 24) + 1
+    assert L.pnp_selective_scan_bwd(C.byref(s), None) == -1 and b"stride" in L.pnp_last_error()
+    s.dout_tstride = 0
+    s.f.dim, s.f.N = 1 << 22, 62
+    assert L.pnp_selective_scan_bwd(C.byref(s), None) == -1 and b"too many channels" in L.pnp_last_error()
+
+
 def test_c_empty_batches_launch_nothing():
     from pnp_amd import _lib
     L = _lib.load()

@@ -1,0 +1,330 @@
+"""Calls of the sequence operators (pnp_amd.seqops) that their documentation allows at its edges: offsets past 32 bits,
+the same tensor twice, broadcast and negated views, states that autograd or a graph holds, growing states."""
+import pytest
+import torch
+
+import seq_plain as P
+from test_seqops_gpu import S, Draw, dev, plain_scan, run_scan, scan_inputs   # noqa: F401  (S: the fixture)
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+# ---------------------------------------------------------------------------------- autograd
+def test_second_gradients_are_refused(S):
+    x, w = dev(Draw(1)(2, 9, 16), True), torch.ones(16, 4, device="cuda")
+    B = dev(Draw(2)(2, 9, 4))
+    for y in (S.add_rms_norm(x, w[:, 0])[0], S.add_rms_norm(x, w[:, 0], x)[1], S.causal_conv(x, w)[0],
+              S.selective_scan(x, x, -w, B, B)[0]):
+        g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="second gradient"):
+            g.sum().backward()
+
+
+def test_a_state_advanced_in_place_is_refused_by_the_graph_that_holds_it(S):
+    d = Draw(3)
+    x, w, A, B = dev(d(2, 5, 8), True), dev(d(8, 4)), -torch.ones(8, 4, device="cuda"), dev(d(2, 5, 4))
+    conv, ssm = torch.zeros(2, 3, 8, device="cuda"), torch.zeros(2, 8, 4, device="cuda")
+    y, _ = S.causal_conv(x, w, state=conv)
+    o, _ = S.selective_scan(x, x, A, B, B, state=ssm)
+    with torch.no_grad():
+        S.causal_conv_step(x[:, 0], conv, w)
+        S.selective_scan_step(x[:, 0], ssm, x[:, 0], A, B[:, 0], B[:, 0])
+    for t in (y, o):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            t.sum().backward()
+    with torch.inference_mode():      # no versions there: the same numbers
+        c2, s2 = torch.zeros(2, 3, 8, device="cuda"), torch.zeros(2, 8, 4, device="cuda")
+        S.causal_conv_step(x[:, 0], c2, w)
+        S.selective_scan_step(x[:, 0], s2, x[:, 0], A, B[:, 0], B[:, 0])
+        assert torch.equal(c2, conv) and torch.equal(s2, ssm)
+
+
+def test_the_stream_written_in_place_is_refused(S):
+    x, r = dev(Draw(4)(3, 16), True), dev(Draw(5)(3, 16))
+    y, s = S.add_rms_norm(x, torch.ones(16, device="cuda"), r)
+    with torch.no_grad():
+        s += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_the_same_tensor_twice(S):
+    """Gradients of a tensor in several places are the sums of the places' gradients (fp32: a rounding an addition)."""
+    d = Draw(6)
+    x, w, A, B = dev(d(2, 40, 16), True), dev(1 + d(16)), -dev(d(16, 8).abs()), dev(d(2, 40, 8), True)
+    dy = dev(d(2, 40, 16))
+    apart = lambda t, n: [t.detach().clone().requires_grad_() for _ in range(n)]   # noqa: E731
+
+    def same(got, parts):
+        terms = torch.stack([p.double() for p in parts])
+        P.close(got, terms.sum(0), terms.abs().sum(0), len(parts))
+
+    y, s = S.add_rms_norm(x, w, x)
+    a = apart(x, 2)
+    y2, s2 = S.add_rms_norm(a[0], w, a[1])
+    assert torch.equal(y, y2) and torch.equal(s, s2)
+    same(*torch.autograd.grad([y, s], x, [dy, dy]), torch.autograd.grad([y2, s2], a, [dy, dy]))
+    o, _ = S.selective_scan(x, x, A, B, B, z=x)
+    a, b = apart(x, 3), apart(B, 2)
+    o2, _ = S.selective_scan(a[0], a[1], A, b[0], b[1], z=a[2])
+    assert torch.equal(o, o2)
+    gx, gB = torch.autograd.grad(o, [x, B], dy)
+    g = torch.autograd.grad(o2, a + b, dy)
+    same(gx, g[:3])
+    same(gB, g[3:])
+
+
+def test_gradients_of_the_last_state_alone_and_of_the_output_alone(S):
+    d = Draw(7)
+    v = {k: dev(t, k != "starts") for k, t in scan_inputs(d, 2, 45, 24, 16, 1, BF).items()}
+    w = dev(d(24, 3), True)
+    leaves = [t for k, t in v.items() if k != "starts"]
+    dl, dy = dev(d(2, 24, 16)), dev(d(2, 45, 24, dtype=BF))
+    o, last = run_scan(S, v)
+    for outs, gs, full in (([last], [dl], [torch.zeros_like(o), dl]), ([o], [dy], [dy, torch.zeros_like(last)])):
+        got = torch.autograd.grad(outs, leaves, gs, retain_graph=True, materialize_grads=True)
+        want = torch.autograd.grad([o, last], leaves, full, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    y, last = S.causal_conv(v["u"], w, starts=v["starts"])
+    dl = dev(d(2, 2, 24, dtype=BF))
+    for outs, gs, full in (([last], [dl], [torch.zeros_like(y), dl]), ([y], [dy], [dy, torch.zeros_like(last)])):
+        got = torch.autograd.grad(outs, [v["u"], w], gs, retain_graph=True)
+        want = torch.autograd.grad([y, last], [v["u"], w], full, retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------------------------- views
+def test_broadcast_views_and_their_gradients(S):
+    """Rows, batches and gradients that are one row or one batch many times over, against copies of them."""
+    d = Draw(8)
+    one, w, A, B = d(1, 37, 32), dev(d(32, 4)), -dev(d(32, 16).abs()), d(1, 37, 16)
+    dy = dev(d(1, 1, 32)).expand(3, 37, 32)
+
+    def ops(x, B, dy):
+        x, B = x.requires_grad_(), B.requires_grad_()
+        y, s = S.add_rms_norm(x, w[:, 0], x)
+        c, _ = S.causal_conv(x, w, activation="silu")
+        o, last = S.selective_scan(x, x, A, B, B)
+        with torch.no_grad():
+            q = S.quantize_rows(x)
+            p = S.matmul_i8(*q, q[0][0, :5], q[1][0, :5])
+        return [y, s, c, o, last, p] + [g for t in (y, s, c, o) for g in torch.autograd.grad(t, x, dy, retain_graph=True)] + \
+            list(torch.autograd.grad(o, B, dy))
+
+    got = ops(dev(one).expand(3, 37, 32).detach(), dev(B).expand(3, 37, 16).detach(), dy)
+    want = ops(dev(one.repeat(3, 1, 1)), dev(B.repeat(3, 1, 1)), dy.contiguous())
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_views_that_stand_for_their_negative(S):
+    """torch marks such views and leaves the memory as it is."""
+    d = Draw(9)
+    x, w, A, B, st = dev(d(2, 9, 16)), dev(d(16, 4)), dev(d(16, 4).abs()), dev(d(2, 9, 4)), dev(d(2, 3, 16))
+    h = dev(d(2, 16, 4))
+
+    def ops(neg):
+        x_, w_, A_, B_, st_, h_ = (neg(t.clone().requires_grad_()) for t in (x, w, A, B, st, h))
+        y, _ = S.add_rms_norm(x_, w_[:, 0], x_)
+        c, cl = S.causal_conv(x_, w_, w_[:, 0], state=st_)
+        o, last = S.selective_scan(x_, x_, A_, B_, B_, state=h_)
+        back = torch.autograd.grad([y, c, o], [x_, w_, A_, B_], [neg(x), neg(x), neg(x)])
+        with torch.no_grad():
+            q, s = S.quantize_rows(x_)
+            p = S.matmul_i8(neg(q), s, neg(q[0]), neg(s[0]))
+        return [y, c, cl, o, last, q, s, p, *back]
+
+    for a, b in zip(ops(torch._neg_view), ops(torch.neg)):
+        assert torch.equal(a, b)
+    with torch.no_grad(), pytest.raises(ValueError, match="contiguous"):
+        S.causal_conv_step(x[:, 0], torch._neg_view(st), w)
+
+
+# ---------------------------------------------------------------------------------- values
+def test_rows_with_infinity(S):
+    x = torch.randn(4, 64, device="cuda")
+    x[1, 5], x[2, 7], x[3] = float("inf"), float("nan"), 0
+    y, _ = S.add_rms_norm(x, torch.ones(64, device="cuda"))
+    assert torch.isfinite(y[0]).all() and torch.isnan(y[2]).all() and not y[3].any()
+    assert torch.isnan(y[1, 5]) and not y[1, torch.arange(64) != 5].any()
+    q, s, _ = S.add_rms_norm_q8(x, torch.ones(64, device="cuda"))
+    assert torch.isnan(s[1:3]).all() and s[3] == 0 and not q[1:].any()
+
+
+def test_a_growing_state_that_starts_at_zero_in_a_cut_sequence(S):
+    """A > 0 over many chunks: the chunks' factors outgrow fp32 (exp(2 * 128)) while the state is zero."""
+    d = Draw(10)
+    L = 4096
+    u, B = d(1, L, 16), d(1, L, 1, 8)
+    u[:, :2048] = 0
+    delta = torch.where(torch.arange(L) < 2048, 0.5, -20.0)[None, :, None].expand(1, L, 16).contiguous()
+    v = dict(u=u, delta=delta, A=torch.full((16, 8), 2.0), B=B, C=d(1, L, 1, 8), D=None, z=None, bias=None, starts=None, state=None)
+    out, last = run_scan(S, {k: dev(t) for k, t in v.items()})
+    ro, rl, eo, el = plain_scan(v)
+    assert not out[:, :2048].any() and torch.isfinite(out).all()
+    P.close(out, ro, eo, 1, "out")
+    P.close(last, rl, el, 1, "last")
+
+
+# ---------------------------------------------------------------------------------- sizes
+def test_sizes_past_what_is_held_in_32_bits_are_refused(S):
+    n = 2 ** 32 + 16      # 16, to who keeps 32 bits of it
+    one = torch.ones(1, device="cuda", dtype=BF)
+    x, w = one.expand(1, n), one.expand(n)
+    for call in (lambda: S.add_rms_norm(x, w), lambda: S.add_rms_norm_q8(x, w), lambda: S.quantize_rows(x),
+                 lambda: S.causal_conv(x[None], one.expand(n, 4)), lambda: S.causal_conv_step(x, one.expand(1, 3, n), one.expand(n, 4)),
+                 lambda: S.selective_scan(x[None], x[None], one.expand(n, 4), one.expand(1, 1, 4), one.expand(1, 1, 4)),
+                 lambda: S.selective_scan_step(x, one.float().expand(1, n, 4), x, one.expand(n, 4), one.expand(1, 4), one.expand(1, 4)),
+                 lambda: S.matmul_i8(one.to(torch.int8).expand(1, n), one, one.to(torch.int8).expand(1, n), one)):
+        with pytest.raises(ValueError):
+            call()
+
+
+@pytest.fixture(scope="module")
+def tall():
+    """2^20 + 3 rows of 4096: more elements than 32 bits count."""
+    if torch.cuda.get_device_properties(0).total_memory < 200e9:
+        pytest.skip("needs a device with more than 200 GB")
+    x = torch.empty(2 ** 20 + 3, 4096, dtype=BF, device="cuda")
+    torch.manual_seed(0)
+    for part in x.split(2 ** 18):
+        part.normal_()
+    yield x
+    del x
+    torch.cuda.empty_cache()
+
+
+END = 70     # rows compared: a run of their own gives them too
+
+
+def near(a, b, steps):
+    """Steps of bf16, or of a few roundings in fp32: another variant of a kernel, its products fused otherwise."""
+    step = 2.0 ** -7 if a.dtype == BF else 2.0 ** -20
+    a, b = a.double(), b.double()
+    assert ((a - b).abs() <= steps * step * b.abs().clamp_min(b.abs().mean())).all()
+
+
+def test_offsets_past_32_bits_norm_and_product(S, tall):
+    w = 1 + 0.1 * torch.randn(4096, device="cuda")
+    x = tall.requires_grad_()
+    y, _ = S.add_rms_norm(x, w)
+    gx, = torch.autograd.grad(y, x, tall.detach())
+    x2 = tall[-END:].detach().clone().requires_grad_()
+    y2, _ = S.add_rms_norm(x2, w)
+    g2, = torch.autograd.grad(y2, x2, x2.detach())
+    assert torch.equal(y[-END:], y2) and torch.equal(gx[-END:], g2)
+    tall.requires_grad_(False)
+    del x, y, gx
+    q, s = S.quantize_rows(tall)
+    q2, s2 = S.quantize_rows(tall[-END:])
+    assert torch.equal(q[-END:], q2) and torch.equal(s[-END:], s2)
+    wq, ws = S.quantize_rows(torch.randn(4096, 64, device="cuda"))
+    for k in (16, 4096):      # long rows of q; then many columns of the output
+        a, b = (q, wq[:16].repeat(1, 64)) if k == 4096 else (q[:, :64], wq)
+        o = S.matmul_i8(a, s, b, ws[:b.shape[0]], out_dtype=BF)
+        assert torch.equal(o[-END:], S.matmul_i8(a[-END:].contiguous(), s2, b, ws[:b.shape[0]], out_dtype=BF))
+        del o
+
+
+def test_offsets_past_32_bits_convolution(S, tall):
+    w = torch.randn(4096, 4, device="cuda")
+    x = tall[None].requires_grad_()
+    y, last = S.causal_conv(x, w, activation="silu")
+    gx, = torch.autograd.grad(y, x, x.detach())
+    x2 = tall[None, -END:].detach().clone().requires_grad_()
+    y2, last2 = S.causal_conv(x2, w, activation="silu", state=tall[None, -END - 3:-END].detach())
+    g2, = torch.autograd.grad(y2, x2, x2.detach())
+    assert torch.equal(y[:, -END:], y2) and torch.equal(gx[:, -END:], g2) and torch.equal(last, last2)
+
+
+def test_offsets_past_32_bits_scan(S, tall):
+    """The end is a sequence of its own (a start); at most one step of bf16 off, the two runs' tiles lying differently."""
+    L = tall.shape[0]
+    A, B = -torch.rand(4096, 16, device="cuda") - 0.1, torch.randn(1, L, 16, device="cuda", dtype=BF)
+    starts = torch.zeros(1, L, dtype=torch.bool, device="cuda")
+    starts[0, -END] = True
+
+    def run(x, B, starts):
+        x, B = x.requires_grad_(), B.requires_grad_()
+        y, last = S.selective_scan(x, x, A, B, B, z=x, starts=starts)
+        return [y[:, -END:], last] + [g[:, -END:] for g in torch.autograd.grad(y, [x, B], x.detach())]
+
+    got = run(tall[None].detach(), B, starts)
+    want = run(tall[None, -END:].detach().clone(), B[:, -END:].detach().clone(), starts[:, -END:].contiguous())
+    for a, b in zip(got, want):
+        near(a, b, 4)     # (x's gradient is the sum of three, each rounded to bf16 and each maybe a step off)
+
+
+def test_offsets_past_32_bits_steps(S):
+    if torch.cuda.get_device_properties(0).total_memory < 200e9:
+        pytest.skip("needs a device with more than 200 GB")
+    n, d = 2 ** 20 + 5, 2048
+    torch.manual_seed(1)
+    x, w = torch.randn(n, d, device="cuda", dtype=BF), torch.randn(d, 4, device="cuda")
+    conv = torch.zeros(n, 3, d, device="cuda", dtype=BF)
+    conv[-END:].normal_()
+    c2 = conv[-END:].clone()
+    assert conv.numel() > 2 ** 32
+    y, y2 = S.causal_conv_step(x, conv, w), S.causal_conv_step(x[-END:], c2, w)
+    assert torch.equal(y[-END:], y2) and torch.equal(conv[-END:], c2)
+    del conv, y
+    torch.cuda.empty_cache()
+    n = 2 ** 17 + 5
+    ssm = torch.zeros(n, d, 16, device="cuda")
+    ssm[-END:].normal_()
+    s2 = ssm[-END:].clone()
+    assert ssm.numel() > 2 ** 32
+    A, B = -torch.rand(d, 16, device="cuda"), torch.randn(n, 16, device="cuda", dtype=BF)
+    u = x[:n]
+    y = S.selective_scan_step(u, ssm, u, A, B, B, z=u)
+    y2 = S.selective_scan_step(u[-END:], s2, u[-END:], A, B[-END:], B[-END:], z=u[-END:])
+    near(y[-END:], y2, 1)
+    near(ssm[-END:], s2, 1)
+    del ssm, y
+    torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------------------------- graphs
+def test_captured_steps_carry_their_states(S):
+    """Two captured graphs of a step, each with states of its own, replayed in turn against eager steps."""
+    d = Draw(11)
+    w, A = dev(d(32, 4)), -dev(d(32, 16).abs())
+    wq = None
+
+    def step(x, conv, ssm, reset):
+        nonlocal wq
+        u = S.causal_conv_step(x, conv, w, activation="silu", reset=reset)
+        q, s, _ = S.add_rms_norm_q8(u, w[:, 0], x)
+        p = S.matmul_i8(q, s, *wq)
+        return S.selective_scan_step(u, ssm, p[:, :32], A, p[:, 32:48], p[:, 48:], z=x, reset=reset)
+
+    def new():
+        return [dev(d(70, 32)), torch.zeros(70, 3, 32, device="cuda"), torch.zeros(70, 32, 16, device="cuda"),
+                torch.zeros(70, dtype=torch.uint8, device="cuda")]
+
+    wq = S.quantize_rows(dev(d(64, 32)))
+    sets, graphs = [new(), new()], []
+    mirror = [[t.clone() for t in s] for s in sets]
+    for s in sets:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*[t.clone() for t in s])
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            s.append(step(*s))
+        graphs.append(g)
+    for k in range(6):
+        for s, m in zip(sets, mirror):
+            x, r = dev(d(70, 32)), dev(d.starts(70))
+            for to in (s, m):
+                to[0].copy_(x)
+                to[3].copy_(r)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for s, m in zip(sets, mirror):
+            want = step(*m)
+            assert torch.equal(s[4], want) and torch.equal(s[1], m[1]) and torch.equal(s[2], m[2]), k
