@@ -105,9 +105,15 @@ __device__ __forceinline__ int k_of(int g) { return g == 0 ? 0 : g == 1 ? 3 : g 
 // with chunk k_of(g) for the lanes' g-th sixteen (any order of k serves) each such set meets 16 different bank
 // groups: 2.0 -> 1.0 cycles of LDS a read against the order 0, 1, 2, 3.
 //
-// FAST (rows on 16-byte boundaries, K a multiple of 16): ST stages, filled ST - 1 ahead by loads into LDS; such
-// a load writes 64 lanes' chunks in a row, so the lane's global address carries the exchange; chunks past K come
-// from `zeros`.  Otherwise two stages, by way of registers.
+// FAST (rows on 16-byte boundaries, K a multiple of 16): ST stages, filled by loads into LDS; such a load writes
+// 64 lanes' chunks in a row, so the lane's global address carries the exchange; chunks past K come from `zeros`.  A
+// stage's operands are read into registers under the product of the stage before (a quarter of a wave's registers;
+// bf16 out, 8192^3 493 -> 477 us, 2048 x 2048 x 8192 50 -> 46 us, against reading them before their own product),
+// and its buffer is loaded anew, ST stages on, as soon as everybody has.  Otherwise two stages, by way of registers.
+//
+// Bound by the matrix cores at the clock that the power leaves them: 8192^3 2.3 POP/s (a large bf16 library product
+// 1.2 PFLOP/s; of the cycles at 2 GHz the matrix cores are busy about 55 %).  Small products by their few stages:
+// 8192 x 1024 x 256 13 us, 0.33 POP/s.
 __device__ const v4i zeros[1] = {};
 
 template <typename T, int BM, int BN, int WGM, int WGN, bool FAST>
@@ -144,22 +150,24 @@ __global__ __launch_bounds__(64 * WGM* WGN, 2) void i8_tile_kernel(I8Args a) {
 #pragma unroll
     for (int j = 0; j < WM; j++) acc[i][j] = v4i{0, 0, 0, 0};
   const int fr = lane & 15, fc = lane >> 4, kc = k_of(fc);
-  auto product = [&](int buf) {
-    v4i fw[WN], fq[WM];
+  struct Operands { v4i w[WN], q[WM]; };
+  auto read = [&](int buf, Operands& f) {
 #pragma unroll
     for (int i = 0; i < WN; i++) {
       const int r = wn + (fr >> 2) * C + i * 4 + (fr & 3);
-      fw[i] = sw[buf][r * 4 + (kc ^ (r / C & 3))];
+      f.w[i] = sw[buf][r * 4 + (kc ^ (r / C & 3))];
     }
 #pragma unroll
     for (int j = 0; j < WM; j++) {
       const int r = wm + j * 16 + fr;
-      fq[j] = sq[buf][r * 4 + (kc ^ (r >> 2 & 3))];
+      f.q[j] = sq[buf][r * 4 + (kc ^ (r >> 2 & 3))];
     }
+  };
+  auto product = [&](const Operands& f) {
 #pragma unroll
     for (int j = 0; j < WM; j++)
 #pragma unroll
-      for (int i = 0; i < WN; i++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[i], fq[j], acc[i][j], 0, 0, 0);
+      for (int i = 0; i < WN; i++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.w[i], f.q[j], acc[i][j], 0, 0, 0);
   };
   if constexpr (FAST) {
     const uint32_t lw = lds_address(&sw[0][wave * 64]), lq = lds_address(&sq[0][wave * 64]);
@@ -172,14 +180,27 @@ __global__ __launch_bounds__(64 * WGM* WGN, 2) void i8_tile_kernel(I8Args a) {
       for (int i = 0; i < LQ; i++)
         load_to_lds(k + cq[i] < a.K ? pq[i] + k + cq[i] : (const int8_t*)zeros, lq + (buf * BM * 4 + i * NT) * 16);
     };
+    // before stage s's product: this wave's loads of stage s + 1 have arrived, and what it read of stage s is in
+    // registers; then, past the barrier, everybody's have and is: the buffer of stage s is free
+    auto meet = [&]() {
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((ST - 2) * (LW + LQ)) : "memory");
+      __builtin_amdgcn_s_barrier();
+    };
+    Operands f0, f1;
 #pragma unroll
     for (int s = 0; s < ST - 1; s++) fetch(s);
-    for (int s = 0; s < nk; s++) {
-      // this wave's loads of stage s have arrived, and what it read of stage s - 1 is in registers
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((ST - 2) * (LW + LQ)) : "memory");
-      __builtin_amdgcn_s_barrier();   // everybody's have and is: the buffer of stage s - 1 is free
-      fetch(s + ST - 1);
-      product(s % ST);
+    meet();
+    fetch(ST - 1);
+    read(0, f0);
+    for (int s = 0; s < nk; s += 2) {
+      meet();
+      fetch(s + ST);
+      read((s + 1) % ST, f1);
+      product(f0);
+      meet();
+      fetch(s + ST + 1);
+      read((s + 2) % ST, f0);
+      if (s + 1 < nk) product(f1);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the workgroup
   } else {
@@ -201,7 +222,9 @@ __global__ __launch_bounds__(64 * WGM* WGN, 2) void i8_tile_kernel(I8Args a) {
     for (int s = 0; s < nk; s++) {
       __syncthreads();   // stage s is there, and everybody has read stage s - 1
       if (s + 1 < nk) fetch(s + 1);
-      product(s & 1);
+      Operands f;
+      read(s & 1, f);
+      product(f);
       if (s + 1 < nk) put((s + 1) & 1);
     }
   }
@@ -218,7 +241,7 @@ __global__ __launch_bounds__(64 * WGM* WGN, 2) void i8_tile_kernel(I8Args a) {
   }
 }
 
-// Few tokens (16 MT at most): the weights' bytes are what counts.  A workgroup has 16 channels, its 4 waves the
+// Few tokens (16 MT at most): the weights' bytes are what counts (one token by 1000 x 512: 3 us, a launch's own time).  A workgroup has 16 channels, its 4 waves the
 // stages of k in turn, straight from memory to registers; their sums meet in LDS.
 template <typename T, int MT> __global__ __launch_bounds__(256) void i8_rows_kernel(I8Args a) {
   __shared__ v4i part[3][MT][64];
