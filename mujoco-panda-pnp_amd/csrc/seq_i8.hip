@@ -4,8 +4,10 @@
 // Both operands run along k in memory, so a lane's 16 bytes of a row are its operand of
 // v_mfma_i32_16x16x64_i8 as they lie (any order of k serves, as long as both operands have the same).
 // The weights are the instruction's rows and the tokens its columns: a lane then holds 4 output channels
-// of one token.  The channels of a wave are dealt to its fragments so that a lane's 4 of each lie together:
-// fragment i's row 4 g + r is channel 4 WN g + 4 i + r, and a lane stores 4 WN neighbouring channels.
+// of one token.  The channels of a wave are dealt to its fragments so that a lane's 4 of neighbouring fragments make a
+// pack of V channels (16 bytes of output) and the 4 lanes of a token 4 packs in a row, whole 64 bytes a store:
+// fragment i's row 4 g + r is channel 4 V (i / (V / 4)) + V g + 4 (i % (V / 4)) + r.  Against 4 WN neighbouring
+// channels a lane (stores of 16 bytes with gaps between): 8192 x 8192 x 1024 109 -> 89 us, 8192 x 1024 x 256 12.8 -> 11.1.
 #include <type_traits>
 
 #include "seq_dev.h"
@@ -60,38 +62,45 @@ __device__ __forceinline__ void tile_of(int id, int tiles_n, int tiles_m, int& t
   tm = 8 * band + r % h;
 }
 
-// what a lane's channels n .. n + C - 1 are scaled by and get added
-template <int C> struct Channels {
+// A lane's C channels: packs of V, 4 V apart, from n on.
+template <typename T> constexpr int pack_of() { return 16 / (int)sizeof(T); }
+template <typename T> __device__ __forceinline__ int channel(int n, int i) {
+  constexpr int V = pack_of<T>();
+  return n + i / V * 4 * V + i % V;
+}
+// what they are scaled by and get added
+template <typename T, int C> struct Channels {
   float s[C], b[C];
   __device__ __forceinline__ Channels(const I8Args& a, int n) {
 #pragma unroll
     for (int i = 0; i < C; i++) {
-      s[i] = n + i < a.N ? a.wscale[n + i] : 0.f;
-      b[i] = a.bias && n + i < a.N ? a.bias[n + i] : 0.f;
+      const int c = channel<T>(n, i);
+      s[i] = c < a.N ? a.wscale[c] : 0.f;
+      b[i] = a.bias && c < a.N ? a.bias[c] : 0.f;
     }
   }
 };
 template <typename T, int C>
-__device__ __forceinline__ void store_token(const I8Args& a, int64_t m, int n, const int (&acc)[C], const Channels<C>& ch) {
-  if (m >= a.M || n >= a.N) return;
+__device__ __forceinline__ void store_token(const I8Args& a, int64_t m, int n, const int (&acc)[C], const Channels<T, C>& ch) {
+  if (m >= a.M) return;
   const float sm = a.scale[m];
-  T* o = (T*)a.out + m * a.N + n;
+  T* o = (T*)a.out + m * a.N;
   float f[C];
 #pragma unroll
   for (int i = 0; i < C; i++) f[i] = (float)acc[i] * sm * ch.s[i] + ch.b[i];
-  constexpr int V = C * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : C;
+  constexpr int V = C < pack_of<T>() ? C : pack_of<T>();
   if (a.wide) {   // N is a multiple of the pack: a pack is whole or past the end
 #pragma unroll
     for (int i = 0; i < C; i += V) {
       float w[V];
 #pragma unroll
       for (int k = 0; k < V; k++) w[k] = f[i + k];
-      if (n + i < a.N) store_f<V>(o + i, w);
+      if (channel<T>(n, i) < a.N) store_f<V>(o + channel<T>(n, i), w);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < C; i++)
-      if (n + i < a.N) o[i] = from_f<T>(f[i]);
+      if (channel<T>(n, i) < a.N) o[channel<T>(n, i)] = from_f<T>(f[i]);
   }
 }
 
@@ -100,7 +109,7 @@ __device__ __forceinline__ int k_of(int g) { return g == 0 ? 0 : g == 1 ? 3 : g 
 
 // A BN (channels) x BM (tokens) tile by WGN x WGM waves, a stage of BK bytes of k of both operands at a time
 // through LDS.  A row of a stage is 4 chunks of 16 bytes; chunk c of row r lies at c ^ f(r), f the bits of r
-// in which the 4 groups of a fragment's 16 rows differ (r / 4 for tokens, r / (4 WN) for channels, mod 4).  LDS
+// in which the 4 groups of a fragment's 16 rows differ (r / 4 for tokens, r / V for channels, mod 4).  LDS
 // serves a 16-byte read 16 lanes at a time, of the first 32 lanes 0 .. 3, 12 .. 15, 20 .. 27 and then the others;
 // with chunk k_of(g) for the lanes' g-th sixteen (any order of k serves) each such set meets 16 different bank
 // groups: 2.0 -> 1.0 cycles of LDS a read against the order 0, 1, 2, 3.
@@ -111,16 +120,16 @@ __device__ __forceinline__ int k_of(int g) { return g == 0 ? 0 : g == 1 ? 3 : g 
 // bf16 out, 8192^3 493 -> 477 us, 2048 x 2048 x 8192 50 -> 46 us, against reading them before their own product),
 // and its buffer is loaded anew, ST stages on, as soon as everybody has.  Otherwise two stages, by way of registers.
 //
-// Bound by the matrix cores at the clock that the power leaves them: 8192^3 2.3 POP/s (a large bf16 library product
-// 1.2 PFLOP/s; of the cycles at 2 GHz the matrix cores are busy about 55 %).  Small products by their few stages:
-// 8192 x 1024 x 256 13 us, 0.33 POP/s.
+// Bound by the matrix cores at the clock that the power leaves them: 8192^3 460 us, 2.4 POP/s (a large bf16 library
+// product reaches 1.2 PFLOP/s here; of the cycles at 2 GHz the matrix cores are busy 57 %).  Short sums by their output:
+// 8192 x 1024 x 256 11 us, of which a launch of one tile 4.5 and the writing of 17 MB about 5.
 __device__ const v4i zeros[1] = {};
 
 template <typename T, int BM, int BN, int WGM, int WGN, bool FAST>
 __global__ __launch_bounds__(64 * WGM* WGN, 2) void i8_tile_kernel(I8Args a) {
-  constexpr int NT = 64 * WGM * WGN, ST = FAST ? 4 : 2, WM = BM / WGM / 16, WN = BN / WGN / 16, C = 4 * WN;
+  constexpr int NT = 64 * WGM * WGN, ST = FAST ? 4 : 2, WM = BM / WGM / 16, WN = BN / WGN / 16, C = 4 * WN, V = pack_of<T>(), P = V / 4;
   constexpr int LW = BN * 4 / NT, LQ = BM * 4 / NT;   // chunks of a stage a thread
-  static_assert(LW * NT == BN * 4 && LQ * NT == BM * 4, "whole chunks a thread");
+  static_assert(LW * NT == BN * 4 && LQ * NT == BM * 4 && WN % P == 0, "whole chunks a thread, whole packs a lane");
   __shared__ v4i sw[ST][BN * 4], sq[ST][BM * 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = (wave % WGN) * (BN / WGN), wm = (wave / WGN) * (BM / WGM);
@@ -135,7 +144,7 @@ __global__ __launch_bounds__(64 * WGM* WGN, 2) void i8_tile_kernel(I8Args a) {
 #pragma unroll
   for (int i = 0; i < LW; i++) {
     const int r = (i * NT + tid) >> 2;
-    cw[i] = ((tid & 3) ^ (r / C & 3)) * 16;
+    cw[i] = ((tid & 3) ^ (r / V & 3)) * 16;
     pw[i] = a.w + (int64_t)(n0 + r < a.N ? n0 + r : a.N - 1) * a.ws;
   }
 #pragma unroll
@@ -154,8 +163,8 @@ __global__ __launch_bounds__(64 * WGM* WGN, 2) void i8_tile_kernel(I8Args a) {
   auto read = [&](int buf, Operands& f) {
 #pragma unroll
     for (int i = 0; i < WN; i++) {
-      const int r = wn + (fr >> 2) * C + i * 4 + (fr & 3);
-      f.w[i] = sw[buf][r * 4 + (kc ^ (r / C & 3))];
+      const int r = wn + i / P * 4 * V + (fr >> 2) * V + i % P * 4 + (fr & 3);
+      f.w[i] = sw[buf][r * 4 + (kc ^ (r / V & 3))];
     }
 #pragma unroll
     for (int j = 0; j < WM; j++) {
@@ -228,8 +237,8 @@ __global__ __launch_bounds__(64 * WGM* WGN, 2) void i8_tile_kernel(I8Args a) {
       if (s + 1 < nk) put((s + 1) & 1);
     }
   }
-  const int n = n0 + wn + fc * C;
-  const Channels<C> ch(a, n);
+  const int n = n0 + wn + fc * V;
+  const Channels<T, C> ch(a, n);
 #pragma unroll
   for (int j = 0; j < WM; j++) {
     int o[C];
@@ -265,7 +274,7 @@ template <typename T, int MT> __global__ __launch_bounds__(256) void i8_rows_ker
     for (int j = 0; j < MT; j++) part[wave - 1][j][lane] = acc[j];
   __syncthreads();
   if (wave) return;
-  const Channels<4> ch(a, n0 + fc * 4);
+  const Channels<T, 4> ch(a, n0 + fc * 4);
 #pragma unroll
   for (int j = 0; j < MT; j++) {
     const v4i s = acc[j] + part[0][j][lane] + part[1][j][lane] + part[2][j][lane];
