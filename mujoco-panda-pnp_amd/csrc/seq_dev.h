@@ -36,6 +36,21 @@ template <int V, typename T> __device__ __forceinline__ void store_f(T* p, const
   *reinterpret_cast<Pack<T, V>*>(p) = k;
 }
 
+// p + elems (the same in the wave: a scalar address) + bytes (the lane's 32-bit offset): the form of
+// address that costs one register.  The compiler would add the offset to the tensor's base once and keep
+// that, two registers a tensor, if it saw through the scalar sum.
+#define SEQ_GLOBAL __attribute__((address_space(1)))
+template <typename T> __device__ __forceinline__ const T* at(const void* p, int64_t elems, uint32_t bytes) {
+  uint64_t base = (uint64_t)(static_cast<const T*>(p) + elems);
+  asm("" : "+s"(base));
+  return (const T*)(const SEQ_GLOBAL T*)((const SEQ_GLOBAL char*)base + bytes);
+}
+template <typename T> __device__ __forceinline__ T* at(void* p, int64_t elems, uint32_t bytes) {
+  uint64_t base = (uint64_t)(static_cast<T*>(p) + elems);
+  asm("" : "+s"(base));
+  return (T*)(SEQ_GLOBAL T*)((SEQ_GLOBAL char*)base + bytes);
+}
+
 // sigmoid by the hardware's exp2 and reciprocal: 1 / (1 + 2^(-x log2 e)), relative error a few 2^-24;
 // x -> -inf gives 1 / inf = 0, x -> inf 1
 __device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }

@@ -117,21 +117,6 @@ __device__ __forceinline__ void load_state4(const float* p, int n, int N, float 
   for (int i = 0; i < 4; i++) h[i] = n + i < N ? p[n + i] : 0.f;
 }
 
-// p + elems (the same in the workgroup: a scalar address) + bytes (the thread's 32-bit offset): the form of
-// address that costs one register.  The compiler would add the offset to the tensor's base once and keep
-// that, two registers a tensor, if it saw through the scalar sum.
-#define SEQ_GLOBAL __attribute__((address_space(1)))
-template <typename T> __device__ __forceinline__ const T* at(const void* p, int64_t elems, uint32_t bytes) {
-  uint64_t base = (uint64_t)(static_cast<const T*>(p) + elems);
-  asm("" : "+s"(base));
-  return (const T*)(const SEQ_GLOBAL T*)((const SEQ_GLOBAL char*)base + bytes);
-}
-template <typename T> __device__ __forceinline__ T* at(void* p, int64_t elems, uint32_t bytes) {
-  uint64_t base = (uint64_t)(static_cast<T*>(p) + elems);
-  asm("" : "+s"(base));
-  return (T*)(SEQ_GLOBAL T*)((SEQ_GLOBAL char*)base + bytes);
-}
-
 // the thread's packs of 4 states of a tile's B, then C
 template <typename T, int S, int TT, int NBC, bool WIDE>
 __device__ __forceinline__ void load_bc(const ScanArgs& a, int64_t b, int g, int64_t t, int64_t t1, float4 (&o)[(NBC + NT - 1) / NT]) {
