@@ -24,16 +24,22 @@ template <typename T> __device__ __forceinline__ T from_f(float v) { return (T)v
 // V elements of T moved by one load or store (V * sizeof(T) <= 16, aligned to it)
 template <typename T, int V> struct alignas(V * sizeof(T)) Pack { T v[V]; };
 
-template <int V, typename T> __device__ __forceinline__ void load_f(const T* p, float (&o)[V]) {
-  const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
+// the same from anywhere an element may lie
+template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) LoosePack { T v[V]; };
+template <typename T, int V, bool EVEN> struct PackOf { typedef Pack<T, V> type; };
+template <typename T, int V> struct PackOf<T, V, false> { typedef LoosePack<T, V> type; };
+
+// EVEN: p is on a pack's boundary
+template <int V, bool EVEN = true, typename T> __device__ __forceinline__ void load_f(const T* p, float (&o)[V]) {
+  const auto k = *reinterpret_cast<const typename PackOf<T, V, EVEN>::type*>(p);
 #pragma unroll
   for (int i = 0; i < V; i++) o[i] = to_f(k.v[i]);
 }
-template <int V, typename T> __device__ __forceinline__ void store_f(T* p, const float (&o)[V]) {
-  Pack<T, V> k;
+template <int V, bool EVEN = true, typename T> __device__ __forceinline__ void store_f(T* p, const float (&o)[V]) {
+  typename PackOf<T, V, EVEN>::type k;
 #pragma unroll
   for (int i = 0; i < V; i++) k.v[i] = from_f<T>(o[i]);
-  *reinterpret_cast<Pack<T, V>*>(p) = k;
+  *reinterpret_cast<typename PackOf<T, V, EVEN>::type*>(p) = k;
 }
 
 // p + elems (the same in the wave: a scalar address) + bytes (the lane's 32-bit offset): the form of
@@ -82,7 +88,7 @@ template <int CTRL> __device__ __forceinline__ float dpp(float v) {
 #define SEQ_DPP_ROR8 0x128        // lane i of 16 -> i + 8 mod 16 (the same as xor 8)
 
 // the sum over groups of S neighbouring lanes, in every lane of the group (S 1 .. 64, a power of two);
-// every lane of the wave takes part.  Mirrors serve as xor 4 / xor 8 once the lanes they pair hold equal
+// every lane of the group takes part.  Mirrors serve as xor 4 / xor 8 once the lanes they pair hold equal
 // sums of their quads / halves.
 template <int S> __device__ __forceinline__ float group_sum(float v) {
   if (S >= 2) v += dpp<SEQ_DPP_XOR1>(v);
@@ -95,13 +101,13 @@ template <int S> __device__ __forceinline__ float group_sum(float v) {
 }
 // max that keeps NaN (fmaxf drops it)
 __device__ __forceinline__ float max_nan(float a, float b) { return (a > b || a != a) ? a : b; }
-__device__ __forceinline__ float wave_max_nan(float v) {
-  v = max_nan(v, dpp<SEQ_DPP_XOR1>(v));
-  v = max_nan(v, dpp<SEQ_DPP_XOR2>(v));
-  v = max_nan(v, dpp<SEQ_DPP_HALF_MIRROR>(v));
-  v = max_nan(v, dpp<SEQ_DPP_MIRROR>(v));
-  v = max_nan(v, __shfl_xor(v, 16, 64));
-  v = max_nan(v, __shfl_xor(v, 32, 64));
+template <int S> __device__ __forceinline__ float group_max_nan(float v) {
+  if (S >= 2) v = max_nan(v, dpp<SEQ_DPP_XOR1>(v));
+  if (S >= 4) v = max_nan(v, dpp<SEQ_DPP_XOR2>(v));
+  if (S >= 8) v = max_nan(v, dpp<SEQ_DPP_HALF_MIRROR>(v));
+  if (S >= 16) v = max_nan(v, dpp<SEQ_DPP_MIRROR>(v));
+  if (S >= 32) v = max_nan(v, __shfl_xor(v, 16, 64));
+  if (S >= 64) v = max_nan(v, __shfl_xor(v, 32, 64));
   return v;
 }
 

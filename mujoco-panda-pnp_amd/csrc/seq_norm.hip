@@ -7,8 +7,17 @@
 //   dx = ds + rho (w dy - n mean(w dy n)),  dw = sum over rows of dy n
 //
 // Bound by HBM: a row is read once, kept in registers between its sums and its outputs, and written
-// once.  One wave holds a row of up to 4 packs a lane, a workgroup of 256 threads a wider one (up to
-// 8 packs a thread); rows past that are read twice (the second time from cache).
+// once.  A row that fits gets 8, 16 or 32 lanes with a pack each, a longer one a wave (up to 4 packs a
+// lane), then a workgroup of 256 threads (up to 8 packs a thread); rows past that are read twice (the
+// second time from cache).
+//
+// Rows that are no whole packs, or not on their boundaries (EVEN false): packs from wherever they lie,
+// the last one moved back to end with the row.  Its first elements are another lane's too: written
+// twice, the same value, and counted once.
+//
+// Measured, with a residual: bf16, 8192 x 4096, 42 us forward (268 MB, 6.3 TB/s: part of it from cache), 57 back
+// (336 MB); 16384 x 4096 both in 210 us (1.07 GB at 5.1 TB/s, a large copy's rate); rows of 4095 46 and 60 us (by
+// elements 96 and 167); 200000 rows of 64 19 us (by whole waves 61).
 #include <type_traits>
 
 #include "seq_dev.h"
@@ -32,21 +41,35 @@ struct NormArgs {
 
 // sum over the TPR threads of a row, in each of them; red: NT / 64 floats of LDS, a use apart each call
 template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red) {
-  v = group_sum<64>(v);
-  if (TPR == 64) return v;
+  v = group_sum<TPR < 64 ? TPR : 64>(v);
+  if (TPR <= 64) return v;
   const int w = threadIdx.x >> 6;
   if ((threadIdx.x & 63) == 0) red[w] = v;
   __syncthreads();
   return red[0] + red[1] + red[2] + red[3];
 }
 template <int TPR> __device__ __forceinline__ float row_max(float v, float* red) {
-  v = wave_max_nan(v);
-  if (TPR == 64) return v;
+  v = group_max_nan<TPR < 64 ? TPR : 64>(v);
+  if (TPR <= 64) return v;
   const int w = threadIdx.x >> 6;
   if ((threadIdx.x & 63) == 0) red[w] = v;
   __syncthreads();
   return max_nan(max_nan(red[0], red[1]), max_nan(red[2], red[3]));
 }
+
+// a lane's pack of a row: where it lies, and how many of its elements are its neighbour's
+template <int V, bool EVEN> struct Place {
+  int i, skip;
+  bool on;
+  __device__ __forceinline__ Place(int at, int dim) : i(at), skip(0), on(at < dim) {
+    if (!EVEN && at + V > dim) {
+      skip = at + V - dim;
+      i = dim - V;
+    }
+  }
+  __device__ __forceinline__ bool own(int k) const { return EVEN || k >= skip; }
+  __device__ __forceinline__ float once(int k, float v) const { return own(k) ? v : 0.f; }   // v where the element counts
+};
 
 // scale and 1 / scale of a row whose largest magnitude is m: 0 / 0 where the scale would be below the
 // least normal number, NaN / 0 where m is not finite
@@ -64,17 +87,18 @@ __device__ __forceinline__ int8_t q8(float y, float inv) {
 
 // T: x and y; R: the residual stream; V elements a load; TPR threads a row; NV packs a thread (0: rows
 // of any length, read twice); Q8: 8-bit output
-template <typename T, typename R, int V, int TPR, int NV, bool Q8>
+template <typename T, typename R, int V, bool EVEN, int TPR, int NV, bool Q8>
 __device__ __forceinline__ void norm_fwd_row(const NormArgs& a, int64_t row, float (&red)[2][NT / 64]) {
+  typedef Place<V, EVEN> At;
   const int lane = threadIdx.x % TPR;
   const T* x = (const T*)a.x + row * a.xs;
   const R* r = a.r ? (const R*)a.r + row * a.rs : nullptr;
   R* so = a.s ? (R*)a.s + row * a.dim : nullptr;
   auto read = [&](int i, float (&v)[V]) {
-    load_f<V>(x + i, v);
+    load_f<V, EVEN>(x + i, v);
     if (r) {
       float b[V];
-      load_f<V>(r + i, b);
+      load_f<V, EVEN>(r + i, b);
 #pragma unroll
       for (int k = 0; k < V; k++) v[k] = to_f(from_f<R>(v[k] + b[k]));
     }
@@ -82,13 +106,13 @@ __device__ __forceinline__ void norm_fwd_row(const NormArgs& a, int64_t row, flo
   // short rows take their weights along with the row, not after its sum
   constexpr bool EARLY = NV == 1;
   float early[V];
-  if (EARLY && a.w && lane * V < a.dim) load_f<V>(a.w + lane * V, early);
+  if (EARLY && a.w && lane * V < a.dim) load_f<V, EVEN>(a.w + At(lane * V, a.dim).i, early);
   auto scaled = [&](int i, float rho, float (&v)[V]) {
     float w[V];
     if (EARLY)
 #pragma unroll
       for (int k = 0; k < V; k++) w[k] = early[k];
-    else if (a.w) load_f<V>(a.w + i, w);
+    else if (a.w) load_f<V, EVEN>(a.w + i, w);
 #pragma unroll
     for (int k = 0; k < V; k++) v[k] = a.w ? v[k] * rho * w[k] : v[k] * rho;
   };
@@ -97,31 +121,31 @@ __device__ __forceinline__ void norm_fwd_row(const NormArgs& a, int64_t row, flo
     float v[NV][V];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      const int i = (j * TPR + lane) * V;
-      if (i < a.dim) read(i, v[j]);
+      const At p((j * TPR + lane) * V, a.dim);
+      if (p.on) read(p.i, v[j]);
       else
 #pragma unroll
         for (int k = 0; k < V; k++) v[j][k] = 0.f;
     }
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      const int i = (j * TPR + lane) * V;
-      if (so && i < a.dim) store_f<V>(so + i, v[j]);
+      const At p((j * TPR + lane) * V, a.dim);
+      if (so && p.on) store_f<V, EVEN>(so + p.i, v[j]);
 #pragma unroll
-      for (int k = 0; k < V; k++) sum += v[j][k] * v[j][k];
+      for (int k = 0; k < V; k++) sum += p.once(k, v[j][k]) * p.once(k, v[j][k]);
     }
     const float rho = 1.f / sqrtf(row_sum<TPR>(sum, red[0]) / (float)a.dim + a.eps);
     if (a.rstd && lane == 0) a.rstd[row] = rho;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      const int i = (j * TPR + lane) * V;
-      if (i >= a.dim) continue;
-      scaled(i, rho, v[j]);
+      const At p((j * TPR + lane) * V, a.dim);
+      if (!p.on) continue;
+      scaled(p.i, rho, v[j]);
       if constexpr (Q8) {
 #pragma unroll
         for (int k = 0; k < V; k++) m = max_nan(m, fabsf(v[j][k]));
       } else {
-        store_f<V>((T*)a.y + row * a.dim + i, v[j]);
+        store_f<V, EVEN>((T*)a.y + row * a.dim + p.i, v[j]);
       }
     }
     if constexpr (Q8) {
@@ -130,53 +154,56 @@ __device__ __forceinline__ void norm_fwd_row(const NormArgs& a, int64_t row, flo
       if (lane == 0) a.scale[row] = scale;
 #pragma unroll
       for (int j = 0; j < NV; j++) {
-        const int i = (j * TPR + lane) * V;
-        if (i >= a.dim) continue;
-        Pack<int8_t, V> o;
+        const At p((j * TPR + lane) * V, a.dim);
+        if (!p.on) continue;
+        typename PackOf<int8_t, V, EVEN>::type o;
 #pragma unroll
         for (int k = 0; k < V; k++) o.v[k] = q8(v[j][k], inv);
-        *reinterpret_cast<Pack<int8_t, V>*>(a.q + row * a.qs + i) = o;
+        *reinterpret_cast<typename PackOf<int8_t, V, EVEN>::type*>(a.q + row * a.qs + p.i) = o;
       }
     }
   } else {
-    for (int i = lane * V; i < a.dim; i += TPR * V) {
+    for (int c = lane * V; c < a.dim; c += TPR * V) {
+      const At p(c, a.dim);
       float v[V];
-      read(i, v);
-      if (so) store_f<V>(so + i, v);
+      read(p.i, v);
+      if (so) store_f<V, EVEN>(so + p.i, v);
 #pragma unroll
-      for (int k = 0; k < V; k++) sum += v[k] * v[k];
+      for (int k = 0; k < V; k++) sum += p.once(k, v[k]) * p.once(k, v[k]);
     }
     const float rho = 1.f / sqrtf(row_sum<TPR>(sum, red[0]) / (float)a.dim + a.eps);
     if (a.rstd && lane == 0) a.rstd[row] = rho;
-    for (int i = lane * V; i < a.dim; i += TPR * V) {
+    for (int c = lane * V; c < a.dim; c += TPR * V) {
+      const At p(c, a.dim);
       float v[V];
-      read(i, v);
-      scaled(i, rho, v);
+      read(p.i, v);
+      scaled(p.i, rho, v);
       if constexpr (Q8) {
 #pragma unroll
         for (int k = 0; k < V; k++) m = max_nan(m, fabsf(v[k]));
       } else {
-        store_f<V>((T*)a.y + row * a.dim + i, v);
+        store_f<V, EVEN>((T*)a.y + row * a.dim + p.i, v);
       }
     }
     if constexpr (Q8) {
       float scale, inv;
       q8_scale(row_max<TPR>(m, red[1]), scale, inv);
       if (lane == 0) a.scale[row] = scale;
-      for (int i = lane * V; i < a.dim; i += TPR * V) {
+      for (int c = lane * V; c < a.dim; c += TPR * V) {
+        const At p(c, a.dim);
         float v[V];
-        read(i, v);
-        scaled(i, rho, v);
-        Pack<int8_t, V> o;
+        read(p.i, v);
+        scaled(p.i, rho, v);
+        typename PackOf<int8_t, V, EVEN>::type o;
 #pragma unroll
         for (int k = 0; k < V; k++) o.v[k] = q8(v[k], inv);
-        *reinterpret_cast<Pack<int8_t, V>*>(a.q + row * a.qs + i) = o;
+        *reinterpret_cast<typename PackOf<int8_t, V, EVEN>::type*>(a.q + row * a.qs + p.i) = o;
       }
     }
   }
 }
 
-// rows dealt to the grid; whole waves (TPR 64) or the whole workgroup work on one
+// rows dealt to the grid; up to a wave (TPR 64) or the whole workgroup works on one
 #define SEQ_ROWS(BODY)                                                                                      \
   for (int64_t row = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR; row < a.rows;                    \
        row += (int64_t)gridDim.x * (NT / TPR)) {                                                            \
@@ -184,15 +211,16 @@ __device__ __forceinline__ void norm_fwd_row(const NormArgs& a, int64_t row, flo
     if (TPR > 64) __syncthreads(); /* the next row's sums go where this row's were read */                  \
   }
 
-template <typename T, typename R, int V, int TPR, int NV, bool Q8>
+template <typename T, typename R, int V, bool EVEN, int TPR, int NV, bool Q8>
 __global__ __launch_bounds__(NT) void norm_fwd_kernel(NormArgs a) {
   __shared__ float red[2][NT / 64];
-  SEQ_ROWS((norm_fwd_row<T, R, V, TPR, NV, Q8>(a, row, red)))
+  SEQ_ROWS((norm_fwd_row<T, R, V, EVEN, TPR, NV, Q8>(a, row, red)))
 }
 
 // rows in 8 bits: the norm's kernel without the norm
-template <typename T, int V, int TPR, int NV>
+template <typename T, int V, bool EVEN, int TPR, int NV>
 __device__ __forceinline__ void quantize_row(const NormArgs& a, int64_t row, float (&red)[NT / 64]) {
+  typedef Place<V, EVEN> At;
   const int lane = threadIdx.x % TPR;
   const T* x = (const T*)a.x + row * a.xs;
   int8_t* q = a.q + row * a.qs;
@@ -201,46 +229,48 @@ __device__ __forceinline__ void quantize_row(const NormArgs& a, int64_t row, flo
     float v[NV][V];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      const int i = (j * TPR + lane) * V;
+      const At p((j * TPR + lane) * V, a.dim);
 #pragma unroll
       for (int k = 0; k < V; k++) v[j][k] = 0.f;
-      if (i < a.dim) load_f<V>(x + i, v[j]);
+      if (p.on) load_f<V, EVEN>(x + p.i, v[j]);
 #pragma unroll
       for (int k = 0; k < V; k++) m = max_nan(m, fabsf(v[j][k]));
     }
     q8_scale(row_max<TPR>(m, red), scale, inv);
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      const int i = (j * TPR + lane) * V;
-      if (i >= a.dim) continue;
-      Pack<int8_t, V> o;
+      const At p((j * TPR + lane) * V, a.dim);
+      if (!p.on) continue;
+      typename PackOf<int8_t, V, EVEN>::type o;
 #pragma unroll
       for (int k = 0; k < V; k++) o.v[k] = q8(v[j][k], inv);
-      *reinterpret_cast<Pack<int8_t, V>*>(q + i) = o;
+      *reinterpret_cast<typename PackOf<int8_t, V, EVEN>::type*>(q + p.i) = o;
     }
   } else {
-    for (int i = lane * V; i < a.dim; i += TPR * V) {
+    for (int c = lane * V; c < a.dim; c += TPR * V) {
+      const At p(c, a.dim);
       float v[V];
-      load_f<V>(x + i, v);
+      load_f<V, EVEN>(x + p.i, v);
 #pragma unroll
       for (int k = 0; k < V; k++) m = max_nan(m, fabsf(v[k]));
     }
     q8_scale(row_max<TPR>(m, red), scale, inv);
-    for (int i = lane * V; i < a.dim; i += TPR * V) {
+    for (int c = lane * V; c < a.dim; c += TPR * V) {
+      const At p(c, a.dim);
       float v[V];
-      load_f<V>(x + i, v);
-      Pack<int8_t, V> o;
+      load_f<V, EVEN>(x + p.i, v);
+      typename PackOf<int8_t, V, EVEN>::type o;
 #pragma unroll
       for (int k = 0; k < V; k++) o.v[k] = q8(v[k], inv);
-      *reinterpret_cast<Pack<int8_t, V>*>(q + i) = o;
+      *reinterpret_cast<typename PackOf<int8_t, V, EVEN>::type*>(q + p.i) = o;
     }
   }
   if (lane == 0) a.scale[row] = scale;
 }
 
-template <typename T, int V, int TPR, int NV> __global__ __launch_bounds__(NT) void quantize_kernel(NormArgs a) {
+template <typename T, int V, bool EVEN, int TPR, int NV> __global__ __launch_bounds__(NT) void quantize_kernel(NormArgs a) {
   __shared__ float red[NT / 64];
-  SEQ_ROWS((quantize_row<T, V, TPR, NV>(a, row, red)))
+  SEQ_ROWS((quantize_row<T, V, EVEN, TPR, NV>(a, row, red)))
 }
 
 struct NormBwdArgs {
@@ -254,8 +284,9 @@ struct NormBwdArgs {
 
 // A workgroup takes rows blockIdx, blockIdx + gridDim, ...: the weight's gradient stays in registers
 // over all of them (a thread keeps its columns) and leaves as one row of `part`.
-template <typename T, typename R, int V, int TPR, int NV>
+template <typename T, typename R, int V, bool EVEN, int TPR, int NV>
 __global__ __launch_bounds__(NT) void norm_bwd_kernel(NormBwdArgs a) {
+  typedef Place<V, EVEN> At;
   constexpr int RPB = NT / TPR;
   __shared__ float red[2][NT / 64];
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
@@ -271,100 +302,104 @@ __global__ __launch_bounds__(NT) void norm_bwd_kernel(NormBwdArgs a) {
     const float rho = a.rstd[row];
     float dot = 0.f;
     auto pair = [&](int i, float (&g)[V], float (&n)[V]) {
-      load_f<V>(dy + i, g);
-      load_f<V>(s + i, n);
+      load_f<V, EVEN>(dy + i, g);
+      load_f<V, EVEN>(s + i, n);
 #pragma unroll
       for (int k = 0; k < V; k++) n[k] *= rho;
     };
     auto weigh = [&](int i, float (&g)[V]) {
       float w[V];
       if (!a.w) return;
-      load_f<V>(a.w + i, w);
+      load_f<V, EVEN>(a.w + i, w);
 #pragma unroll
       for (int k = 0; k < V; k++) g[k] *= w[k];
     };
     auto put = [&](int i, float mean, const float (&g)[V], const float (&n)[V]) {
       float d[V], b[V];
-      if (ds) load_f<V>(ds + i, b);
+      if (ds) load_f<V, EVEN>(ds + i, b);
 #pragma unroll
       for (int k = 0; k < V; k++) {
         d[k] = rho * (g[k] - n[k] * mean);
         if (ds) d[k] += b[k];
       }
-      store_f<V>(dx + i, d);
-      if (dr) store_f<V>(dr + i, d);
+      store_f<V, EVEN>(dx + i, d);
+      if (dr) store_f<V, EVEN>(dr + i, d);
     };
     if constexpr (NV > 0) {
       float g[NV][V], n[NV][V];
 #pragma unroll
       for (int j = 0; j < NV; j++) {
-        const int i = (j * TPR + lane) * V;
-        if (i < a.dim) pair(i, g[j], n[j]);
+        const At p((j * TPR + lane) * V, a.dim);
+        if (p.on) pair(p.i, g[j], n[j]);
         else
 #pragma unroll
           for (int k = 0; k < V; k++) g[j][k] = n[j][k] = 0.f;
       }
 #pragma unroll
       for (int j = 0; j < NV; j++) {
-        const int i = (j * TPR + lane) * V;
-        if (i >= a.dim) continue;
+        const At p((j * TPR + lane) * V, a.dim);
+        if (!p.on) continue;
 #pragma unroll
         for (int k = 0; k < V; k++) acc[j][k] += g[j][k] * n[j][k];
-        weigh(i, g[j]);
+        weigh(p.i, g[j]);
 #pragma unroll
-        for (int k = 0; k < V; k++) dot += g[j][k] * n[j][k];
+        for (int k = 0; k < V; k++) dot += p.once(k, g[j][k]) * p.once(k, n[j][k]);
       }
       const float mean = row_sum<TPR>(dot, red[flip]) * rdim;
       flip ^= 1;   // (the next row's sums may be written while a slow wave still reads this row's)
 #pragma unroll
       for (int j = 0; j < NV; j++) {
-        const int i = (j * TPR + lane) * V;
-        if (i < a.dim) put(i, mean, g[j], n[j]);
+        const At p((j * TPR + lane) * V, a.dim);
+        if (p.on) put(p.i, mean, g[j], n[j]);
       }
     } else {
-      for (int i = lane * V; i < a.dim; i += TPR * V) {
+      for (int c = lane * V; c < a.dim; c += TPR * V) {
+        const At p(c, a.dim);
         float g[V], n[V];
-        pair(i, g, n);
-        weigh(i, g);
+        pair(p.i, g, n);
+        weigh(p.i, g);
 #pragma unroll
-        for (int k = 0; k < V; k++) dot += g[k] * n[k];
+        for (int k = 0; k < V; k++) dot += p.once(k, g[k]) * p.once(k, n[k]);
       }
       const float mean = row_sum<TPR>(dot, red[flip]) * rdim;
       flip ^= 1;
-      for (int i = lane * V; i < a.dim; i += TPR * V) {
+      for (int c = lane * V; c < a.dim; c += TPR * V) {
+        const At p(c, a.dim);
         float g[V], n[V];
-        pair(i, g, n);
-        weigh(i, g);
-        put(i, mean, g, n);
+        pair(p.i, g, n);
+        weigh(p.i, g);
+        put(p.i, mean, g, n);
       }
     }
   }
   if constexpr (NV > 0) {
     if (!a.part) return;
-    if constexpr (RPB > 1) {   // the waves' sums of the same columns, in wave order
-      __shared__ float sh[RPB - 1][64 * V];
+    float* part = a.part + (int64_t)blockIdx.x * a.dim;
+    auto leave = [&](const At& p, const float (&sums)[V]) {   // (a column's sum is its owner's)
+#pragma unroll
+      for (int k = 0; k < V; k++)
+        if (p.on && p.own(k)) part[p.i + k] = sums[k];
+    };
+    if constexpr (RPB > 1) {   // the rows' sums of the same columns, in the order of their lanes
+      __shared__ float sh[RPB - 1][TPR * V];
 #pragma unroll
       for (int j = 0; j < NV; j++) {
         if (sub)
 #pragma unroll
           for (int k = 0; k < V; k++) sh[sub - 1][lane * V + k] = acc[j][k];
         __syncthreads();
-        const int i = (j * TPR + lane) * V;
-        if (!sub && i < a.dim) {
-#pragma unroll
+        if (!sub) {
+#pragma unroll 4
           for (int u = 0; u < RPB - 1; u++)
 #pragma unroll
             for (int k = 0; k < V; k++) acc[j][k] += sh[u][lane * V + k];
-          store_f<V>(a.part + (int64_t)blockIdx.x * a.dim + i, acc[j]);
+          leave(At((j * TPR + lane) * V, a.dim), acc[j]);
         }
         __syncthreads();
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < NV; j++) {
-        const int i = (j * TPR + lane) * V;
-        if (i < a.dim) store_f<V>(a.part + (int64_t)blockIdx.x * a.dim + i, acc[j]);
-      }
+      for (int j = 0; j < NV; j++) leave(At((j * TPR + lane) * V, a.dim), acc[j]);
     }
   }
 }
@@ -406,7 +441,8 @@ __global__ __launch_bounds__(1024) void column_sums_kernel(const float* part, in
   }
 }
 
-// ---- host: the variant by the row's length.  A wave for rows of up to 4 packs a lane, else a workgroup.
+// ---- host: the variant by the row's length.  The fewest lanes that hold a row with a pack each, from 8 on, then more
+// packs a lane.  (bf16, 200000 rows of 64 by whole waves, 8 of 64 lanes at work: 61 us.)
 struct RowPlan { int tpr, nv; };
 // workgroups of a launch: a launch holds fewer than 2^32 threads
 unsigned row_blocks(int64_t rows, int tpr) {
@@ -414,23 +450,39 @@ unsigned row_blocks(int64_t rows, int tpr) {
   return (unsigned)(n < (1 << 22) ? n : (1 << 22));
 }
 RowPlan plan_rows(int dim, int V) {
-  for (int nv = 1; nv <= 4; nv *= 2)
+  for (int tpr = 8; tpr <= 64; tpr *= 2)
+    if (dim <= tpr * V) return {tpr, 1};
+  for (int nv = 2; nv <= 4; nv *= 2)
     if (dim <= 64 * V * nv) return {64, nv};
   for (int nv = 2; nv <= 8; nv *= 2)
     if (dim <= NT * V * nv) return {NT, nv};
   return {NT, 0};
 }
+// elements a pack: 16 bytes of T, or one where a row has fewer
+int row_pack(int dim, int type) {
+  const int W = 16 / type_bytes(type);
+  return dim < W ? 1 : W;
+}
 
-template <typename F> int32_t by_plan(RowPlan p, F f) {
-  if (p.tpr == 64) {
-    if (p.nv == 1) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
-    if (p.nv == 2) return f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
-    return f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+template <int N> using Int = std::integral_constant<int, N>;
+// ALL false: rows of a few elements, one a lane
+template <bool ALL, typename F> int32_t by_plan(RowPlan p, F f) {
+  if constexpr (ALL) {
+    if (p.tpr == 16) return f(Int<16>(), Int<1>());
+    if (p.tpr == 32) return f(Int<32>(), Int<1>());
+    if (p.tpr == 64) {
+      if (p.nv == 1) return f(Int<64>(), Int<1>());
+      if (p.nv == 2) return f(Int<64>(), Int<2>());
+      return f(Int<64>(), Int<4>());
+    }
+    if (p.tpr == NT) {
+      if (p.nv == 2) return f(Int<NT>(), Int<2>());
+      if (p.nv == 4) return f(Int<NT>(), Int<4>());
+      if (p.nv == 8) return f(Int<NT>(), Int<8>());
+      return f(Int<NT>(), Int<0>());
+    }
   }
-  if (p.nv == 2) return f(std::integral_constant<int, NT>(), std::integral_constant<int, 2>());
-  if (p.nv == 4) return f(std::integral_constant<int, NT>(), std::integral_constant<int, 4>());
-  if (p.nv == 8) return f(std::integral_constant<int, NT>(), std::integral_constant<int, 8>());
-  return f(std::integral_constant<int, NT>(), std::integral_constant<int, 0>());
+  return f(Int<8>(), Int<1>());
 }
 
 // rows start on a pack's boundary
@@ -438,30 +490,31 @@ bool packs(const void* p, int64_t stride, int bytes, int V) {
   return !p || (aligned_to(p, (size_t)bytes * V) && stride % V == 0);
 }
 
-template <typename T, typename R, int V> int32_t launch_fwd(const NormArgs& a, hipStream_t st) {
+template <typename T, typename R, int V, bool EVEN> int32_t launch_fwd(const NormArgs& a, hipStream_t st) {
   const RowPlan p = plan_rows(a.dim, V);
   const unsigned grid = row_blocks(a.rows, p.tpr);
-  return by_plan(p, [&](auto tpr, auto nv) -> int32_t {
-    if (a.q) hipLaunchKernelGGL((norm_fwd_kernel<T, R, V, tpr, nv, true>), dim3(grid), dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((norm_fwd_kernel<T, R, V, tpr, nv, false>), dim3((unsigned)grid), dim3(NT), 0, st, a);
+  return by_plan<(V > 1)>(p, [&](auto tpr, auto nv) -> int32_t {
+    if (a.q) hipLaunchKernelGGL((norm_fwd_kernel<T, R, V, EVEN, tpr, nv, true>), dim3(grid), dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((norm_fwd_kernel<T, R, V, EVEN, tpr, nv, false>), dim3(grid), dim3(NT), 0, st, a);
     return pnp_check_launch("norm_fwd_kernel");
   });
 }
 
 template <typename T, typename R> int32_t run_fwd(const NormArgs& a, hipStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const bool wide = a.dim % V == 0 && packs(a.x, a.xs, sizeof(T), V) && packs(a.r, a.rs, sizeof(R), V) &&
+  if (a.dim < V) return launch_fwd<T, R, 1, true>(a, st);
+  const bool even = a.dim % V == 0 && packs(a.x, a.xs, sizeof(T), V) && packs(a.r, a.rs, sizeof(R), V) &&
                     packs(a.w, 0, 4, V) && packs(a.y, a.dim, sizeof(T), V) && packs(a.s, a.dim, sizeof(R), V) &&
                     packs(a.q, a.qs, 1, V);
-  return wide ? launch_fwd<T, R, V>(a, st) : launch_fwd<T, R, 1>(a, st);
+  return even ? launch_fwd<T, R, V, true>(a, st) : launch_fwd<T, R, V, false>(a, st);
 }
 
-// workgroups of the gradient: enough for the chip, few enough that their rows of `part` stay small
-// next to what they read (each takes 8 rows or more where there are that many)
+// workgroups of the gradient: one a CU, and more as long as their rows of `part` stay small next to what they read
+// (8 rows a thread, or more)
 int64_t bwd_blocks(int64_t rows, int tpr) {
   const int64_t per = NT / tpr;
-  const int64_t want = ceil_div(rows, per * 8);
-  return want < 1 ? 1 : want > 1024 ? 1024 : want;
+  const int64_t want = ceil_div(rows, per * 8), least = ceil_div(rows, per) < 256 ? ceil_div(rows, per) : 256;
+  return want < least ? least : want > 1024 ? 1024 : want;
 }
 constexpr int64_t DW_STRIPS = 64;   // row strips of norm_dw_kernel
 int64_t bwd_parts(int64_t rows, int dim, int V) {
@@ -469,11 +522,11 @@ int64_t bwd_parts(int64_t rows, int dim, int V) {
   return p.nv ? bwd_blocks(rows, p.tpr) : DW_STRIPS;
 }
 
-template <typename T, typename R, int V> int32_t launch_bwd(NormBwdArgs a, float* dw, hipStream_t st) {
+template <typename T, typename R, int V, bool EVEN> int32_t launch_bwd(NormBwdArgs a, float* dw, hipStream_t st) {
   const RowPlan p = plan_rows(a.dim, V);
   const int64_t grid = bwd_blocks(a.rows, p.tpr);
-  int32_t rc = by_plan(p, [&](auto tpr, auto nv) -> int32_t {
-    hipLaunchKernelGGL((norm_bwd_kernel<T, R, V, tpr, nv>), dim3((unsigned)grid), dim3(NT), 0, st, a);
+  int32_t rc = by_plan<(V > 1)>(p, [&](auto tpr, auto nv) -> int32_t {
+    hipLaunchKernelGGL((norm_bwd_kernel<T, R, V, EVEN, tpr, nv>), dim3((unsigned)grid), dim3(NT), 0, st, a);
     return pnp_check_launch("norm_bwd_kernel");
   });
   if (rc || !dw) return rc;
@@ -486,25 +539,28 @@ template <typename T, typename R, int V> int32_t launch_bwd(NormBwdArgs a, float
 
 template <typename T, typename R> int32_t run_bwd(const NormBwdArgs& a, float* dw, hipStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const bool wide = a.dim % V == 0 && packs(a.dy, a.dys, sizeof(T), V) && packs(a.s, a.ss, sizeof(R), V) &&
+  if (a.dim < V) return launch_bwd<T, R, 1, true>(a, dw, st);
+  const bool even = a.dim % V == 0 && packs(a.dy, a.dys, sizeof(T), V) && packs(a.s, a.ss, sizeof(R), V) &&
                     packs(a.ds, a.dss, sizeof(R), V) && packs(a.w, 0, 4, V) && packs(a.dx, a.dim, sizeof(T), V) &&
-                    packs(a.dres, a.dim, sizeof(R), V) && packs(a.part, a.dim, 4, V);
-  return wide ? launch_bwd<T, R, V>(a, dw, st) : launch_bwd<T, R, 1>(a, dw, st);
+                    packs(a.dres, a.dim, sizeof(R), V);
+  return even ? launch_bwd<T, R, V, true>(a, dw, st) : launch_bwd<T, R, V, false>(a, dw, st);
 }
 
 template <typename T> int32_t run_quantize(const NormArgs& a, hipStream_t st) {
   constexpr int W = 16 / sizeof(T);
-  auto go = [&](auto v) -> int32_t {
+  auto go = [&](auto v, auto even) -> int32_t {
     constexpr int V = decltype(v)::value;
+    constexpr bool EVEN = decltype(even)::value;
     const RowPlan p = plan_rows(a.dim, V);
     const unsigned grid = row_blocks(a.rows, p.tpr);
-    return by_plan(p, [&](auto tpr, auto nv) -> int32_t {
-      hipLaunchKernelGGL((quantize_kernel<T, V, tpr, nv>), dim3((unsigned)grid), dim3(NT), 0, st, a);
+    return by_plan<(V > 1)>(p, [&](auto tpr, auto nv) -> int32_t {
+      hipLaunchKernelGGL((quantize_kernel<T, V, EVEN, tpr, nv>), dim3(grid), dim3(NT), 0, st, a);
       return pnp_check_launch("quantize_kernel");
     });
   };
-  const bool wide = a.dim % W == 0 && packs(a.x, a.xs, sizeof(T), W) && packs(a.q, a.qs, 1, W);
-  return wide ? go(std::integral_constant<int, W>()) : go(std::integral_constant<int, 1>());
+  if (a.dim < W) return go(Int<1>(), std::true_type());
+  const bool even = a.dim % W == 0 && packs(a.x, a.xs, sizeof(T), W) && packs(a.q, a.qs, 1, W);
+  return even ? go(Int<W>(), std::true_type()) : go(Int<W>(), std::false_type());
 }
 
 bool rows_ok(int64_t rows, int dim) { return rows >= 0 && rows <= ((int64_t)1 << 40) && dim > 0 && dim <= (1 << 24); }
@@ -548,9 +604,7 @@ extern "C" int64_t pnp_rms_norm_bwd_workspace(const pnp_norm_bwd_desc* d) {
     return PNP_ERR_ARG;
   }
   if (!d->rows) return 0;
-  // whichever of the two loads the tensors' alignment leads to
-  const int64_t wide = bwd_parts(d->rows, d->dim, 16 / type_bytes(d->type)), one = bwd_parts(d->rows, d->dim, 1);
-  return (wide > one ? wide : one) * d->dim;
+  return bwd_parts(d->rows, d->dim, row_pack(d->dim, d->type)) * d->dim;
 }
 
 extern "C" int32_t pnp_rms_norm_bwd(const pnp_norm_bwd_desc* d, void* stream) {

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import seq_plain as P
+import test_seqops_gpu as T
 from test_seqops_gpu import S, Draw, dev, plain_scan, run_scan, scan_inputs   # noqa: F401  (S: the fixture)
 
 pytestmark = pytest.mark.gpu
@@ -141,14 +142,50 @@ def test_views_that_stand_for_their_negative(S):
         S.causal_conv_step(x[:, 0], torch._neg_view(st), w)
 
 
+# ---------------------------------------------------------------------------------- odd rows
+@pytest.mark.parametrize("dtype", T.TYPES, ids=T.ids)
+@pytest.mark.parametrize("rows,dim", [(5, 2), (70, 4), (3, 7), (300, 9), (33, 16), (5, 63), (40, 65), (9, 100), (130, 129), (2, 513),
+                                      (3, 1025), (2, 4095), (2, 8191), (2, 16401)])
+def test_rows_of_any_length(S, dtype, rows, dim):
+    """Rows by 8, 16, 32 and 64 lanes, a workgroup and in parts; whole packs of a row and not."""
+    T.test_norm_and_gradient(S, dtype, rows, dim)
+    T.test_norm_in_8_bits(S, dtype, rows, dim)
+
+
+@pytest.mark.parametrize("dtype", T.TYPES, ids=T.ids)
+@pytest.mark.parametrize("dim", [8, 24, 61, 512, 2050])
+def test_rows_that_begin_anywhere(S, dtype, dim):
+    """Columns cut out of wider tensors, from an odd one on, against copies: the same values, each written once or the same."""
+    d = Draw(dim)
+    wide_rows = [dev(d(37, dim + 5, dtype=dtype)) for _ in range(4)]
+    w = dev(1 + d(dim + 1))
+
+    def ops(x, r, dy, ds, w):
+        x, r, w = (t.detach().requires_grad_() for t in (x, r, w))
+        y, s = S.add_rms_norm(x, w, r)
+        back = torch.autograd.grad([y, s], [x, r, w], [dy, ds])
+        with torch.no_grad():
+            return [y, s, *back, *S.add_rms_norm_q8(x, w, r), *S.quantize_rows(x)]
+
+    got = ops(*[t[:, 3:3 + dim] for t in wide_rows], w[1:])
+    want = ops(*[t[:, 3:3 + dim].contiguous() for t in wide_rows], w[1:].clone())
+    for a, b in zip(got, want):       # (the sums of two variants: a few roundings, so a step of the output's type)
+        step = {torch.float32: 2.0 ** -20, torch.bfloat16: 2.0 ** -7, torch.float16: 2.0 ** -10, torch.int8: 0}[a.dtype]
+        a, b = a.double(), b.double()
+        assert ((a - b).abs() <= step * b.abs().clamp_min(b.abs().mean()) + (step == 0)).all()
+    for t, u in zip(wide_rows, [dev(v) for v in (lambda d: [d(37, dim + 5, dtype=dtype) for _ in range(4)])(Draw(dim))]):
+        assert torch.equal(t, u)      # what is around them is as it was
+
+
 # ---------------------------------------------------------------------------------- values
-def test_rows_with_infinity(S):
-    x = torch.randn(4, 64, device="cuda")
-    x[1, 5], x[2, 7], x[3] = float("inf"), float("nan"), 0
-    y, _ = S.add_rms_norm(x, torch.ones(64, device="cuda"))
+@pytest.mark.parametrize("dim,at", [(64, 5), (61, 58), (5, 0), (1003, 999), (20001, 19997)])
+def test_rows_with_infinity(S, dim, at):
+    x = torch.randn(4, dim, device="cuda")
+    x[1, at], x[2, dim // 2], x[3] = float("inf"), float("nan"), 0
+    y, _ = S.add_rms_norm(x, torch.ones(dim, device="cuda"))
     assert torch.isfinite(y[0]).all() and torch.isnan(y[2]).all() and not y[3].any()
-    assert torch.isnan(y[1, 5]) and not y[1, torch.arange(64) != 5].any()
-    q, s, _ = S.add_rms_norm_q8(x, torch.ones(64, device="cuda"))
+    assert torch.isnan(y[1, at]) and not y[1, torch.arange(dim) != at].any()
+    q, s, _ = S.add_rms_norm_q8(x, torch.ones(dim, device="cuda"))
     assert torch.isnan(s[1:3]).all() and s[3] == 0 and not q[1:].any()
 
 
