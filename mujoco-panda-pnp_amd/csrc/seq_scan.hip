@@ -45,7 +45,7 @@ struct ScanArgs {
   int dim, N, groups, per;       // per: channels of a group
   int tiles;                     // workgroups across a group's channels
   int nch;                       // chunks of the length
-  int64_t chunk;                 // tokens of a chunk, a multiple of the tile
+  int64_t chunk;                 // tokens of a chunk, a multiple of TR
   int64_t nck;                   // states kept a sequence: one each TR tokens
   const void *u, *delta, *z, *Bm, *Cm;
   int64_t ub, ut, db, dt, zb, zt, Bb, Bt, Cb, Ct;
@@ -71,29 +71,42 @@ template <int S> __device__ __forceinline__ Where where(const ScanArgs& a, int f
   return w;
 }
 
-// E neighbouring channels of one token; those past `left` as 0.  WIDE: packs of V are whole or past it,
-// and aligned.
+// E neighbouring channels of one token; those past `left` as 0.  WIDE: packs of V are whole or past it, and on their
+// boundaries; otherwise whole ones come from wherever they lie, the last channels one by one (by elements throughout,
+// bf16, 2 x 2048 x 2047 x 16: 127 us forward, 204 back).
 template <typename T, int E> struct Raw { T v[E]; };
 template <int E, bool WIDE, typename T> __device__ __forceinline__ void load_channels(const T* p, int left, Raw<T, E>& o) {
-  constexpr int V = !WIDE ? 1 : E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
+  constexpr int V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
 #pragma unroll
   for (int i = 0; i < E; i += V) {
-    Pack<T, V> w;
+    typename PackOf<T, V, WIDE>::type w;
 #pragma unroll
     for (int k = 0; k < V; k++) w.v[k] = (T)0.f;
-    if (i < left) w = *reinterpret_cast<const Pack<T, V>*>(p + i);
+    if constexpr (WIDE) {
+      if (i < left) w = *reinterpret_cast<const Pack<T, V>*>(p + i);
+    } else if (i + V <= left) {
+      w = *reinterpret_cast<const LoosePack<T, V>*>(p + i);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V - 1; k++)
+        if (i + k < left) w.v[k] = p[i + k];
+    }
 #pragma unroll
     for (int k = 0; k < V; k++) o.v[i + k] = w.v[k];
   }
 }
 template <int E, bool WIDE, typename T> __device__ __forceinline__ void store_channels(T* p, int left, const float (&v)[E]) {
-  constexpr int V = !WIDE ? 1 : E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
+  constexpr int V = E * (int)sizeof(T) > 16 ? 16 / (int)sizeof(T) : E;
 #pragma unroll
   for (int i = 0; i < E; i += V) {
     float w[V];
 #pragma unroll
     for (int k = 0; k < V; k++) w[k] = v[i + k];
-    if (i < left) store_f<V>(p + i, w);
+    if (WIDE ? i < left : i + V <= left) store_f<V, WIDE>(p + i, w);
+    else if (!WIDE && i < left)
+#pragma unroll
+      for (int k = 0; k < V; k++)
+        if (i + k < left) p[i + k] = from_f<T>(w[k]);
   }
 }
 
@@ -105,12 +118,13 @@ template <bool WIDE, typename T> __device__ __forceinline__ float4 load_states(c
     load_f<4>(p + n, v);
     return float4{v[0], v[1], v[2], v[3]};
   }
-  float4 r;
-  r.x = n < N ? to_f(p[n]) : 0.f;
-  r.y = n + 1 < N ? to_f(p[n + 1]) : 0.f;
-  r.z = n + 2 < N ? to_f(p[n + 2]) : 0.f;
-  r.w = n + 3 < N ? to_f(p[n + 3]) : 0.f;
-  return r;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (n + 4 <= N) load_f<4, false>(p + n, v);
+  else
+#pragma unroll
+    for (int i = 0; i < 3; i++)
+      if (n + i < N) v[i] = to_f(p[n + i]);
+  return float4{v[0], v[1], v[2], v[3]};
 }
 __device__ __forceinline__ void load_state4(const float* p, int n, int N, float (&h)[4]) {
 #pragma unroll
@@ -801,22 +815,30 @@ bool scan_ok(const pnp_scan_desc* d) {
          d->dim % d->groups == 0 && type_bytes(d->type) && d->B <= ((int64_t)1 << 31) && d->L <= ((int64_t)1 << 31);
 }
 
-// how a call is cut: chunks of the length where sequences and channels alone leave the chip idle
+// How a call is cut: chunks of the length where sequences and channels alone leave the chip idle, up to 1024
+// workgroups.  A chunk costs its tokens twice (about 0.18 us a token that a workgroup walks, and with two launches more
+// 10 us), so the fewer the workgroups the shorter it may be; the chain over the chunks costs 0.09 us each, which
+// weighs as much as the walk at 2 sqrt(L) of them.  Measured, forward and gradient, fp32, N 16, chunks of 128 at the
+// least / of 64 / 32 / 16: 1 x 1000 x 64 149 / 101 / 76 / 56 us, 4 x 192 x 128 122 / - / 50 / 40; with 128 and more
+// workgroups the other way: 32 x 100 x 256 (128) 79 / 79 / 81, 100 x 128 x 256 (400) 115 / - / 143 / 149.
 struct Plan { int S, tiles, nch; int64_t chunk, nck, blocks; };
 Plan plan(const pnp_scan_desc* d) {
   Plan p;
   p.S = lanes_of(d->N);
-  const int per = d->dim / d->groups, tt = 32;   // (a multiple of every tile)
+  const int per = d->dim / d->groups;
   p.tiles = (int)ceil_div(per, NT / p.S);
   const int64_t base = d->B * d->groups * p.tiles;
   int64_t nch = 1;
   if (base < 512) {
     nch = ceil_div(1024, base ? base : 1);
-    const int64_t most = d->L / (4 * tt);   // a chunk of 4 tiles at least
+    const int64_t most = d->L / (base <= 64 ? 16 : base <= 128 ? 64 : 128);
     if (nch > most) nch = most;
-    if (nch < 1) nch = 1;
+    while (nch * nch > 6 * d->L) nch = nch * 15 / 16;
+    if (nch < 3) nch = 1;   // (two chunks walk as many tokens one after the other as one)
   }
-  p.chunk = ceil_div(ceil_div(d->L ? d->L : 1, nch), tt) * tt;
+  p.chunk = ceil_div(d->L ? d->L : 1, nch);
+  const int tt = p.chunk > 16 ? 32 : 16;   // (whole tiles, but in the shortest)
+  p.chunk = ceil_div(p.chunk, tt) * tt;
   p.nch = (int)(d->L ? ceil_div(d->L, p.chunk) : 1);
   p.nck = ceil_div(d->L, TR);
   p.blocks = base * p.nch;

@@ -11,6 +11,13 @@ pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
 
 
+def near(a, b, steps):
+    """Steps of a 16-bit type, or of a few roundings in fp32: another variant of a kernel, its products fused otherwise."""
+    step = {torch.float32: 2.0 ** -20, torch.bfloat16: 2.0 ** -7, torch.float16: 2.0 ** -10}[a.dtype]
+    a, b = a.double(), b.double()
+    assert ((a - b).abs() <= steps * step * b.abs().clamp_min(b.abs().mean())).all()
+
+
 # ---------------------------------------------------------------------------------- autograd
 def test_second_gradients_are_refused(S):
     x, w = dev(Draw(1)(2, 9, 16), True), torch.ones(16, 4, device="cuda")
@@ -177,6 +184,33 @@ def test_rows_that_begin_anywhere(S, dtype, dim):
         assert torch.equal(t, u)      # what is around them is as it was
 
 
+# ---------------------------------------------------------------------------------- scans
+@pytest.mark.parametrize("dtype", T.TYPES, ids=T.ids)
+@pytest.mark.parametrize("B,L,D,N,G", [(1, 48, 8, 16, 1), (2, 50, 40, 16, 1), (1, 97, 10, 4, 1), (2, 300, 24, 3, 2), (1, 130, 66, 64, 2),
+                                       (3, 161, 7, 8, 1), (1, 900, 5, 32, 1)])
+def test_scans_cut_in_short_chunks(S, dtype, B, L, D, N, G):
+    T.test_scan_and_gradient(S, dtype, B, L, D, N, G)
+
+
+@pytest.mark.parametrize("dtype", T.TYPES, ids=T.ids)
+@pytest.mark.parametrize("D,N", [(64, 16), (37, 16), (70, 6), (130, 5)])
+def test_scans_of_channels_that_begin_anywhere(S, dtype, D, N):
+    """u, delta, z, B, C cut out of wider tensors, from an odd column on, against copies of them."""
+    d = Draw(D * N)
+    one = [dev(d(2, 75, D + 4, dtype=dtype)) for _ in range(4)]
+    two = [dev(d(2, 75, N + 3, dtype=dtype)) for _ in range(2)]
+    A = -dev(d(D, N).abs())
+
+    def ops(u, delta, z, dy, B, C):
+        v = [t.detach().requires_grad_() for t in (u, delta, z, B, C)]
+        o, last = S.selective_scan(v[0], v[1], A, v[3], v[4], z=v[2])
+        return [o, last, *torch.autograd.grad(o, v, dy)]
+
+    cut = [t[..., 3:3 + D] for t in one] + [t[..., 1:1 + N] for t in two]
+    for a, b in zip(ops(*cut), ops(*[t.contiguous() for t in cut])):
+        near(a, b, 1)
+
+
 # ---------------------------------------------------------------------------------- values
 @pytest.mark.parametrize("dim,at", [(64, 5), (61, 58), (5, 0), (1003, 999), (20001, 19997)])
 def test_rows_with_infinity(S, dim, at):
@@ -233,13 +267,6 @@ def tall():
 
 
 END = 70     # rows compared: a run of their own gives them too
-
-
-def near(a, b, steps):
-    """Steps of bf16, or of a few roundings in fp32: another variant of a kernel, its products fused otherwise."""
-    step = 2.0 ** -7 if a.dtype == BF else 2.0 ** -20
-    a, b = a.double(), b.double()
-    assert ((a - b).abs() <= steps * step * b.abs().clamp_min(b.abs().mean())).all()
 
 
 def test_offsets_past_32_bits_norm_and_product(S, tall):
