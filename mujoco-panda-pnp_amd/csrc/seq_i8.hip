@@ -26,17 +26,32 @@ struct I8Args {
   int wide;   // rows of out start on 16-byte boundaries
 };
 
-// 16 bytes of a row from k on, zeros past its K elements; any alignment
+// 16 bytes of a row, wherever they lie.  (Aligned words shifted into place, one more load and 4 instructions: 8191^3
+// 1014 against 732 us.)
+__device__ __forceinline__ v4i whole16(const int8_t* p) {
+  v4i v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+// the same from k on, zeros past the row's K: its end by the words that hold some of it, shifted into place (by bytes
+// the few rows of 64 x 1000 x 1001 took 12 us)
+typedef int __attribute__((may_alias)) word;
 __device__ __forceinline__ v4i load16(const int8_t* row, int k, int K) {
+  const int n = K - k;
+  if (n >= 16) return whole16(row + k);
   v4i v = {0, 0, 0, 0};
-  if (k + 16 <= K) {
-    __builtin_memcpy(&v, row + k, 16);
-  } else if (k < K) {
-    int w[4] = {0, 0, 0, 0};
+  if (n <= 0) return v;
+  const int8_t* p = row + k;
+  const int by = (int)((uintptr_t)p & 3);
+  const word* w = reinterpret_cast<const word*>(p - by);
+  int d[5];
 #pragma unroll
-    for (int i = 0; i < 16; i++)
-      if (k + i < K) w[i >> 2] |= (int)(uint8_t)row[k + i] << (8 * (i & 3));
-    v = v4i{w[0], w[1], w[2], w[3]};
+  for (int i = 0; i < 5; i++) d[i] = 4 * i < by + n ? w[i] : 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int left = n - 4 * i;   // bytes of word i that are the row's
+    v[i] = (int)__builtin_amdgcn_alignbyte((uint32_t)d[i + 1], (uint32_t)d[i], (uint32_t)by) &
+           (left >= 4 ? -1 : left <= 0 ? 0 : (1 << 8 * left) - 1);
   }
   return v;
 }
@@ -118,7 +133,8 @@ __device__ __forceinline__ int k_of(int g) { return g == 0 ? 0 : g == 1 ? 3 : g 
 // 64 lanes' chunks in a row, so the lane's global address carries the exchange; chunks past K come from `zeros`.  A
 // stage's operands are read into registers under the product of the stage before (a quarter of a wave's registers;
 // bf16 out, 8192^3 493 -> 477 us, 2048 x 2048 x 8192 50 -> 46 us, against reading them before their own product),
-// and its buffer is loaded anew, ST stages on, as soon as everybody has.  Otherwise two stages, by way of registers.
+// and its buffer is loaded anew, ST stages on, as soon as everybody has.  Otherwise two stages, by way of
+// registers that hold the next two.
 //
 // Bound by the matrix cores at the clock that the power leaves them: 8192^3 460 us, 2.4 POP/s (a large bf16 library
 // product reaches 1.2 PFLOP/s here; of the cycles at 2 GHz the matrix cores are busy 57 %).  Short sums by their output:
@@ -213,28 +229,41 @@ __global__ __launch_bounds__(64 * WGM* WGN, 2) void i8_tile_kernel(I8Args a) {
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the workgroup
   } else {
-    v4i rw[LW], rq[LQ];
-    auto fetch = [&](int s) {
+    struct Chunks { v4i w[LW], q[LQ]; } r0, r1;
+    auto fetch = [&](int s, Chunks& r) {
+      if ((s + 1) * BK <= a.K) {
 #pragma unroll
-      for (int i = 0; i < LW; i++) rw[i] = load16(pw[i], s * BK + cw[i], a.K);
+        for (int i = 0; i < LW; i++) r.w[i] = whole16(pw[i] + s * BK + cw[i]);
 #pragma unroll
-      for (int i = 0; i < LQ; i++) rq[i] = load16(pq[i], s * BK + cq[i], a.K);
+        for (int i = 0; i < LQ; i++) r.q[i] = whole16(pq[i] + s * BK + cq[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < LW; i++) r.w[i] = load16(pw[i], s * BK + cw[i], a.K);
+#pragma unroll
+        for (int i = 0; i < LQ; i++) r.q[i] = load16(pq[i], s * BK + cq[i], a.K);
+      }
     };
-    auto put = [&](int buf) {
+    auto put = [&](int buf, const Chunks& r) {
 #pragma unroll
-      for (int i = 0; i < LW; i++) sw[buf][i * NT + tid] = rw[i];
+      for (int i = 0; i < LW; i++) sw[buf][i * NT + tid] = r.w[i];
 #pragma unroll
-      for (int i = 0; i < LQ; i++) sq[buf][i * NT + tid] = rq[i];
+      for (int i = 0; i < LQ; i++) sq[buf][i * NT + tid] = r.q[i];
     };
-    fetch(0);
-    put(0);
-    for (int s = 0; s < nk; s++) {
-      __syncthreads();   // stage s is there, and everybody has read stage s - 1
-      if (s + 1 < nk) fetch(s + 1);
+    auto stage = [&](int s, Chunks& r) {   // r: stage s + 1, and then s + 3
       Operands f;
+      __syncthreads();   // stage s is there, and everybody has read stage s - 1
       read(s & 1, f);
       product(f);
-      if (s + 1 < nk) put((s + 1) & 1);
+      put((s + 1) & 1, r);
+      if (s + 3 < nk) fetch(s + 3, r);
+    };
+    fetch(0, r0);
+    if (nk > 1) fetch(1, r1);
+    put(0, r0);
+    if (nk > 2) fetch(2, r0);
+    for (int s = 0; s < nk; s += 2) {
+      stage(s, r1);
+      if (s + 1 < nk) stage(s + 1, r0);
     }
   }
   const int n = n0 + wn + fc * V;
