@@ -137,7 +137,7 @@ __device__ __forceinline__ int k_of(int g) { return g == 0 ? 0 : g == 1 ? 3 : g 
 // registers that hold the next two.
 //
 // Bound by the matrix cores at the clock that the power leaves them: 8192^3 460 us, 2.4 POP/s (a large bf16 library
-// product reaches 1.2 PFLOP/s here; of the cycles at 2 GHz the matrix cores are busy 57 %).  Short sums by their output:
+// product reaches 1.2 PFLOP/s here; the matrix cores are busy in 65 % of the cycles).  Short sums by their output:
 // 8192 x 1024 x 256 11 us, of which a launch of one tile 4.5 and the writing of 17 MB about 5.
 __device__ const v4i zeros[1] = {};
 
