@@ -184,6 +184,22 @@ def test_rows_that_begin_anywhere(S, dtype, dim):
         assert torch.equal(t, u)      # what is around them is as it was
 
 
+# ---------------------------------------------------------------------------------- products
+@pytest.mark.parametrize("M,N", [(1, 40), (19, 33), (40, 20), (64, 17), (70, 65), (300, 257), (1700, 1500), (3600, 3600)])
+def test_products_of_rows_that_begin_anywhere(S, M, N):
+    """Every alignment of both operands and ends of rows of every length, each variant; the sum is exact."""
+    g = torch.Generator().manual_seed(M * N)
+    q, w = (torch.randint(-128, 128, (n, 340), generator=g, dtype=torch.int8).cuda() for n in (M, N))
+    one, ones = torch.ones(M, device="cuda"), torch.ones(N, device="cuda")
+    for K, i, j in [(1, 0, 3), (5, 1, 1), (15, 2, 0), (16, 3, 2), (17, 0, 1), (63, 1, 2), (64, 16, 0), (65, 0, 0), (79, 3, 3), (127, 2, 1),
+                    (128, 0, 16), (130, 1, 0), (191, 0, 2), (192, 7, 9), (257, 0, 0), (300, 5, 4), (321, 1, 3)]:
+        a, b = q[:, i:i + K], w[:, j:j + K]
+        assert torch.equal(S.matmul_i8(a, one, b, ones).double(), a.double() @ b.double().t()), (K, i, j)
+        if M * N < 10 ** 6:    # rows a multiple of 16 apart, as quantize_rows leaves them
+            rows = (lambda t: torch.zeros(t.shape[0], (K + 15) // 16 * 16 + 16, dtype=torch.int8, device="cuda")[:, :K].copy_(t))
+            assert torch.equal(S.matmul_i8(rows(a), one, rows(b), ones).double(), a.double() @ b.double().t()), K
+
+
 # ---------------------------------------------------------------------------------- scans
 @pytest.mark.parametrize("dtype", T.TYPES, ids=T.ids)
 @pytest.mark.parametrize("B,L,D,N,G", [(1, 48, 8, 16, 1), (2, 50, 40, 16, 1), (1, 97, 10, 4, 1), (2, 300, 24, 3, 2), (1, 130, 66, 64, 2),
