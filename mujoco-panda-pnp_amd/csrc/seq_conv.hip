@@ -347,6 +347,7 @@ struct ConvStepArgs {
   const uint8_t* reset;
   void* y;
 };
+// One token: the state moves up by one in place.  Bound by memory: fp32, 8192 x 512, W 4, 21 us, 134 MB at 6.3 TB/s.
 template <typename T, int W, int V> __global__ __launch_bounds__(NT) void conv_step_kernel(ConvStepArgs a) {
   const int64_t packs = a.dim / V;
   for (int64_t id = (int64_t)blockIdx.x * NT + threadIdx.x; id < a.B * packs; id += (int64_t)gridDim.x * NT) {

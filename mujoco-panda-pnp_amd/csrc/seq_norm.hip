@@ -217,7 +217,7 @@ __global__ __launch_bounds__(NT) void norm_fwd_kernel(NormArgs a) {
   SEQ_ROWS((norm_fwd_row<T, R, V, EVEN, TPR, NV, Q8>(a, row, red)))
 }
 
-// rows in 8 bits: the norm's kernel without the norm
+// rows in 8 bits: the norm's kernel without the norm (bf16, 8192 x 1024: 7.8 us, 4.5 of it a launch's own)
 template <typename T, int V, bool EVEN, int TPR, int NV>
 __device__ __forceinline__ void quantize_row(const NormArgs& a, int64_t row, float (&red)[NT / 64]) {
   typedef Place<V, EVEN> At;

@@ -182,7 +182,13 @@ template <int S> __device__ __forceinline__ float token_sums(float (&q)[group_of
   return q[0];
 }
 
-// STATE: the chunk's state from a zero start and its decay alone
+// STATE: the chunk's state from a zero start and its decay alone.
+//
+// Bound by the VALU: exp2 and 4 instructions a state and token, and what a token costs a lane beyond (3 reads of LDS, the
+// sum over the channel's lanes) by its 4 states.  Bf16, 4 x 2048 x 2048 x 16: 84 us, the VALU busy in 89 % of the cycles
+// (268 M states and tokens: 10.7 lane instructions each, 8 by count), the chunks' states 60 us, 93 %.  Fp32, 512 x 33 x 512
+// x 16 with the states for the gradient: 74 us, 240 MB, 68 %.  Tiles whose waves share nothing, without barriers, take
+// as long.
 template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__(NT, fwd_waves(S, sizeof(T))) void scan_fwd_kernel(ScanArgs a) {
   constexpr int TT = tile_f(S, sizeof(T)), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S, G = group_of(S), U = E / 2;
   __shared__ float4 dd[TT][CW / 2];                                 // dt, dt u of two channels; then y in dt's place
@@ -399,7 +405,7 @@ template <int S> __device__ __forceinline__ void channel_sums(float (&v)[8]) {
   if (S < 2) v[0] += dpp<SEQ_DPP_XOR1>(v[0]);
 }
 
-// a chunk's adjoint from a zero end, and its decay
+// a chunk's adjoint from a zero end, and its decay: as the chunk's state, 64 us (VALU 88 %)
 template <typename T, int S, bool WIDE> __global__ __launch_bounds__(NT) void scan_adjoint_kernel(ScanBwdArgs a) {
   constexpr int TT = tile_f(S, sizeof(T)), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S, U = E / 2;
   const ScanArgs& f = a.f;
@@ -496,6 +502,11 @@ template <typename T, int S, bool WIDE> __global__ __launch_bounds__(NT) void sc
   if (ng == 0) f.dsum[w.row * f.dim + ch] = dsum;
 }
 
+// The gradient.  An inner tile's states are walked forward again from the one that was kept (keeping all would be 8 times
+// the memory traffic) and stay with their decays in registers for the way back; sums over the lanes of a channel (three a
+// token) and over the channels of a wave (8 a lane) are halved at each step.  Bound by the VALU, about 26 instructions a
+// state and token, at 2 waves a SIMD, which is what 8 tokens' states in registers leave (3 spill): bf16, 4 x 2048 x 2048 x
+// 16, 282 us, VALU 77 %; fp32, 512 x 33 x 512 x 16, 205 us, 66 % (33 tokens are 2 tiles of 16 and one of 1).
 template <typename T, int S, bool WIDE> __global__ __launch_bounds__(NT, 2) void scan_bwd_kernel(ScanBwdArgs a) {
   constexpr int TT = tile_b(S), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S, G = group_of(S);
   const ScanArgs& f = a.f;
