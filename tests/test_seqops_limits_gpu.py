@@ -209,6 +209,13 @@ def test_scans_cut_in_short_chunks(S, dtype, B, L, D, N, G):
 
 
 @pytest.mark.parametrize("dtype", T.TYPES, ids=T.ids)
+@pytest.mark.parametrize("B,L,D,N,G", [(2101, 3, 8, 16, 1), (1100, 18, 6, 4, 2), (700, 1, 250, 16, 1)])
+def test_scans_of_many_sequences(S, dtype, B, L, D, N, G):
+    """More than the chip holds at once: a workgroup takes several."""
+    T.test_scan_and_gradient(S, dtype, B, L, D, N, G)
+
+
+@pytest.mark.parametrize("dtype", T.TYPES, ids=T.ids)
 @pytest.mark.parametrize("D,N", [(64, 16), (37, 16), (70, 6), (130, 5)])
 def test_scans_of_channels_that_begin_anywhere(S, dtype, D, N):
     """u, delta, z, B, C cut out of wider tensors, from an odd column on, against copies of them."""
