@@ -35,7 +35,9 @@ constexpr int NT = 256;
 constexpr int tile_f(int S, int bytes) {   // 4 or 8 channels a thread: registers for 4 waves a SIMD
   return S == 1 ? 8 : S == 2 ? (bytes == 4 ? 8 : 16) : S == 4 ? (bytes == 4 ? 16 : 32) : 32;
 }
-constexpr int tile_b(int S) { return S == 1 ? 8 : 16; }
+// (N 5 .. 8, fp32: 16 tokens spill, 512 x 33 x 512 x 8 forward and gradient 195 us against 165; bf16, 4 x 2048 x 2048 x 8,
+// 305 against 313 the other way.  N 16, fp32 and bf16: 271 and 471 us by 16 tokens, 279 and 502 by 8.)
+constexpr int tile_b(int S, int bytes) { return S == 1 || (S == 2 && bytes == 4) ? 8 : 16; }
 constexpr int TR = 8;
 // waves a SIMD that the forward is built for: what its registers allow without spills
 constexpr int fwd_waves(int S, int bytes) { return S >= 8 || (S == 1 && bytes == 4) ? 3 : 4; }
@@ -508,7 +510,7 @@ template <typename T, int S, bool WIDE> __global__ __launch_bounds__(NT) void sc
 // state and token, at 2 waves a SIMD, which is what 8 tokens' states in registers leave (3 spill): bf16, 4 x 2048 x 2048 x
 // 16, 282 us, VALU 77 %; fp32, 512 x 33 x 512 x 16, 205 us, 66 % (33 tokens are 2 tiles of 16 and one of 1).
 template <typename T, int S, bool WIDE> __global__ __launch_bounds__(NT, 2) void scan_bwd_kernel(ScanBwdArgs a) {
-  constexpr int TT = tile_b(S), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S, G = group_of(S);
+  constexpr int TT = tile_b(S, sizeof(T)), CW = NT / S, E = TT / S, RT = CW / E, NP = 4 * S, G = group_of(S);
   const ScanArgs& f = a.f;
   __shared__ float4 dd[TT][CW];                        // dt, dy, u, dt u; then dt, dy, sum g B, sum g (a h') A
   __shared__ float yb[TT][CW];                         // sum C h
