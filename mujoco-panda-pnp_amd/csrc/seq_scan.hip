@@ -377,6 +377,7 @@ struct ScanBwdArgs {
   void *du, *ddelta, *dz, *dB, *dC;
   float *dA, *dD, *dbias, *dstate;
   float* part;    // [B * nch][dim * N + 2 dim]: dA, dD, ddelta_bias of a chunk
+  float* strips;  // [sum_strips(B * nch)][dim * N + 2 dim]
   float* bc;      // [tiles][B * L][groups][2][4 S]: dB, dC of a workgroup's channels
 };
 
@@ -731,11 +732,10 @@ template <typename T> __global__ __launch_bounds__(NT) void scan_bc_kernel(const
   }
 }
 
-// dA, dD, ddelta_bias from the chunks' rows
-__global__ __launch_bounds__(1024) void scan_sums_kernel(const float* part, int64_t rows, int dim, int N, float* dA, float* dD, float* dbias) {
+// sums of 64 columns of part[rows][cols], the rows dealt to 16 waves and joined in wave order; in wave 0
+__device__ __forceinline__ float rows_sum(const float* part, int64_t rows, int64_t cols, int64_t c) {
   __shared__ float sh[16][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t cols = (int64_t)dim * (N + 2), c = (int64_t)blockIdx.x * 64 + lane;
   float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
   if (c < cols) {
     int64_t r = w;
@@ -750,14 +750,29 @@ __global__ __launch_bounds__(1024) void scan_sums_kernel(const float* part, int6
   }
   sh[w][lane] = (s0 + s1) + (s2 + s3);
   __syncthreads();
-  if (w || c >= cols) return;
   float s = 0.f;
+  if (!w)
 #pragma unroll
-  for (int i = 0; i < 16; i++) s += sh[i][lane];
+    for (int i = 0; i < 16; i++) s += sh[i][lane];
+  return s;
+}
+
+// dA, dD, ddelta_bias from the chunks' rows
+__global__ __launch_bounds__(1024) void scan_sums_kernel(const float* part, int64_t rows, int dim, int N, float* dA, float* dD, float* dbias) {
+  const int64_t cols = (int64_t)dim * (N + 2), c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const float s = rows_sum(part, rows, cols, c);
+  if (threadIdx.x >= 64 || c >= cols) return;
   const int64_t na = (int64_t)dim * N;
   if (c < na) dA[c] = s;
   else if (c < na + dim) { if (dD) dD[c - na] = s; }
   else if (dbias) dbias[c - na - dim] = s;
+}
+// many rows first in strips of STRIP (40944 rows of 550: by the few workgroups of all rows 540 us)
+constexpr int64_t STRIP = 512;
+__global__ __launch_bounds__(1024) void scan_strips_kernel(const float* part, int64_t rows, int64_t cols, float* out) {
+  const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63), r = blockIdx.y * STRIP;
+  const float s = rows_sum(part + r * cols, rows - r < STRIP ? rows - r : STRIP, cols, c);
+  if (threadIdx.x < 64 && c < cols) out[blockIdx.y * cols + c] = s;
 }
 
 // One token: a lane holds 4 states of a channel, a workgroup NT / S channels of one sequence (so that the
@@ -857,6 +872,8 @@ Plan plan(const pnp_scan_desc* d) {
   p.blocks = base * p.nch;
   return p;
 }
+// strips that the sums over rows are taken in first: none for few rows, at most 2^15 (the launch's second dimension)
+int64_t sum_strips(int64_t rows) { return rows > 2 * STRIP && rows <= STRIP << 15 ? ceil_div(rows, STRIP) : 0; }
 int64_t split_floats(const pnp_scan_desc* d, const Plan& p) {
   return p.nch > 1 ? d->B * p.nch * d->dim * (int64_t)(4 * p.S + 1) : 0;
 }
@@ -942,8 +959,15 @@ template <typename T, int S> int32_t run_scan_bwd(ScanBwdArgs a, int64_t blocks,
                        (T*)a.dB, (T*)a.dC);
     if (const int32_t rc = pnp_check_launch("scan_bc_kernel")) return rc;
   }
-  hipLaunchKernelGGL(scan_sums_kernel, dim3((unsigned)ceil_div((int64_t)f.dim * (f.N + 2), 64)), dim3(1024), 0, st, a.part, f.B * f.nch, f.dim,
-                     f.N, a.dA, a.dD, a.dbias);
+  const int64_t cols = (int64_t)f.dim * (f.N + 2), part_rows = f.B * f.nch, strips = sum_strips(part_rows);
+  const float* part = a.part;
+  if (strips) {
+    hipLaunchKernelGGL(scan_strips_kernel, dim3((unsigned)ceil_div(cols, 64), (unsigned)strips), dim3(1024), 0, st, part, part_rows, cols, a.strips);
+    if (const int32_t rc = pnp_check_launch("scan_strips_kernel")) return rc;
+    part = a.strips;
+  }
+  hipLaunchKernelGGL(scan_sums_kernel, dim3((unsigned)ceil_div(cols, 64)), dim3(1024), 0, st, part, strips ? strips : part_rows, f.dim, f.N, a.dA,
+                     a.dD, a.dbias);
   return pnp_check_launch("scan_sums_kernel");
 }
 
@@ -1042,7 +1066,7 @@ extern "C" int64_t pnp_scan_bwd_workspace(const pnp_scan_bwd_desc* d) {
   }
   const pnp_scan_desc& f = d->f;
   const Plan p = plan(&f);
-  return split_floats(&f, p) + f.B * p.nch * f.dim * (int64_t)(f.N + 2) + p.tiles * f.B * f.L * f.groups * (int64_t)(8 * p.S);
+  return split_floats(&f, p) + (f.B * p.nch + sum_strips(f.B * p.nch)) * f.dim * (int64_t)(f.N + 2) + p.tiles * f.B * f.L * f.groups * (int64_t)(8 * p.S);
 }
 
 extern "C" int32_t pnp_selective_scan_bwd(const pnp_scan_bwd_desc* d, void* stream) {
@@ -1078,7 +1102,8 @@ extern "C" int32_t pnp_selective_scan_bwd(const pnp_scan_bwd_desc* d, void* stre
   a.du = d->du; a.ddelta = d->ddelta; a.dz = d->dz; a.dB = d->dB; a.dC = d->dC;
   a.dA = d->dA; a.dD = d->dD; a.dbias = d->ddelta_bias; a.dstate = d->dstate;
   a.part = d->workspace + split_floats(&f, p);
-  a.bc = a.part + f.B * p.nch * f.dim * (int64_t)(f.N + 2);
+  a.strips = a.part + f.B * p.nch * f.dim * (int64_t)(f.N + 2);
+  a.bc = a.strips + sum_strips(f.B * p.nch) * f.dim * (int64_t)(f.N + 2);
   if (!f.B) {
     hipLaunchKernelGGL(scan_sums_kernel, dim3((unsigned)ceil_div((int64_t)f.dim * (f.N + 2), 64)), dim3(1024), 0, st, (const float*)nullptr,
                        (int64_t)0, f.dim, f.N, a.dA, a.dD, a.dbias);
