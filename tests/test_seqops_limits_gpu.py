@@ -209,7 +209,8 @@ def test_scans_cut_in_short_chunks(S, dtype, B, L, D, N, G):
 
 
 @pytest.mark.parametrize("dtype", T.TYPES, ids=T.ids)
-@pytest.mark.parametrize("B,L,D,N,G", [(2101, 3, 8, 16, 1), (1100, 18, 6, 4, 2), (700, 1, 250, 16, 1)])
+@pytest.mark.parametrize("B,L,D,N,G", [(2101, 3, 8, 16, 1), (1100, 18, 6, 4, 2), (700, 1, 250, 16, 1), (2300, 8, 5, 7, 1), (4099, 2, 9, 2, 1),
+                                       (1030, 16, 20, 40, 2)])
 def test_scans_of_many_sequences(S, dtype, B, L, D, N, G):
     """More than the chip holds at once: a workgroup takes several."""
     T.test_scan_and_gradient(S, dtype, B, L, D, N, G)
