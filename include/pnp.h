@@ -528,9 +528,10 @@ int32_t pnp_env_evaluate_f64(pnp_model* model, const pnp_state_f64* state, const
 
 /* s = x + residual (x alone where residual is NULL), held in res_type; rho = 1 / sqrt(mean(s^2) + eps);
  * y = s * rho * weight.  rows x dim.  Forward writes s (may be NULL without a residual), rstd = rho
- * [rows] (may be NULL) and y (type `type`), or, where q is given instead of y, q = rint(y / scale) in
- * 8 bits with scale = max|y| / 127 per row (0 for a row of zeros; NaN, with q = 0, for a row that holds
- * NaN or infinity).  weight NULL: ones. */
+ * [rows] (may be NULL) and y (type `type`), or, where q is given instead of y, q = rint(y / scale), the
+ * fp32 quotient rounded to nearest even, in 8 bits with scale = max|y| / 127 per row (0, with q = 0, where
+ * that is below the least normal fp32, as in a row of zeros; NaN, with q = 0, for a row that holds NaN or
+ * infinity).  weight NULL: ones. */
 typedef struct pnp_norm_desc {
   int64_t rows;
   int32_t dim, type, res_type;

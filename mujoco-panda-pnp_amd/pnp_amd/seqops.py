@@ -82,8 +82,9 @@ def add_rms_norm(x, weight, residual=None, eps=1e-6):
 
 def add_rms_norm_q8(x, weight, residual=None, eps=1e-6):
     """``add_rms_norm`` with its output in 8 bits: returns ``(q, scale, s)``, ``y ~ q * scale[..., None]``
-    with ``scale = max|y| / 127`` of the row (0 for a row of zeros; NaN, and q 0, where the row holds
-    infinity or NaN) and q rounded to nearest even from the unrounded y.  For serving: no gradient."""
+    with ``scale = max|y| / 127`` of the row (0, and q 0, where that is below the least normal fp32, as in a
+    row of zeros; NaN, and q 0, where the row holds infinity or NaN) and q the fp32 quotient ``y / scale`` of
+    the unrounded y, rounded to nearest even.  For serving: no gradient."""
     return _ext.add_rms_norm_q8(x, weight, residual, eps)
 
 

@@ -416,3 +416,54 @@ def test_captured_steps_carry_their_states(S):
         for s, m in zip(sets, mirror):
             want = step(*m)
             assert torch.equal(s[4], want) and torch.equal(s[1], m[1]) and torch.equal(s[2], m[2]), k
+
+
+# ---------------------------------------------------------------------------------- 8 bits next to halves
+def halves(rows, dim, dtype, g):
+    """Rows whose values lie on both sides of the halves between two steps of 8 bits, up to two steps of fp32 away."""
+    top = (torch.rand(rows, 1, generator=g) * 3 + 0.5).to(dtype).float()
+    x = ((torch.randint(0, 127, (rows, dim), generator=g) + 0.5) * (top / 127)).to(dtype)
+    if dtype == torch.float32:
+        x = x.view(torch.int32).add(torch.randint(-2, 3, (rows, dim), generator=g, dtype=torch.int32)).view(torch.float32)
+    x = x * torch.where(torch.rand(rows, dim, generator=g) < 0.5, -1, 1).to(dtype)
+    x[:, dim // 2] = top[:, 0].to(dtype)
+    return x
+
+
+@pytest.mark.parametrize("dtype", T.TYPES, ids=T.ids)
+@pytest.mark.parametrize("dim", [3, 40, 64, 333, 1024, 2047, 9000, 20001])
+def test_8_bits_are_the_rounded_quotient(S, dtype, dim):
+    """q is the fp32 quotient by the scale rounded to nearest even, next to halves too (the product with 1 / scale is not)."""
+    x = halves(max(300, 200000 // dim), dim, dtype, torch.Generator().manual_seed(dim))
+    q, scale = S.quantize_rows(dev(x))
+    top = x.float().abs().amax(1) / 127
+    assert torch.equal(scale.cpu(), top)
+    assert torch.equal(q.cpu(), torch.round(x.float() / top[:, None]).to(torch.int8))
+
+
+@pytest.mark.parametrize("rows,dim", [(8192, 2048), (60000, 256), (900, 20001)])
+def test_8_bits_of_the_norm_are_the_rounded_quotient(S, rows, dim):
+    """fp32: y as it is before 8 bits is the norm's own output (the same arithmetic)."""
+    x, w = torch.randn(rows, dim, device="cuda"), 1 + 0.1 * torch.randn(dim, device="cuda")
+    with torch.no_grad():
+        y, _ = S.add_rms_norm(x, w)
+        q, scale, _ = S.add_rms_norm_q8(x, w)
+    y, scale = y.cpu(), scale.cpu()
+    assert torch.equal(scale, y.abs().amax(1) / 127)
+    assert torch.equal(q.cpu(), torch.round(y / scale[:, None]).to(torch.int8))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF], ids=T.ids)
+def test_8_bits_of_small_rows(S, dtype):
+    """Down to the least normal scale, and 0 below it.  A power of two changes the scale and nothing else, but for fp32
+    at 2^-118: scales there begin at 2^-126, and half of such a one is below the normal numbers, where x itself is rounded
+    (spacing 2^-149).  So the rounded quotient of what x is decides."""
+    x = halves(700, 333, dtype, torch.Generator().manual_seed(1))
+    _, scale = S.quantize_rows(x.cuda())
+    for e in (-50, -70, -100, -118):
+        x2 = x * 2.0 ** e
+        q2, s2 = S.quantize_rows(x2.cuda())
+        assert torch.equal(s2, scale * 2.0 ** e), e
+        assert torch.equal(q2.cpu(), torch.round(x2.float() / s2.cpu()[:, None]).to(torch.int8)), e
+    q2, s2 = S.quantize_rows(x.cuda() * 2.0 ** -122)
+    assert not q2.any() and not s2.any()
