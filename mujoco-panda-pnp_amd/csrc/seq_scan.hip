@@ -265,14 +265,18 @@ template <typename T, int S, bool STATE, bool WIDE> __global__ __launch_bounds__
         if (ANY && k >= n) break;
         const float2 d = reinterpret_cast<const float2*>(dd[p + k])[mine2];
         const float4 b = sB[p + k][ng];
-        if (ANY && (bits >> (p + k) & 1)) {
-          h[0] = h[1] = h[2] = h[3] = 0.f;
+        if (ANY && (bits >> (p + k) & 1)) {   // (without the product with its decay, which may be infinity: 0 times that is NaN)
+          h[0] = d.y * b.x;
+          h[1] = d.y * b.y;
+          h[2] = d.y * b.z;
+          h[3] = d.y * b.w;
           if (STATE) dsum = __builtin_nanf("");
+        } else {
+          h[0] = exp2_f(d.x * A2[0]) * h[0] + d.y * b.x;
+          h[1] = exp2_f(d.x * A2[1]) * h[1] + d.y * b.y;
+          h[2] = exp2_f(d.x * A2[2]) * h[2] + d.y * b.z;
+          h[3] = exp2_f(d.x * A2[3]) * h[3] + d.y * b.w;
         }
-        h[0] = exp2_f(d.x * A2[0]) * h[0] + d.y * b.x;
-        h[1] = exp2_f(d.x * A2[1]) * h[1] + d.y * b.y;
-        h[2] = exp2_f(d.x * A2[2]) * h[2] + d.y * b.z;
-        h[3] = exp2_f(d.x * A2[3]) * h[3] + d.y * b.w;
         if (STATE) {
           dsum += d.x;
         } else {
@@ -809,12 +813,14 @@ template <typename T, int S, bool W4, bool STREAM> __global__ __launch_bounds__(
     const float4 bm = load_states<W4>((const T*)a.Bm + b * a.Bb + (int64_t)g * a.N, 4 * ng, a.N);
     const float4 cm = load_states<W4>((const T*)a.Cm + b * a.Cb + (int64_t)g * a.N, 4 * ng, a.N);
     const float dt = softplus_f(raw), dtu = dt * uv;
-    if (a.starts && a.starts[b]) h[0] = h[1] = h[2] = h[3] = 0.f;
+    const bool begins = a.starts && a.starts[b];
+    if (begins) h[0] = h[1] = h[2] = h[3] = 0.f;
     const float bv[4] = {bm.x, bm.y, bm.z, bm.w}, cv[4] = {cm.x, cm.y, cm.z, cm.w};
     float y = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      h[i] = exp2_f(dt * (A2[i] * SEQ_LOG2E)) * h[i] + dtu * bv[i];
+      const float e = exp2_f(dt * (A2[i] * SEQ_LOG2E));
+      h[i] = (begins ? 0.f : e) * h[i] + dtu * bv[i];   // (a decay may be infinity: 0 times that is NaN)
       y += cv[i] * h[i];
     }
     y = group_sum<S>(y);

@@ -467,3 +467,27 @@ def test_8_bits_of_small_rows(S, dtype):
         assert torch.equal(q2.cpu(), torch.round(x2.float() / s2.cpu()[:, None]).to(torch.int8)), e
     q2, s2 = S.quantize_rows(x.cuda() * 2.0 ** -122)
     assert not q2.any() and not s2.any()
+
+
+# ---------------------------------------------------------------------------------- starts of growing states
+@pytest.mark.parametrize("dtype", T.TYPES, ids=T.ids)
+@pytest.mark.parametrize("L,N", [(40, 4), (40, 16), (900, 8)])
+def test_a_start_whose_decay_outgrows_fp32(S, dtype, L, N):
+    """exp(dt A) = exp(12 * 10) at the starts: its place is taken by 0, not by a product with a state of 0."""
+    d = Draw(L + N)
+    v = scan_inputs(d, 2, L, 24, N, 1, dtype)
+    v["A"], v["bias"] = torch.full((24, N), 10.0), None
+    v["starts"] = d.starts(2, L, p=0.05)
+    v["starts"][:, 0] = 1
+    v["delta"] = torch.where(v["starts"][..., None] != 0, 12.0, -9.0).expand(2, L, 24).to(dtype).contiguous()
+    T.check_scan(S, v, d, dtype)
+    for t in (0, L // 2):      # one token at a time, each the start of a sequence
+        g = {k: dev(x) for k, x in v.items()}
+        h = g["state"].clone()
+        y = S.selective_scan_step(g["u"][:, t], h, torch.full_like(g["u"][:, t], 12.0), g["A"], g["B"][:, t], g["C"][:, t],
+                                  reset=torch.ones(2, dtype=torch.bool, device="cuda"))
+        one = {k: x if k in ("A", "state") else None if x is None or k in ("D", "z") else x[:, t:t + 1] for k, x in v.items()}
+        one["delta"], one["starts"] = torch.full_like(one["u"], 12.0), torch.ones(2, 1, dtype=torch.uint8)
+        ro, rl, eo, el = plain_scan(one)
+        P.close(y[:, None], ro, eo, 1, "out")
+        P.close(h, rl, el, 1, "state")
