@@ -129,8 +129,16 @@ Tensor value(const MaybeTensor& t) { return t ? *t : Tensor(); }
 
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants(const MaybeTensor& t) { return t && wants(*t); }
+// the operators have gradients and no derivative forward: a tangent is refused, not dropped
+bool tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool tangent(const MaybeTensor& t) { return t && tangent(*t); }
+template <typename... Ts> void backward_only(const char* name, const Ts&... ts) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(tangent(ts) || ...) || !c10::AutogradState::get_tls_state().get_fw_grad_mode(), name,
+                              " has no forward-mode derivative");
+}
 template <typename... Ts> bool training(const Ts&... ts) { return at::GradMode::is_enabled() && (wants(ts) || ...); }
 template <typename... Ts> void serving(const char* name, const Ts&... ts) {
+  backward_only(name, ts...);
   TORCH_CHECK_VALUE(!training(ts...), name, " has no gradient: call it under torch.no_grad()");
 }
 
@@ -208,6 +216,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
     return {o.y, o.s};   // without a residual s is x: the stream goes on through here, one rounding of dx + ds
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    backward_only("add_rms_norm", grads[0], grads[1]);
     const auto saved = ctx->get_saved_variables();
     const Tensor &s0 = saved[0], &w = saved[1], &rstd = saved[2];
     const ScalarType type = (ScalarType)ctx->saved_data["type"].toInt();
@@ -261,6 +270,7 @@ NormIn norm_in(const Tensor& x, const MaybeTensor& w, const MaybeTensor& r, doub
 }
 
 std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& residual, double eps) {
+  backward_only("add_rms_norm", x, weight, residual);
   const NormIn in = norm_in(x, weight, residual, eps);
   if (training(x, in.w, in.r)) {
     const variable_list o = NormFn::apply(x, maybe(in.r), in.w, eps);
@@ -375,6 +385,7 @@ struct ConvFn : torch::autograd::Function<ConvFn> {
     return {y, last};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    backward_only("causal_conv", grads[0], grads[1]);
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &starts = saved[3], &state = saved[4];
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(6);
@@ -411,6 +422,7 @@ bool is_silu(const c10::optional<std::string>& a) {
 
 std::tuple<Tensor, Tensor> causal_conv(const Tensor& x_, const Tensor& weight, const MaybeTensor& bias, const c10::optional<std::string>& act,
                                        const MaybeTensor& starts_, const MaybeTensor& state_) {
+  backward_only("causal_conv", x_, weight, bias, state_);
   activation(x_, "x");
   dims(x_, "x", 3);
   channels(x_, "x");
@@ -536,6 +548,7 @@ struct ScanFn : torch::autograd::Function<ScanFn> {
     return {o.out, o.last};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    backward_only("selective_scan", grads[0], grads[1]);
     if (!grads[0].defined() && !grads[1].defined()) return variable_list(10);
     const auto s = ctx->get_saved_variables();
     const ScanIn v{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]};
@@ -570,6 +583,7 @@ void state32(const Tensor& s, at::IntArrayRef want, const Tensor& like) {
 std::tuple<Tensor, Tensor> selective_scan(const Tensor& u, const Tensor& delta, const Tensor& A, const Tensor& B, const Tensor& C,
                                           const MaybeTensor& D, const MaybeTensor& z, const MaybeTensor& bias, const MaybeTensor& starts_,
                                           const MaybeTensor& state_) {
+  backward_only("selective_scan", u, delta, A, B, C, D, z, bias, state_);
   const ScanIn v = scan_in(u, delta, A, B, C, D, z, bias, 2);
   const Tensor starts = marks(starts_, "starts", u.sizes().slice(0, 2), u);
   Tensor state;

@@ -25,6 +25,9 @@ included).  Sequences of different lengths go padded on the left, with a start a
 packed sequences go one after the other in a row.  Padding is a sequence of its own, with outputs of its
 own: where weights are trained it holds finite values, since a gradient of zero times NaN is NaN.
 
+Derivatives are reverse-mode gradients, once: a second gradient is an error, and so is an input with a
+forward-mode tangent (``NotImplementedError``).
+
 A captured graph may hold any call, its backward pass too; as everywhere in torch, no eager graph of the
 same leaves may live while a backward pass is captured (capture over detached copies of the leaves, or
 after the eager graphs are gone).

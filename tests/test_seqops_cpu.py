@@ -238,3 +238,32 @@ def test_serving_calls_refuse_gradients():
                  lambda: S.selective_scan_step(x, x, x, x, x, x)):
         with pytest.raises(ValueError, match="no gradient"):
             call()
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent is never dropped: the operators have gradients, and no derivative forward."""
+    import torch.autograd.forward_ad as fwad
+    from pnp_amd import seqops as S
+    x, w, A = torch.zeros(2, 3, 8), torch.ones(8, 4), -torch.ones(8, 4)
+    B, h, i8 = torch.zeros(2, 3, 4), torch.zeros(2, 8, 4), torch.zeros(2, 8, dtype=torch.int8)
+    with fwad.dual_level():
+        dual = lambda t: fwad.make_dual(t, torch.ones_like(t))   # noqa: E731
+        for call in (lambda: S.add_rms_norm(dual(x), w[:, 0]), lambda: S.add_rms_norm(x, dual(w[:, 0])),
+                     lambda: S.add_rms_norm(x, w[:, 0], dual(x)), lambda: S.causal_conv(dual(x), w), lambda: S.causal_conv(x, dual(w)),
+                     lambda: S.causal_conv(x, w, dual(w[:, 0])), lambda: S.causal_conv(x, w, state=dual(x)),
+                     lambda: S.selective_scan(dual(x), x, A, B, B), lambda: S.selective_scan(x, dual(x), A, B, B),
+                     lambda: S.selective_scan(x, x, dual(A), B, B), lambda: S.selective_scan(x, x, A, dual(B), B),
+                     lambda: S.selective_scan(x, x, A, B, dual(B)), lambda: S.selective_scan(x, x, A, B, B, D=dual(w[:, 0])),
+                     lambda: S.selective_scan(x, x, A, B, B, z=dual(x)), lambda: S.selective_scan(x, x, A, B, B, delta_bias=dual(w[:, 0])),
+                     lambda: S.selective_scan(x, x, A, B, B, state=dual(h)),
+                     lambda: S.add_rms_norm_q8(dual(x), w[:, 0]), lambda: S.quantize_rows(dual(x)),
+                     lambda: S.matmul_i8(i8, dual(w[:2, 0]), i8, w[:2, 0]), lambda: S.causal_conv_step(x[:, 0], dual(x), w),
+                     lambda: S.selective_scan_step(dual(x[:, 0]), h, x[:, 0], A, B[:, 0], B[:, 0]),
+                     lambda: S.selective_scan_step(x[:, 0], dual(h), x[:, 0], A, B[:, 0], B[:, 0])):
+            for mode in (torch.enable_grad, torch.no_grad):   # (forward mode does not ask for either)
+                with mode(), pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                    call()
+        with pytest.raises(ValueError, match="no CPU path"):      # a dual level by itself is nothing to refuse
+            S.add_rms_norm(x, w[:, 0])
+    with pytest.raises(ValueError, match="no CPU path"):
+        S.quantize_rows(x)

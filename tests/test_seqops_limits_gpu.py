@@ -491,3 +491,21 @@ def test_a_start_whose_decay_outgrows_fp32(S, dtype, L, N):
         ro, rl, eo, el = plain_scan(one)
         P.close(y[:, None], ro, eo, 1, "out")
         P.close(h, rl, el, 1, "state")
+
+
+# ---------------------------------------------------------------------------------- forward mode
+def test_tangents_are_refused_back_as_well(S):
+    import torch.autograd.forward_ad as fwad
+    x, w, A, B = dev(Draw(1)(2, 9, 16), True), torch.ones(16, 4, device="cuda"), -torch.ones(16, 4, device="cuda"), dev(Draw(2)(2, 9, 4))
+    outs = [S.add_rms_norm(x, w[:, 0])[0], S.add_rms_norm(x, w[:, 0], x)[1], S.causal_conv(x, w)[0], S.selective_scan(x, x, A, B, B)[0]]
+    with fwad.dual_level():
+        for y in outs:
+            dy = fwad.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                torch.autograd.grad(y, x, dy)
+        d = fwad.make_dual(x.detach(), torch.ones_like(x))
+        for call in (lambda: S.add_rms_norm(d, w[:, 0]), lambda: S.causal_conv(d, w), lambda: S.selective_scan(d, x, A, B, B)):
+            with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                call()
+        with torch.inference_mode():      # where torch itself goes without tangents
+            assert torch.equal(S.add_rms_norm(d, w[:, 0])[0], S.add_rms_norm(x, w[:, 0])[0])
