@@ -60,18 +60,19 @@ class _Block(nn.Module):
             u, z = self.in_proj(y).chunk(2, dim=-1)
         else:
             y, scale, stream = seqops.add_rms_norm_q8(h, self.norm, stream)
-            u, z = seqops.matmul_i8(y, scale, *q["in_proj"]).chunk(2, dim=-1)
+            u, z = seqops.matmul_i8(y, scale, *q["in_proj"], out_dtype=h.dtype).chunk(2, dim=-1)
         u = seqops.causal_conv_step(u, conv, self.conv_weight, self.conv_bias, activation="silu", reset=reset)
-        x_dbl = self.x_proj(u) if q is None else seqops.matmul_i8(*seqops.quantize_rows(u), *q["x_proj"])
+        x_dbl = self.x_proj(u) if q is None else seqops.matmul_i8(*seqops.quantize_rows(u), *q["x_proj"], out_dtype=u.dtype)
         delta, A, B, C = self._scan_inputs(x_dbl)
         o = seqops.selective_scan_step(u, ssm, delta, A, B, C, D=self.D, z=z, delta_bias=self.dt_bias, reset=reset)
-        h = self.out_proj(o) if q is None else seqops.matmul_i8(*seqops.quantize_rows(o), *q["out_proj"])
+        h = self.out_proj(o) if q is None else seqops.matmul_i8(*seqops.quantize_rows(o), *q["out_proj"], out_dtype=o.dtype)
         return h, stream
 
 
 class HistoryEncoder(nn.Module):
     """in_dim values a token -> dim features; ``layers`` blocks of ``expand * dim`` channels, ``state`` states a
-    channel (up to 64), a convolution over ``width`` tokens (2 to 4).  Runs on a HIP device only."""
+    channel (up to 64), a convolution over ``width`` tokens (2 to 4).  Runs on a HIP device only, in its
+    parameters' type (fp32, or ``.to(torch.bfloat16)`` / fp16: inputs and features are of that type then)."""
 
     def __init__(self, in_dim, dim=256, layers=1, state=16, width=4, expand=2, dt_rank=None):
         super().__init__()
