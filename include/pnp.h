@@ -569,7 +569,8 @@ int32_t pnp_quantize_rows(const void* x, int64_t x_stride, int32_t type, int64_t
                           int64_t q_stride, float* scale, void* stream);
 
 /* out[m][n] = (sum_k q[m][k] * wq[n][k]) * scale[m] * wscale[n] + bias[n] (bias may be NULL), the sum
- * in 32-bit integers: exact for K <= 131071. */
+ * in 32-bit integers: exact for K <= 131071.  M up to 2^31, N up to 2^24, and fewer than 2^23 tiles of
+ * 256 x 256 outputs. */
 typedef struct pnp_i8_desc {
   int64_t M;
   int32_t N, K, out_type, pad;

@@ -365,7 +365,9 @@ extern "C" int32_t pnp_matmul_i8(const pnp_i8_desc* d, void* stream) {
     pnp_set_error("%s: bad shape or type", fn);
     return PNP_ERR_ARG;
   }
-  if (ceil_div(d->M, 64) * ceil_div(d->N, 64) >= ((int64_t)1 << 23)) {
+  // a launch holds fewer than 2^32 threads: 512 a tile of 256 x 256, which is what so many outputs go by (the smaller
+  // tiles serve below 192 of these, the kernel for few tokens at most N / 16 workgroups of 256)
+  if (d->M > 64 && ceil_div(d->M, 256) * ceil_div(d->N, 256) >= ((int64_t)1 << 23)) {
     pnp_set_error("%s: too many tiles for one launch", fn);
     return PNP_ERR_ARG;
   }

@@ -101,7 +101,8 @@ def quantize_rows(x):
 def matmul_i8(q, scale, wq, wscale, bias=None, out_dtype=torch.float32):
     """``out[..., n] = sum_k q[..., k] wq[n, k] * scale[...] * wscale[n] + bias[n]``: q [..., K] and wq
     [N, K] in int8, the sum exact (32-bit integers; K up to 131071), scaled in fp32 and rounded once to
-    ``out_dtype``.  For serving: no gradient."""
+    ``out_dtype``.  Up to 2^31 rows of q, N up to 2^24, and fewer than 2^23 tiles of 256 x 256 outputs; past
+    these a ``PnpError``.  For serving: no gradient."""
     return _ext.matmul_i8(q, scale, wq, wscale, bias, out_dtype)
 
 

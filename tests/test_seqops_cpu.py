@@ -267,3 +267,13 @@ def test_forward_mode_derivatives_are_refused():
             S.add_rms_norm(x, w[:, 0])
     with pytest.raises(ValueError, match="no CPU path"):
         S.quantize_rows(x)
+
+
+def test_c_product_refuses_more_tiles_than_a_launch_holds():
+    from pnp_amd import _lib
+    L = _lib.load()
+    d = _i8()
+    d.M, d.N = 1 << 31, 257          # 2^23 * 2 tiles
+    assert L.pnp_matmul_i8(C.byref(d), None) == -1 and b"too many tiles" in L.pnp_last_error()
+    d.N = 1
+    assert L.pnp_matmul_i8(C.byref(d), None) == -1 and b"too many tiles" in L.pnp_last_error()

@@ -509,3 +509,19 @@ def test_tangents_are_refused_back_as_well(S):
                 call()
         with torch.inference_mode():      # where torch itself goes without tangents
             assert torch.equal(S.add_rms_norm(d, w[:, 0])[0], S.add_rms_norm(x, w[:, 0])[0])
+
+
+# ---------------------------------------------------------------------------------- sizes of one launch
+def test_a_product_of_more_tokens_than_small_tiles_would_serve(S):
+    """2^29 + 5 tokens: past 2^23 tiles of 64 x 64, which nothing uses at this size."""
+    if torch.cuda.get_device_properties(0).total_memory < 200e9:
+        pytest.skip("needs a device with more than 200 GB")
+    M, K = 2 ** 29 + 5, 16
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randint(-128, 128, (M, K), generator=g, dtype=torch.int8, device="cuda")
+    w = torch.randint(-128, 128, (3, K), generator=g, dtype=torch.int8, device="cuda")
+    out = S.matmul_i8(q, torch.ones(M, device="cuda"), w, torch.ones(3, device="cuda"))
+    for part in (slice(0, END), slice(2 ** 28 - 7, 2 ** 28 + 300), slice(M - END, M)):
+        assert torch.equal(out[part].double(), q[part].double() @ w.double().t().contiguous())
+    del q, out
+    torch.cuda.empty_cache()
