@@ -585,7 +585,8 @@ int32_t pnp_matmul_i8(const pnp_i8_desc* d, void* stream);
  * sigmoid(pre) where silu).  Tokens before t = 0 come from state [B][W - 1][dim] (type `type`, zeros
  * where NULL).  starts [B][L] (bytes, may be NULL): a token with a nonzero start begins a sequence, it
  * and what follows see nothing from before it.  last_state [B][W - 1][dim] (may be NULL): the last
- * W - 1 tokens of the sequence that goes on, zeros before its start.  W 2, 3 or 4. */
+ * W - 1 tokens of the sequence that goes on, zeros before its start.  W 2, 3 or 4; B and L up to 2^31; calls with
+ * B * ceil(L / 8) * dim below 2^32 fit a launch, larger ones may be refused. */
 typedef struct pnp_conv_desc {
   int64_t B, L;
   int32_t dim, width, type, silu;
@@ -622,8 +623,10 @@ int32_t pnp_causal_conv_step(const void* x, int64_t x_stride, void* state, const
  * h[t] = a * h[t - 1] + dt * u * Bm[b][t][g][n]; y = sum_n Cm[b][t][g][n] * h + D[d] * u;
  * out = y * z * sigmoid(z) (y where z is NULL).  Channel d belongs to group g = d / (dim / groups).
  * h before t = 0: state [B][dim][N] (zeros where NULL); last_state the h after the last token.
- * N 1 .. 64; token strides up to PNP_SCAN_MAX_TSTRIDE elements.  ckpt (may be NULL; pnp_scan_ckpt_floats): the states the gradient starts its pieces
- * from.  workspace (pnp_scan_workspace floats) serves the split over the length. */
+ * N 1 .. 64; token strides up to PNP_SCAN_MAX_TSTRIDE elements; B and L up to 2^31, and
+ * B * groups * ceil(dim / groups / C) below 2^24, C = 256, 128, 64, 32, 16 channels for N up to 4, 8, 16, 32, 64
+ * (the gradient: dim * (N + 2) below 2^28 too).  ckpt (may be NULL; pnp_scan_ckpt_floats): the states the gradient starts
+ * its pieces from.  workspace (pnp_scan_workspace floats) serves the split over the length. */
 #define PNP_SCAN_MAX_TSTRIDE (1 << 24)
 typedef struct pnp_scan_desc {
   int64_t B, L;

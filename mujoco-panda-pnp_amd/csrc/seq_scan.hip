@@ -920,6 +920,7 @@ bool bc_even(const ScanArgs& a, int bytes) {
     __VA_ARGS__;                                              \
   }()
 
+// (a length is cut in chunks below 512 workgroups only, of 256 / S channels each: 2^19 threads at most)
 int32_t chain(const ScanArgs& a, const float* first, int S, int back, hipStream_t st) {
   const int64_t n = a.B * a.dim * 4 * S;
   hipLaunchKernelGGL(scan_chain_kernel, dim3((unsigned)ceil_div(n, NT)), dim3(NT), 0, st, a, first, 4 * S, back);
@@ -1027,7 +1028,7 @@ static int32_t scan_check(const pnp_scan_desc* d, const Plan& p, const char* fn)
     pnp_set_error("%s: null buffer", fn);
     return PNP_ERR_ARG;
   }
-  if (p.blocks >= (1 << 24) || d->B * (int64_t)d->dim * p.S >= ((int64_t)1 << 30)) {
+  if (p.blocks >= (1 << 24)) {   // (a launch holds fewer than 2^32 threads)
     pnp_set_error("%s: too many sequences for one launch", fn);
     return PNP_ERR_ARG;
   }

@@ -111,7 +111,8 @@ def causal_conv(x, weight, bias=None, activation=None, starts=None, state=None):
     ``pre * sigmoid(pre)`` where ``activation`` is "silu"; x [B, L, D].  What lies before t = 0 comes from
     ``state`` [B, W - 1, D] (x's type; zeros without one).  Returns ``(y, last_state)``: the last W - 1
     tokens of the sequence that goes on (zeros before its start), for the next call or for
-    ``causal_conv_step``.  ``starts``: see the module's text."""
+    ``causal_conv_step``.  ``starts``: see the module's text.  One launch: calls with B * ceil(L / 8) * D below
+    2^32 always fit; one that does not is a ``PnpError``."""
     return _ext.causal_conv(x, weight, bias, activation, starts, state)
 
 
@@ -128,7 +129,9 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, starts=No
     [B, L, N], or [B, L, groups, N] where each ``dim / groups`` neighbouring channels share a group; D and
     delta_bias [dim].  h before t = 0 is ``state`` [B, dim, N] in fp32 (zeros without one).  Returns
     ``(out, last_state)``, the state in fp32 for the next call or for ``selective_scan_step``.
-    ``starts``: see the module's text."""
+    ``starts``: see the module's text.  One launch: B * groups * ceil(dim / groups / C) below 2^24, with C 256,
+    128, 64, 32, 16 for N up to 4, 8, 16, 32, 64, and dim * (N + 2) below 2^28 with a gradient; past these a
+    ``PnpError``."""
     return _ext.selective_scan(u, delta, A, B, C, D, z, delta_bias, starts, state)
 
 

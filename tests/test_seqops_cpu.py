@@ -277,3 +277,12 @@ def test_c_product_refuses_more_tiles_than_a_launch_holds():
     assert L.pnp_matmul_i8(C.byref(d), None) == -1 and b"too many tiles" in L.pnp_last_error()
     d.N = 1
     assert L.pnp_matmul_i8(C.byref(d), None) == -1 and b"too many tiles" in L.pnp_last_error()
+
+
+def test_c_scan_refuses_more_sequences_than_a_launch_holds():
+    from pnp_amd import _lib
+    L = _lib.load()
+    d = _scan()
+    for B, dim, N, groups in ((1 << 24, 8, 16, 1), (1 << 23, 16, 16, 2), (1 << 20, 257 * 8, 64, 1), (1 << 20, 16, 1, 16)):
+        d.B, d.dim, d.N, d.groups = B, dim, N, groups
+        assert L.pnp_selective_scan(C.byref(d), None) == -1 and b"too many sequences" in L.pnp_last_error()

@@ -525,3 +525,23 @@ def test_a_product_of_more_tokens_than_small_tiles_would_serve(S):
         assert torch.equal(out[part].double(), q[part].double() @ w.double().t().contiguous())
     del q, out
     torch.cuda.empty_cache()
+
+
+def test_a_scan_of_more_states_than_a_chain_would_serve(S):
+    """2^17 + 5 sequences of one token, 2048 channels, 16 states: 2^30 lanes of 4 states; no chunks, so nothing is chained."""
+    if torch.cuda.get_device_properties(0).total_memory < 200e9:
+        pytest.skip("needs a device with more than 200 GB")
+    n, d = 2 ** 17 + 5, 2048
+    torch.manual_seed(2)
+    x, B, A = torch.randn(n, 1, d, device="cuda", dtype=BF), torch.randn(n, 1, 16, device="cuda", dtype=BF), -torch.rand(d, 16, device="cuda")
+
+    def run(x, B):
+        x, B = x.detach().requires_grad_(), B.detach().requires_grad_()
+        y, last = S.selective_scan(x, x, A, B, B, z=x)
+        return [t[-END:].clone() for t in (y.detach(), last.detach(), *torch.autograd.grad(y, [x, B], x.detach()))]
+
+    got = run(x, B)
+    torch.cuda.empty_cache()
+    for a, b in zip(got, run(x[-END:], B[-END:])):      # (the same kernels: a sequence's arithmetic is its own)
+        assert torch.equal(a, b)
+    torch.cuda.empty_cache()
