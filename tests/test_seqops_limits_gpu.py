@@ -545,3 +545,22 @@ def test_a_scan_of_more_states_than_a_chain_would_serve(S):
     for a, b in zip(got, run(x[-END:], B[-END:])):      # (the same kernels: a sequence's arithmetic is its own)
         assert torch.equal(a, b)
     torch.cuda.empty_cache()
+
+
+# ---------------------------------------------------------------------------------- the product's largest tiles
+@pytest.mark.parametrize("dtype", T.TYPES, ids=T.ids)
+@pytest.mark.parametrize("M,N", [(3600, 3600), (6001, 2050), (2049, 5384)])
+@pytest.mark.parametrize("K", [16, 64, 80, 128, 192, 208, 256, 320, 1040])
+def test_products_of_large_tiles_over_many_stages(S, dtype, M, N, K):
+    """Rows on 16-byte boundaries, 192 tiles of 256 x 256 and more; every element, whole and partial last stages.  Roundings:
+    the sum's in fp32, two products, the bias's addition."""
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    q, w = (torch.randint(-128, 128, (n, K), generator=g, dtype=torch.int8, device="cuda") for n in (M, N))
+    s, ws, b = (torch.rand(n, generator=g, device="cuda") + 0.01 for n in (M, N, N))
+    if dtype == torch.float16:
+        s = s * 2.0 ** -12      # (sums of 16 million would overflow half precision)
+    out = S.matmul_i8(q, s, w, ws, bias=b, out_dtype=dtype).double()
+    scaled = q.double() @ w.double().t().contiguous() * s.double()[:, None] * ws.double()
+    slack = 4 * P.E32 * (scaled.abs() + b.double())
+    ref = scaled + b.double()
+    assert ((out - ref).abs() <= slack + P.STEP[dtype] * (ref.abs() + slack) + P.TINY[dtype]).all()
