@@ -286,3 +286,13 @@ def test_c_scan_refuses_more_sequences_than_a_launch_holds():
     for B, dim, N, groups in ((1 << 24, 8, 16, 1), (1 << 23, 16, 16, 2), (1 << 20, 257 * 8, 64, 1), (1 << 20, 16, 1, 16)):
         d.B, d.dim, d.N, d.groups = B, dim, N, groups
         assert L.pnp_selective_scan(C.byref(d), None) == -1 and b"too many sequences" in L.pnp_last_error()
+
+
+# ---------------------------------------------------------------------------------- build
+@pytest.mark.skipif(shutil.which("make") is None, reason="needs make")
+def test_objects_are_built_anew_where_their_flags_change():
+    """The Makefile holds the compiler's flags: objects of others must not be linked."""
+    csrc = os.path.join(ROOT, "mujoco-panda-pnp_amd", "csrc")
+    plan = subprocess.run(["make", "-n", "-W", "Makefile", "-C", csrc], check=True, capture_output=True, text=True).stdout
+    for unit in ("seq_norm.hip", "seq_scan.hip", "tqc_fused.hip", "step.hip", "ik_dls.hip", "resident.cpp", "seq_torch.cpp"):
+        assert unit in plan, unit
