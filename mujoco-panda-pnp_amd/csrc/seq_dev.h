@@ -57,8 +57,9 @@ template <typename T> __device__ __forceinline__ T* at(void* p, int64_t elems, u
   return (T*)(SEQ_GLOBAL T*)((SEQ_GLOBAL char*)base + bytes);
 }
 
-// sigmoid by the hardware's exp2 and reciprocal: 1 / (1 + 2^(-x log2 e)), relative error a few 2^-24;
-// x -> -inf gives 1 / inf = 0, x -> inf 1
+// sigmoid by the hardware's exp2 and reciprocal: 1 / (1 + 2^(-x log2 e)); x -> -inf gives 1 / inf = 0, x -> inf 1.
+// Relative error in steps of 2^-24: for x < 0 about |x| + 3 (exp2 turns the rounding of its argument, |x| log2 e steps,
+// into |x|), for x > 0 about 2, and the hardware's exp2 and reciprocal, a unit each.
 __device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
 #define SEQ_LOG2E 1.44269504088896340736f
 __device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rcpf(1.f + exp2_f(-SEQ_LOG2E * x)); }
@@ -66,7 +67,8 @@ __device__ __forceinline__ float sigmoid_f(float x) { return __builtin_amdgcn_rc
 // softplus(x) = max(x, 0) + log(1 + e) with e = exp(-|x|) in (0, 1]: no overflow.  The logarithm as
 // log(1 + e) = 2 atanh(s), s = e / (2 + e) <= 1 / 3: relative accuracy for small results too (log of the
 // rounded 1 + e would lose it: at x = -10 to 1e-3).  atanh(s) / s is a polynomial in s^2, fitted to the
-// least largest relative error on [0, 1/9] (4e-9); in all within 5 steps of 2^-24 of the function.
+// least largest relative error on [0, 1/9] (4e-9).  In all, in steps of 2^-24 of the function: for x < 0
+// about |x| + 5 (as the sigmoid), for x > 0 about 4, and the hardware's exp2 and reciprocal.
 __device__ __forceinline__ float softplus_f(float x) {
   const float e = exp2_f(-SEQ_LOG2E * fabsf(x));
   const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
