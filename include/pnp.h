@@ -518,7 +518,7 @@ int32_t pnp_env_evaluate_f64(pnp_model* model, const pnp_state_f64* state, const
  *
  * `type` of a tensor: PNP_F32, PNP_BF16 or PNP_F16.  Tensors are device memory of the current
  * device, the last dimension contiguous; `*_stride` fields are in elements, outputs without one
- * are contiguous and overlap no input (but a step's state, advanced in place).  Weights, biases, states, statistics and sums are fp32 whatever `type` is.  An
+ * are contiguous and overlap no input (but a step's state, advanced in place, which no other input overlaps).  Weights, biases, states, statistics and sums are fp32 whatever `type` is.  An
  * empty batch is PNP_OK and launches nothing.  Workspaces belong to the caller: one call's
  * workspace is free again when the call's work on its stream is done.  No atomics: the same call
  * gives the same bits. */

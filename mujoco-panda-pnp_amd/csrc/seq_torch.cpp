@@ -123,6 +123,19 @@ void advanced(const Tensor& state) {
   if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
 }
 
+// an input of a call that advances `state` in place, copied first where the two share memory: some of the call's
+// workgroups may read it after others have written
+Tensor apart(const Tensor& t, const Tensor& state) {
+  if (!t.defined() || !t.numel() || !state.numel() || !t.is_alias_of(state)) return t;
+  const auto end = [](const Tensor& v) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < v.dim(); i++) last += (v.size(i) - 1) * v.stride(i);
+    return (const char*)v.const_data_ptr() + (last + 1) * (int64_t)v.element_size();
+  };
+  const bool meet = (const char*)t.const_data_ptr() < end(state) && (const char*)state.const_data_ptr() < end(t);
+  return meet ? t.clone(at::MemoryFormat::Contiguous) : t;
+}
+
 // autograd nodes take what may be missing as an optional (an undefined tensor among their inputs is an error)
 MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
 Tensor value(const MaybeTensor& t) { return t ? *t : Tensor(); }
@@ -452,8 +465,9 @@ Tensor causal_conv_step(const Tensor& x_, const Tensor& state, const Tensor& wei
   activation(state, "state", &x_);
   shaped(state, "state", {x_.size(0), w.size(1) - 1, x_.size(1)});
   in_place(state);
-  const Tensor reset = marks(reset_, "reset", x_.sizes().slice(0, 1), x_), x = lines(x_), y = fresh(x.sizes(), x.scalar_type(), x);
-  CALL(causal_conv_step, x, cptr(x), x.stride(0), mptr(state), cfloat(w), cfloat(b), cbyte(reset), x.size(0), (int32_t)x.size(1),
+  const Tensor reset = apart(marks(reset_, "reset", x_.sizes().slice(0, 1), x_), state), x = apart(lines(x_), state);
+  const Tensor wa = apart(w, state), ba = apart(b, state), y = fresh(x.sizes(), x.scalar_type(), x);
+  CALL(causal_conv_step, x, cptr(x), x.stride(0), mptr(state), cfloat(wa), cfloat(ba), cbyte(reset), x.size(0), (int32_t)x.size(1),
        (int32_t)w.size(1), code_of(x.scalar_type()), (int32_t)silu, mptr(y));
   advanced(state);
   return y;
@@ -602,10 +616,11 @@ std::tuple<Tensor, Tensor> selective_scan(const Tensor& u, const Tensor& delta, 
 Tensor selective_scan_step(const Tensor& u, const Tensor& state, const Tensor& delta, const Tensor& A, const Tensor& B, const Tensor& C,
                            const MaybeTensor& D, const MaybeTensor& z, const MaybeTensor& bias, const MaybeTensor& reset_) {
   serving("selective_scan_step", u, state, delta, A, B, C, D, z, bias);
-  const ScanIn v = scan_in(u, delta, A, B, C, D, z, bias, 1);
+  ScanIn v = scan_in(u, delta, A, B, C, D, z, bias, 1);
   state32(state, {u.size(0), u.size(1), A.size(1)}, u);
   in_place(state);
-  const Tensor reset = marks(reset_, "reset", u.sizes().slice(0, 1), u), out = fresh(u.sizes(), u.scalar_type(), u);
+  for (Tensor* t : {&v.u, &v.delta, &v.A, &v.B, &v.C, &v.D, &v.z, &v.bias}) *t = apart(*t, state);
+  const Tensor reset = apart(marks(reset_, "reset", u.sizes().slice(0, 1), u), state), out = fresh(u.sizes(), u.scalar_type(), u);
   pnp_scan_desc d = scan_desc(v, reset, state, true);
   d.out = mptr(out); d.last_state = mfloat(state);
   CALL(selective_scan_step, u, &d);

@@ -118,8 +118,8 @@ def causal_conv(x, weight, bias=None, activation=None, starts=None, state=None):
 
 def causal_conv_step(x, state, weight, bias=None, activation=None, reset=None):
     """One token of each of B sequences: x [B, D] -> y [B, D], ``state`` [B, W - 1, D] (contiguous, x's
-    type) advanced in place.  ``reset`` [B] (uint8 or bool) nonzero: that sequence begins at this token.
-    For serving: no gradient."""
+    type) advanced in place (inputs that lie in it are copied first).  ``reset`` [B] (uint8 or bool) nonzero: that
+    sequence begins at this token.  For serving: no gradient."""
     return _ext.causal_conv_step(x, state, weight, bias, activation, reset)
 
 
@@ -137,6 +137,6 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, starts=No
 
 def selective_scan_step(u, state, delta, A, B, C, D=None, z=None, delta_bias=None, reset=None):
     """One token of each of B sequences: u, delta, z [B, dim], B, C [B, N] or [B, groups, N] -> out [B, dim],
-    ``state`` [B, dim, N] (fp32, contiguous) advanced in place.  ``reset`` [B] (uint8 or bool) nonzero: that
-    sequence begins at this token.  For serving: no gradient."""
+    ``state`` [B, dim, N] (fp32, contiguous) advanced in place (inputs that lie in it are copied first).
+    ``reset`` [B] (uint8 or bool) nonzero: that sequence begins at this token.  For serving: no gradient."""
     return _ext.selective_scan_step(u, state, delta, A, B, C, D, z, delta_bias, reset)

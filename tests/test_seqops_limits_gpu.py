@@ -564,3 +564,29 @@ def test_products_of_large_tiles_over_many_stages(S, dtype, M, N, K):
     slack = 4 * P.E32 * (scaled.abs() + b.double())
     ref = scaled + b.double()
     assert ((out - ref).abs() <= slack + P.STEP[dtype] * (ref.abs() + slack) + P.TINY[dtype]).all()
+
+
+# ---------------------------------------------------------------------------------- a step's inputs in its state
+def test_steps_whose_inputs_lie_in_their_state(S):
+    """Views of the state that a step advances in place, as its inputs: what they held before the call."""
+    d = Draw(12)
+    n, dim, N = 300, 520, 16
+    state, w = dev(d(n, 3, dim)), dev(d(dim, 4))
+    flat = state.view(n, -1)
+    for x in (flat[:, 7:7 + dim], flat[:, 1030:1030 + dim], state[:, 2], flat[:1, :dim].expand(n, dim)):
+        want_state, want_x = state.clone(), x.clone()
+        held = state.clone()
+        want = S.causal_conv_step(want_x, want_state, w)
+        assert torch.equal(S.causal_conv_step(x, state, w), want) and torch.equal(state, want_state)
+        state.copy_(held)
+    h, A, B, u = dev(d(n, dim, N)), -dev(d(dim, N).abs()), dev(d(n, N)), dev(d(n, dim))
+    flat = h.view(n, -1)
+    for v in (dict(u=flat[:, 100:100 + dim]), dict(B=h[:, 5], C=h[:, dim - 1]), dict(A=h[n - 1]), dict(delta=flat[:, -dim:], z=flat[:, :dim]),
+              dict(D=flat[3, :dim], B=h[:1, 0].expand(n, N))):
+        held = h.clone()
+        call = lambda h, v: S.selective_scan_step(v.get("u", u), h, v.get("delta", u), v.get("A", A), v.get("B", B), v.get("C", B),   # noqa: E731
+                                                  D=v.get("D"), z=v.get("z"))
+        want_h = h.clone()
+        want = call(want_h, {k: t.clone() for k, t in v.items()})
+        assert torch.equal(call(h, v), want) and torch.equal(h, want_h), v.keys()
+        h.copy_(held)
