@@ -162,6 +162,8 @@ struct ConvBwdArgs {
 //
 // Four channels a lane: with eight the filters and sums spill (bf16, 2 x 8191 x 2048: 125 against 59 us).  The tokens
 // within a run and its sequence go without the questions that the run's ends ask (59 -> 49 us, 201 MB at 4.1 TB/s).
+// Channels that are no multiple of 4, one a lane, with the weights' sums: bf16, 2 x 4096 x 2047, 40 us, x 2048 29 and x 2044
+// (by fours, rows across lines) 37.
 template <typename T, int W, int V> __global__ __launch_bounds__(NT, 2) void conv_bwd_kernel(ConvBwdArgs a) {
   const ConvArgs& f = a.f;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // (a wave's run, its marks and its age are scalars)

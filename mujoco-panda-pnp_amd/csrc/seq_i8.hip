@@ -136,8 +136,9 @@ __device__ __forceinline__ int k_of(int g) { return g == 0 ? 0 : g == 1 ? 3 : g 
 // and its buffer is loaded anew, ST stages on, as soon as everybody has.  Otherwise two stages, by way of
 // registers that hold the next two.
 //
-// Bound by the matrix cores at the clock that the power leaves them: 8192^3 460 us, 2.4 POP/s (a large bf16 library
-// product reaches 1.2 PFLOP/s here; the matrix cores are busy in 65 % of the cycles).  Short sums by their output:
+// Bound by the matrix cores and the clock that the card's power leaves them: 8192^3 450 to 550 us from run to run, 2.4 to
+// 2.0 POP/s (the library's int8 product 533 us).  They are busy in 65 % of the cycles; a wave waits in 29 % of its own,
+// for LDS and at the stages' barriers.  Short sums by their output:
 // 8192 x 1024 x 256 11 us, of which a launch of one tile 4.5 and the writing of 17 MB about 5.
 __device__ const v4i zeros[1] = {};
 
@@ -282,8 +283,9 @@ __global__ __launch_bounds__(64 * WGM* WGN, 2) void i8_tile_kernel(I8Args a) {
 // Few tokens (16 MT at most): the weights' bytes are what counts.  A workgroup has 16 channels, its 4 waves stages of k
 // in turn, straight from memory to registers; their sums meet in LDS.  A wave takes two stages that lie together, whole
 // lines of the weights (by single stages, half lines: one token by 4096 x 4096 10.7 against 7.4 us, 64 tokens 25 against
-// 15).  One token by 1000 x 512 5 us and by 4096 x 4096 7.4, of which a launch in a row of them 4.5; by 16384 x 8192
-// 24 us, 5.6 TB/s.
+// 15).  One token by 1000 x 512 5 us and by 4096 x 4096 7.0, of which a launch in a row of them 4.5; by 16384 x 8192
+// 24 us, 5.6 TB/s.  16, 33 and 64 tokens by 4096 x 4096 7.8, 13 and 15 us: N / 16 workgroups are one a CU, and each wave
+// waits for its own loads.
 template <typename T, int MT> __global__ __launch_bounds__(256) void i8_rows_kernel(I8Args a) {
   __shared__ v4i part[3][MT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fc = lane >> 4;

@@ -15,9 +15,10 @@
 // the last one moved back to end with the row.  Its first elements are another lane's too: written
 // twice, the same value, and counted once.
 //
-// Measured, with a residual: bf16, 8192 x 4096, 42 us forward (268 MB, 6.3 TB/s: part of it from cache), 57 back
-// (336 MB); 16384 x 4096 both in 210 us (1.07 GB at 5.1 TB/s, a large copy's rate); rows of 4095 46 and 60 us (by
-// elements 96 and 167); 200000 rows of 64 19 us (by whole waves 61).
+// Measured, with a residual: bf16, 8192 x 4096, 42 us forward (268 MB, 6.3 TB/s: part of it from cache), 63 back with
+// the weight's sums (336 MB); 16384 x 4096 both in 210 us (1.07 GB at 5.1 TB/s, a large copy's rate); rows of 4095 45
+// and 89 us, of 4100 54 and 100 (by elements, of 4095, 96 and 167); 200000 rows of 64 19 and 23 us (by whole waves 61
+// forward).
 #include <type_traits>
 
 #include "seq_dev.h"
